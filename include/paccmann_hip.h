@@ -37,6 +37,8 @@ extern "C" {
 
 /* bits of the int32 status word a forward call leaves on the device */
 #define PCM_STATUS_BAD_TOKEN 1 /* a token id outside [0, vocab) was clamped */
+#define PCM_STATUS_BAD_PARENT 4 /* a beam's parent outside [0, beams): its rows
+                                  were left as they were */
 #define PCM_STATUS_TIMEOUT 2   /* a hand-off inside the persistent forward kernel
                                   gave up (its blocks were not all resident):
                                   the call's outputs are not valid */
@@ -404,6 +406,149 @@ int pcm_stackgru_generate_beam(const pcm_dims *dims,
                                double *beam_scores_out, void *workspace,
                                size_t workspace_bytes, int32_t *status,
                                void *stream);
+
+/* Top logits, distillation, joint beam search -----------------------------------*/
+
+/* element types of logits that these calls take besides fp32 */
+#define PCM_DTYPE_F32 0
+#define PCM_DTYPE_BF16 1
+#define PCM_DTYPE_F16 2
+
+#define PCM_TOP_MAX 64          /* longest list of top logits                  */
+#define PCM_BEAM_MAX 16         /* most beams                                  */
+#define PCM_MAX_VOCAB (1 << 18) /* longest row of these calls                  */
+
+/*
+ * The k largest logits of every row, largest first (equal ones: lowest index
+ * first), and the log-sum-exp of the others at a temperature:
+ *   rest[r] = log sum_{v not listed} exp(logits[r][v] / temperature)
+ * (-inf where nothing is left).  The reference has no distillation; this is
+ * what a teacher writes for pcm_distill_loss.
+ *
+ *   logits   [rows] rows of `vocab` elements of `dtype`, row stride ld elements
+ *   k        1 .. min(vocab, PCM_TOP_MAX)
+ *   values   [rows][k] of `dtype`, exact;  indices int32[rows][k]
+ *   rest     fp32[rows]
+ *   A NaN ranks below every number and makes the row's rest NaN.
+ */
+size_t pcm_top_logits_workspace_bytes(int64_t rows, int32_t vocab, int32_t k);
+int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
+                   int32_t vocab, int32_t k, double temperature, void *values,
+                   int32_t *indices, float *rest, void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/*
+ * Distillation from a teacher's top logits, and the gradient.  Both models are
+ * compared over k + 1 outcomes: the k listed tokens and "any other token".
+ * With u_j = values_j / temperature, teacher p_j = exp(u_j - N) and
+ * p_rest = exp(rest - N), N = log(sum_j exp(u_j) + exp(rest)); the student's
+ * q comes from x = logits / temperature over the whole vocabulary, q_rest
+ * summed over the tokens that are not listed.
+ *   row  = (1 - hard) temperature^2 sum p (log p - log q)
+ *          + hard * cross entropy(logits, target)
+ *   loss = sum_t weight_t sum_b row(t, b)
+ * over the rows with lengths[b] > t; weight_t = step_weight[t], or one over the
+ * number of those rows (as pcm_softmax_ce).
+ *
+ *   logits   [T*B] rows (t * B + b) of `vocab` elements, row stride ld
+ *   values   [T*B][k] of values_dtype, indices int32[T*B][k]: a negative index
+ *            is an absent entry (its value is not read as one); an index
+ *            >= vocab counts as absent and raises PCM_STATUS_BAD_TOKEN; an index
+ *            that appears twice carries both probabilities
+ *   rest     fp32[T*B] at the same temperature, or NULL: the teacher gives the
+ *            other tokens no probability.  A row without any teacher
+ *            probability has no distillation term
+ *   targets  int64[T*B], needed when hard_weight > 0 (clamped like
+ *            pcm_softmax_ce's)
+ *   loss     fp32[1]; dlogits (nullable) [T*B][vocab] of `dtype`, dense: zero in
+ *            rows that take no part, whatever their logits hold
+ *   scratch  fp32[pcm_distill_scratch_floats(T, B)]
+ */
+size_t pcm_distill_scratch_floats(int32_t steps, int32_t batch);
+int pcm_distill_loss(const void *logits, int32_t dtype, int64_t ld,
+                     const void *values, int32_t values_dtype,
+                     const int32_t *indices, const float *rest, int32_t k,
+                     const int64_t *targets, const int32_t *lengths,
+                     const float *step_weight, int32_t steps, int32_t batch,
+                     int32_t vocab, double temperature, double hard_weight,
+                     float *loss, void *dlogits, float *scratch,
+                     int32_t *status, void *stream);
+/* x[i] *= scale[0] (a device scalar); leaves x alone when it is 1. */
+int pcm_scale(void *x, int32_t dtype, int64_t n, const float *scale,
+              void *stream);
+
+/*
+ * One selection of a beam search over beams AND vocabulary: the `width` best of
+ * the beams * vocab candidates
+ *   c[k][v] = scores[k][b] + logits[k][b][v] / temperature - lse[k][b]
+ * of every batch row b, best first, equal ones by lowest k * vocab + v.  Scores
+ * are carried, summed and compared in 64 bits.  (BeamSearch.step of the
+ * reference, utils/search.py:247-275, ranks top_tokens candidates per beam.)
+ *
+ *   logits   rows k * batch + b of `vocab` elements, row stride ld
+ *   scores   fp64[beams][batch]; -inf (or NaN) marks a slot that holds no beam:
+ *            all its candidates are -inf, as are those of a row of logits that
+ *            has no distribution (a NaN, a +inf, nothing above -inf)
+ *   finished uint8[beams][batch] (nullable; needs finished_out and
+ *            0 <= end_token < vocab): a finished beam has one candidate,
+ *            end_token at its own score; its logits are not read
+ *   tokens   int64[width][batch], parents int32[width][batch],
+ *   scores_out fp64[width][batch], finished_out uint8[width][batch]
+ *            (finished[parent], or the token is end_token)
+ *   1 <= beams, width <= PCM_BEAM_MAX and width <= beams * vocab.
+ */
+size_t pcm_beam_select_workspace_bytes(int32_t beams, int32_t batch,
+                                       int32_t vocab, int32_t width);
+int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
+                    const double *scores, const uint8_t *finished,
+                    int32_t beams, int32_t batch, int32_t vocab, int32_t width,
+                    double temperature, int32_t end_token, int64_t *tokens,
+                    int32_t *parents, double *scores_out,
+                    uint8_t *finished_out, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
+#define PCM_MAX_STATES 16
+/* One tensor whose rows belong to beams: element bytes of row r, outer index o
+ * at data + o * outer_stride + r * row_stride, row_bytes of them in one piece
+ * (strides in bytes). */
+typedef struct pcm_state {
+    void *data;
+    int64_t outer;        /* how many outer indices                         */
+    int64_t outer_stride;
+    int64_t row_stride;
+    int64_t row_bytes;
+} pcm_state;
+/*
+ * Lets the states follow their beams, in place: in every state, row
+ * k * batch + b becomes what row parents[k][b] * batch + b was.  No two rows
+ * and no two states may share memory.
+ *   parents  int32[beams][batch]; one outside [0, beams) leaves its rows as
+ *            they were and or-s PCM_STATUS_BAD_PARENT into *status (nullable)
+ */
+int pcm_reorder_states(const int32_t *parents, int32_t beams, int32_t batch,
+                       const pcm_state *states, int32_t count, int32_t *status,
+                       void *stream);
+
+size_t pcm_generate_joint_beam_workspace_bytes(const pcm_dims *dims,
+                                               int32_t beam_width,
+                                               int32_t generate_len);
+/*
+ * pcm_stackgru_generate_beam with the two calls above in place of the
+ * reference's step: every token is selected over beams and vocabulary, hidden
+ * states and stacks follow their beams, and with end_token >= 0 a beam that has
+ * produced it keeps its score and repeats it.
+ *   tokens_out int64[B, generate_len], beam_tokens_out int64[B, beam_width,
+ *   generate_len] (nullable) and beam_scores_out fp64[B, beam_width]
+ *   (nullable): best first, without the prime
+ */
+int pcm_stackgru_generate_joint_beam(
+    const pcm_dims *dims, const pcm_stackgru_params *weights,
+    const float *out_w, const float *out_b, const float *h0,
+    int64_t h0_layer_stride, const int64_t *prime, int32_t prime_len,
+    int32_t generate_len, int32_t beam_width, double temperature,
+    int32_t end_token, int64_t *tokens_out, int64_t *beam_tokens_out,
+    double *beam_scores_out, void *workspace, size_t workspace_bytes,
+    int32_t *status, void *stream);
 
 /* Optimiser ------------------------------------------------------------------*/
 

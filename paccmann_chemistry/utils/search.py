@@ -1,3 +1,3 @@
 from paccmann_chemistry_amd.search import (  # noqa: F401
-    BeamSearch, GreedySearch, SamplingSearch, Search
+    BeamSearch, GreedySearch, JointBeamSearch, SamplingSearch, Search
 )

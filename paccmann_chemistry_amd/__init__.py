@@ -13,8 +13,13 @@ Host-side mirror of the reference's module interface over libpaccmann_hip.so
 from .stack_rnn import StackGRU  # noqa: F401
 from .vae import StackGRUDecoder, StackGRUEncoder, TeacherVAE  # noqa: F401
 from .loss_functions import vae_loss_function  # noqa: F401
-from .search import BeamSearch, GreedySearch, SamplingSearch  # noqa: F401
+from .search import (  # noqa: F401
+    BeamSearch, GreedySearch, JointBeamSearch, SamplingSearch
+)
 from .ops import get_matmul_precision, set_matmul_precision  # noqa: F401
+from .ops import (  # noqa: F401
+    BeamStep, TopLogits, beam_select, distill_loss, reorder_states, top_logits
+)
 from .inference import encode_batches, generate_batches  # noqa: F401
 
 __version__ = '0.1.0'

@@ -20,6 +20,13 @@ SEARCH_GREEDY = 0
 SEARCH_SAMPLING = 1
 STATUS_BAD_TOKEN = 1
 STATUS_TIMEOUT = 2
+STATUS_BAD_PARENT = 4
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+TOP_MAX = 64
+BEAM_MAX = 16
+MAX_STATES = 16
+MAX_VOCAB = 1 << 18
 
 c_float_p = ctypes.c_void_p  # device pointers travel as plain addresses
 
@@ -45,8 +52,17 @@ class PcmStackGRUParams(ctypes.Structure):
     ]
 
 
+class PcmState(ctypes.Structure):
+    _fields_ = [
+        ('data', ctypes.c_void_p), ('outer', ctypes.c_int64),
+        ('outer_stride', ctypes.c_int64), ('row_stride', ctypes.c_int64),
+        ('row_bytes', ctypes.c_int64)
+    ]
+
+
 _I32, _I64, _U64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64
 _F32, _SZ, _VP = ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p
+_F64 = ctypes.c_double
 _DIMS_P = ctypes.POINTER(PcmDims)
 _PARAMS_P = ctypes.POINTER(PcmStackGRUParams)
 
@@ -139,6 +155,39 @@ PROTOTYPES = {
         ctypes.c_int, [
             _VP, _VP, _I32, _I32, _I32, _VP, _F32, _U64, _VP, _I64, _VP, _VP,
             _VP, _VP
+        ]
+    ),
+    'pcm_top_logits_workspace_bytes': (_SZ, [_I64, _I32, _I32]),
+    'pcm_top_logits': (
+        ctypes.c_int, [
+            _VP, _I32, _I64, _I64, _I32, _I32, _F64, _VP, _VP, _VP, _VP, _SZ,
+            _VP
+        ]
+    ),
+    'pcm_distill_scratch_floats': (_SZ, [_I32, _I32]),
+    'pcm_distill_loss': (
+        ctypes.c_int, [
+            _VP, _I32, _I64, _VP, _I32, _VP, _VP, _I32, _VP, _VP, _VP, _I32,
+            _I32, _I32, _F64, _F64, _VP, _VP, _VP, _VP, _VP
+        ]
+    ),
+    'pcm_scale': (ctypes.c_int, [_VP, _I32, _I64, _VP, _VP]),
+    'pcm_beam_select_workspace_bytes': (_SZ, [_I32, _I32, _I32, _I32]),
+    'pcm_beam_select': (
+        ctypes.c_int, [
+            _VP, _I32, _I64, _VP, _VP, _I32, _I32, _I32, _I32, _F64, _I32,
+            _VP, _VP, _VP, _VP, _VP, _SZ, _VP
+        ]
+    ),
+    'pcm_reorder_states': (
+        ctypes.c_int,
+        [_VP, _I32, _I32, ctypes.POINTER(PcmState), _I32, _VP, _VP]
+    ),
+    'pcm_generate_joint_beam_workspace_bytes': (_SZ, [_DIMS_P, _I32, _I32]),
+    'pcm_stackgru_generate_joint_beam': (
+        ctypes.c_int, [
+            _DIMS_P, _PARAMS_P, _VP, _VP, _VP, _I64, _VP, _I32, _I32, _I32,
+            _F64, _I32, _VP, _VP, _VP, _VP, _SZ, _VP, _VP
         ]
     ),
     'pcm_adam_step': (

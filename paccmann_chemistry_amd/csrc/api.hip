@@ -4,6 +4,7 @@
 #include <string.h>
 
 #include "stackgru.h"
+#include "topbeam.h"
 
 int pcm_launch_dropout_add(float *dst, long long ldd, const float *src,
                            long long lds_, int B, int H, uint64_t seed,
@@ -1730,11 +1731,18 @@ struct BeamLayout {
     size_t off_scores;     // double[B][width]
     size_t off_hist_tok;   // int32[G][B][width]
     size_t off_hist_par;   // int32[G][B][width]
+    // joint search (beam_layout(..., true)) only
+    size_t off_jscores;    // double[2][width][B]
+    size_t off_jtok;       // int64[G][width][B]
+    size_t off_jpar;       // int32[G][width][B]
+    size_t off_jfin;       // uint8[2][width][B]
+    size_t off_jwork;      // pcm_beam_select's workspace
+    size_t jwork_bytes;
     size_t total;          // floats
 };
 
 static int beam_layout(const pcm_dims *dims, int width, int generate_len,
-                       BeamLayout *o) {
+                       BeamLayout *o, bool joint = false) {
     PCM_REQUIRE(dims, PCM_EINVAL, "dims is null");
     PCM_REQUIRE(width >= 1 && width <= 16, PCM_EINVAL,
                 "beam_width=%d outside 1..16", width);
@@ -1747,6 +1755,18 @@ static int beam_layout(const pcm_dims *dims, int width, int generate_len,
     if (rc) return rc;
     size_t off = o->g.total;
     const size_t bw = (size_t)dims->batch * width;
+    if (joint) {
+        const size_t g = generate_len > 0 ? generate_len : 1;
+        o->off_jscores = take(off, 4 * bw);
+        o->off_jtok = take(off, 2 * bw * g);
+        o->off_jpar = take(off, bw * g);
+        o->off_jfin = take(off, (2 * bw + 3) / 4);
+        o->jwork_bytes = pcm_beam_select_workspace_bytes(width, dims->batch,
+                                                         dims->vocab, width);
+        o->off_jwork = take(off, (o->jwork_bytes + 3) / 4);
+        o->total = off;
+        return PCM_OK;
+    }
     o->off_scores = take(off, 2 * bw);
     o->off_hist_tok = take(off, bw * (generate_len > 0 ? generate_len : 1));
     o->off_hist_par = take(off, bw * (generate_len > 0 ? generate_len : 1));
@@ -1764,20 +1784,27 @@ size_t pcm_generate_beam_workspace_bytes(const pcm_dims *dims,
     return bl.total * sizeof(float);
 }
 
-int pcm_stackgru_generate_beam(const pcm_dims *dims,
-                               const pcm_stackgru_params *weights,
-                               const float *out_w, const float *out_b,
-                               const float *h0, int64_t h0_layer_stride,
-                               const int64_t *prime, int32_t prime_len,
-                               int32_t generate_len, int32_t beam_width,
-                               int32_t top_tokens, float temperature,
-                               int64_t *tokens_out, int64_t *beam_tokens_out,
-                               double *beam_scores_out, void *workspace,
-                               size_t workspace_bytes, int32_t *status,
-                               void *stream) {
-    PCM_API_GUARD;
+}  // extern "C"
+
+// What the joint search does differently; null for the reference's search.
+struct JointSearch {
+    double temperature;
+    int32_t end_token;   // < 0: beams do not end
+};
+
+static int generate_beam(const pcm_dims *dims,
+                         const pcm_stackgru_params *weights,
+                         const float *out_w, const float *out_b,
+                         const float *h0, int64_t h0_layer_stride,
+                         const int64_t *prime, int32_t prime_len,
+                         int32_t generate_len, int32_t beam_width,
+                         int32_t top_tokens, float temperature,
+                         int64_t *tokens_out, int64_t *beam_tokens_out,
+                         double *beam_scores_out, void *workspace,
+                         size_t workspace_bytes, int32_t *status,
+                         void *stream, const JointSearch *joint) {
     BeamLayout bl;
-    int rc = beam_layout(dims, beam_width, generate_len, &bl);
+    int rc = beam_layout(dims, beam_width, generate_len, &bl, joint != nullptr);
     if (rc) return rc;
     GenLayout &g = bl.g;
     SGLayout &lay = g.lay;   // lay.B = beam_width * B
@@ -1837,9 +1864,18 @@ int pcm_stackgru_generate_beam(const pcm_dims *dims,
     if (lay.use_stack)
         pcm_launch_fill(ws + g.off_S[0], 0.f, (long long)BW * lay.DW, st);
     int64_t *cur_tok = (int64_t *)(ws + g.off_tok);
-    double *scores = (double *)(ws + bl.off_scores);
-    int32_t *hist_tok = (int32_t *)(ws + bl.off_hist_tok);
-    int32_t *hist_par = (int32_t *)(ws + bl.off_hist_par);
+    double *scores = nullptr, *jscores = nullptr;
+    int32_t *hist_tok = nullptr, *hist_par = nullptr;
+    uint8_t *jfin = nullptr;
+    if (joint) {
+        jscores = (double *)(ws + bl.off_jscores);
+        jfin = (uint8_t *)(ws + bl.off_jfin);
+        pcm_launch_beam_start(jscores, jfin, W, B, st);
+    } else {
+        scores = (double *)(ws + bl.off_scores);
+        hist_tok = (int32_t *)(ws + bl.off_hist_tok);
+        hist_par = (int32_t *)(ws + bl.off_hist_par);
+    }
 
     // slots: state copies still fed (the reference's zip() over tokens and
     // states shrinks them when fewer beams than slots exist, vae.py:471-483);
@@ -1874,6 +1910,33 @@ int pcm_stackgru_generate_beam(const pcm_dims *dims,
         rc = pcm_linear_forward(ws + g.off_h[slot][L - 1], Hp, out_w, out_b,
                                 logits, V, slots * B, V, H, st);
         if (rc) return rc;
+        if (joint) {
+            // scores and end flags alternate between two buffers; the chosen
+            // tokens stay in their history and are the next step's input
+            const size_t in = (size_t)(gi & 1) * BW, out = (size_t)BW - in;
+            int64_t *jtok = (int64_t *)(ws + bl.off_jtok) + (size_t)gi * BW;
+            int32_t *jpar = (int32_t *)(ws + bl.off_jpar) + (size_t)gi * BW;
+            const bool ends = joint->end_token >= 0;
+            rc = pcm_beam_select(logits, PCM_DTYPE_F32, V, jscores + in,
+                                 ends ? jfin + in : nullptr, W, B, V, W,
+                                 joint->temperature, joint->end_token, jtok,
+                                 jpar, jscores + out, ends ? jfin + out : nullptr,
+                                 ws + bl.off_jwork, bl.jwork_bytes, st);
+            if (rc) return rc;
+            cur_tok = jtok;
+            if (s + 1 == total_steps) continue;
+            pcm_state follow[PCM_MAX_LAYERS + 1];
+            int n = 0;
+            for (int l = 0; l < L; ++l, ++n)
+                follow[n] = {ws + g.off_h[slot][l], 1, 0,
+                             (int64_t)Hp * 4, (int64_t)Hp * 4};
+            if (lay.use_stack)
+                follow[n++] = {ws + g.off_S[slot], 1, 0, (int64_t)lay.DW * 4,
+                               (int64_t)lay.DW * 4};
+            rc = pcm_reorder_states(jpar, W, B, follow, n, status, st);
+            if (rc) return rc;
+            continue;
+        }
         BeamStepArgs a;
         a.logits = logits; a.scores = scores;
         a.hist_tok = hist_tok; a.hist_parent = hist_par; a.next_tok = cur_tok;
@@ -1888,10 +1951,70 @@ int pcm_stackgru_generate_beam(const pcm_dims *dims,
         beams = a.nb_next;
         slots = a.slots_next;
     }
-    pcm_launch_beam_backtrack(hist_tok, hist_par, scores, B, W, beams,
+    if (joint)
+        pcm_launch_beam_trace((int64_t *)(ws + bl.off_jtok),
+                              (int32_t *)(ws + bl.off_jpar),
+                              jscores + (size_t)(generate_len & 1) * BW, W, B,
                               generate_len, tokens_out, beam_tokens_out,
                               beam_scores_out, st);
+    else
+        pcm_launch_beam_backtrack(hist_tok, hist_par, scores, B, W, beams,
+                                  generate_len, tokens_out, beam_tokens_out,
+                                  beam_scores_out, st);
     return pcm_check_launch("stackgru_generate_beam");
+}
+
+extern "C" {
+
+int pcm_stackgru_generate_beam(const pcm_dims *dims,
+                               const pcm_stackgru_params *weights,
+                               const float *out_w, const float *out_b,
+                               const float *h0, int64_t h0_layer_stride,
+                               const int64_t *prime, int32_t prime_len,
+                               int32_t generate_len, int32_t beam_width,
+                               int32_t top_tokens, float temperature,
+                               int64_t *tokens_out, int64_t *beam_tokens_out,
+                               double *beam_scores_out, void *workspace,
+                               size_t workspace_bytes, int32_t *status,
+                               void *stream) {
+    PCM_API_GUARD;
+    return generate_beam(dims, weights, out_w, out_b, h0, h0_layer_stride, prime,
+                         prime_len, generate_len, beam_width, top_tokens,
+                         temperature, tokens_out, beam_tokens_out,
+                         beam_scores_out, workspace, workspace_bytes, status,
+                         stream, nullptr);
+}
+
+size_t pcm_generate_joint_beam_workspace_bytes(const pcm_dims *dims,
+                                               int32_t beam_width,
+                                               int32_t generate_len) {
+    BeamLayout bl;
+    if (beam_layout(dims, beam_width, generate_len, &bl, true)) return 0;
+    return bl.total * sizeof(float);
+}
+
+int pcm_stackgru_generate_joint_beam(
+    const pcm_dims *dims, const pcm_stackgru_params *weights,
+    const float *out_w, const float *out_b, const float *h0,
+    int64_t h0_layer_stride, const int64_t *prime, int32_t prime_len,
+    int32_t generate_len, int32_t beam_width, double temperature,
+    int32_t end_token, int64_t *tokens_out, int64_t *beam_tokens_out,
+    double *beam_scores_out, void *workspace, size_t workspace_bytes,
+    int32_t *status, void *stream) {
+    PCM_API_GUARD;
+    PCM_REQUIRE(dims && end_token < dims->vocab, PCM_EINVAL,
+                "stackgru_generate_joint_beam: end_token %d outside the "
+                "vocabulary", end_token);
+    PCM_REQUIRE(dims->vocab <= PCM_MAX_VOCAB, PCM_EINVAL,
+                "stackgru_generate_joint_beam: vocabulary %d > %d", dims->vocab,
+                PCM_MAX_VOCAB);
+    PCM_REQUIRE(temperature > 1e-30 && temperature < 1e30, PCM_EINVAL,
+                "stackgru_generate_joint_beam: temperature must be positive");
+    const JointSearch joint = {temperature, end_token};
+    return generate_beam(dims, weights, out_w, out_b, h0, h0_layer_stride, prime,
+                         prime_len, generate_len, beam_width, 1, 1.0f,
+                         tokens_out, beam_tokens_out, beam_scores_out, workspace,
+                         workspace_bytes, status, stream, &joint);
 }
 
 }  // extern "C"

@@ -4,6 +4,7 @@ torch is used for device memory, streams and the autograd graph only; every
 arithmetic operation of the path runs in libpaccmann_hip.so.
 """
 import ctypes
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -69,6 +70,8 @@ def check_status(status, what='token ids'):
         )
     if word & _lib.STATUS_BAD_TOKEN:
         raise RuntimeError(f'index out of range in self ({what})')
+    if word & _lib.STATUS_BAD_PARENT:
+        raise RuntimeError('index out of range in self (parents of beams)')
 
 
 # Packed batches launch over the still-running prefix of the batch (True) or
@@ -641,6 +644,434 @@ def search_step(logits, search, temperature=1.0, seed=0, step=0):
         ), 'pcm_search_step'
     )
     return out.view(logits.shape[:-1])
+
+
+def stackgru_generate_joint_beam(
+    dims, weights, out_w, out_b, h0, prime, generate_len, beam_width,
+    temperature, end_token=None, want_beams=False, status=None
+):
+    """pcm_stackgru_generate_joint_beam; h0 is [B,H] (broadcast) or [L,B,H].
+    Returns tokens i64[B, G] (the best beam of every row, without the prime),
+    and with ``want_beams`` also (beam tokens i64[B, width, G], scores
+    f64[B, width]), best first."""
+    lib = load()
+    require_device(h0, 'generate h0')
+    dev = h0.device
+    n_layers, batch, hid = dims.layers, dims.batch, dims.hidden
+    weights = [None if w is None else _f32(w, 'weight').contiguous()
+               for w in weights]
+    wstruct = _lib.make_params(weights, n_layers)
+    h0 = _f32(h0, 'h0').contiguous()
+    h0_stride = 0 if h0.dim() == 2 else batch * hid
+    prime = prime.to(device=dev, dtype=torch.int64).contiguous().view(-1)
+    tokens = torch.empty(batch, generate_len, dtype=torch.int64, device=dev)
+    beams = scores = None
+    if want_beams:
+        beams = torch.empty(batch, beam_width, generate_len,
+                            dtype=torch.int64, device=dev)
+        scores = torch.empty(batch, beam_width, dtype=torch.float64,
+                             device=dev)
+    nbytes = lib.pcm_generate_joint_beam_workspace_bytes(
+        ctypes.byref(dims), int(beam_width), int(generate_len)
+    )
+    if nbytes == 0:
+        check(-1, 'pcm_generate_joint_beam_workspace_bytes')
+    work = torch.empty(nbytes // 4, dtype=torch.float32, device=dev)
+    out_w = _f32(out_w, 'output_layer.weight').contiguous()
+    out_b = _f32(out_b, 'output_layer.bias').contiguous()
+    with _on(dev):
+        check(
+            lib.pcm_stackgru_generate_joint_beam(
+                ctypes.byref(dims), ctypes.byref(wstruct), ptr(out_w),
+                ptr(out_b), ptr(h0), h0_stride, ptr(prime), prime.numel(),
+                int(generate_len), int(beam_width), float(temperature),
+                -1 if end_token is None else int(end_token), ptr(tokens),
+                ptr(beams), ptr(scores), ptr(work), nbytes, ptr(status),
+                stream_ptr(dev)
+            ), 'pcm_stackgru_generate_joint_beam'
+        )
+    if want_beams:
+        return tokens, beams, scores
+    return tokens
+
+
+# --------------------------------------------------------------------------
+# top logits, distillation, joint beam search
+# --------------------------------------------------------------------------
+class _Here:
+    """A context that is nothing: the device is current already."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _on(device):
+    """Makes ``device`` the current one for a library call."""
+    if torch.cuda.current_device() == device.index:
+        return _HERE
+    return torch.cuda.device(device)
+
+
+def _dtype_code(t, what):
+    code = _lib.DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(
+            f'{what}: expected float32, bfloat16 or float16, got {t.dtype}'
+        )
+    return code
+
+
+def _operand(t, what, device, shape, dtypes):
+    """``t`` on ``device``, of that shape and one of those types, dense."""
+    if t.device != device:
+        raise ValueError(f'{what} is on {t.device}, the logits on {device}')
+    if t.dtype not in dtypes:
+        names = ' or '.join(str(d).split('.')[-1] for d in dtypes)
+        raise TypeError(f'{what}: expected {names}, got {t.dtype}')
+    if t.shape != shape:
+        raise ValueError(
+            f'{what} has shape {tuple(t.shape)}, expected {tuple(shape)}'
+        )
+    return t.contiguous()
+
+
+def _check_temperature(temperature):
+    temperature = float(temperature)
+    if not 1e-30 < temperature < 1e30:
+        raise ValueError(f'temperature {temperature} must be positive')
+    return temperature
+
+
+def _check_vocab(vocab):
+    if not 1 <= vocab <= _lib.MAX_VOCAB:
+        raise ValueError(
+            f'vocabulary of {vocab}: expected 1..{_lib.MAX_VOCAB}'
+        )
+
+
+class TopLogits(NamedTuple):
+    """What ``top_logits`` keeps of a teacher and ``distill_loss`` takes:
+    the largest logits (their own type) and their indices i32[..., k], the
+    log-sum-exp f32[...] of the others at ``temperature`` (None: they are given
+    no probability), and that temperature.  A negative index marks an entry
+    that is absent, so that lists of different lengths fit one tensor."""
+    values: torch.Tensor
+    indices: torch.Tensor
+    rest: Optional[torch.Tensor] = None
+    temperature: float = 1.0
+
+
+def top_logits(logits, k, temperature=1.0):
+    """The ``k`` largest of ``logits[..., V]`` (fp32, bf16 or fp16), largest
+    first, equal ones by index, with log sum exp(logits / temperature) over the
+    others: ``TopLogits`` of shapes [..., k], [..., k], [...].  No gradient.  A
+    NaN ranks below every number and makes its row's ``rest`` NaN."""
+    lib = load()
+    require_device(logits, 'top logits')
+    code = _dtype_code(logits, 'top logits')
+    temperature = _check_temperature(temperature)
+    if logits.dim() < 1:
+        raise ValueError('top logits: a row of logits is needed')
+    vocab = logits.shape[-1]
+    _check_vocab(vocab)
+    k = int(k)
+    if not 1 <= k <= min(vocab, _lib.TOP_MAX):
+        raise ValueError(
+            f'k={k}: expected 1..{min(vocab, _lib.TOP_MAX)} '
+            f'(vocabulary {vocab})'
+        )
+    logits = logits.detach()
+    dev, lead = logits.device, logits.shape[:-1]
+    values = torch.empty(lead + (k, ), dtype=logits.dtype, device=dev)
+    indices = torch.empty(lead + (k, ), dtype=torch.int32, device=dev)
+    rest = torch.empty(lead, dtype=torch.float32, device=dev)
+    if rest.numel():
+        x2, rows, ld = _rows2d(logits, 'top logits')
+        need = lib.pcm_top_logits_workspace_bytes(rows, vocab, k)
+        work = None
+        if need:
+            work = torch.empty(need, dtype=torch.uint8, device=dev)
+        with _on(dev):
+            check(
+                lib.pcm_top_logits(
+                    x2.data_ptr(), code, rows, ld, vocab, k, temperature,
+                    values.data_ptr(), indices.data_ptr(), rest.data_ptr(),
+                    ptr(work), need, stream_ptr(dev)
+                ), 'pcm_top_logits'
+            )
+    return TopLogits(values, indices, rest, temperature)
+
+
+class DistillLossFn(torch.autograd.Function):
+    """loss = distill(logits[T,B,V], teacher); the gradient is computed with
+    the loss and multiplied by the incoming one in ``backward``."""
+
+    @staticmethod
+    def forward(ctx, logits, values, indices, rest, temperature, targets,
+                lengths, hard_weight, step_weight, status):
+        lib = load()
+        steps, batch, vocab = logits.shape
+        dev = logits.device
+        x2, _, ld = _rows2d(logits, 'distill logits')
+        want = ctx.needs_input_grad[0]
+        loss = torch.empty((), device=dev)
+        dlogits = torch.empty(
+            (steps, batch, vocab), dtype=logits.dtype, device=dev
+        ) if want else None
+        scratch = torch.empty(
+            lib.pcm_distill_scratch_floats(steps, batch), device=dev
+        )
+        with _on(dev):
+            check(
+                lib.pcm_distill_loss(
+                    x2.data_ptr(), _lib.DTYPES[logits.dtype], ld,
+                    values.data_ptr(), _lib.DTYPES[values.dtype],
+                    indices.data_ptr(), ptr(rest), indices.shape[-1],
+                    ptr(targets), ptr(lengths), ptr(step_weight), steps, batch,
+                    vocab, temperature, hard_weight, loss.data_ptr(),
+                    ptr(dlogits), scratch.data_ptr(), ptr(status),
+                    stream_ptr(dev)
+                ), 'pcm_distill_loss'
+            )
+        ctx.dlogits = dlogits
+        return loss
+
+    @staticmethod
+    def backward(ctx, dloss):
+        dlogits = ctx.dlogits
+        if dlogits is None:
+            raise RuntimeError(
+                'distill_loss backward called twice: the gradient is handed '
+                'out by the first call (retain_graph is not supported)'
+            )
+        ctx.dlogits = None
+        dev = dlogits.device
+        dloss = _f32(dloss, 'dloss').reshape(1).contiguous()
+        with _on(dev):
+            check(
+                load().pcm_scale(
+                    dlogits.data_ptr(), _lib.DTYPES[dlogits.dtype],
+                    dlogits.numel(), dloss.data_ptr(), stream_ptr(dev)
+                ), 'pcm_scale'
+            )
+        return (dlogits, ) + (None, ) * 9
+
+
+def distill_loss(logits, teacher, targets=None, lengths=None, hard_weight=0.0,
+                 step_weight=None, status=None):
+    """Distillation of ``logits[T,B,V]`` (fp32, bf16 or fp16) from a teacher's
+    ``TopLogits`` of shapes [T,B,k]: per row
+
+        (1 - hard_weight) temperature^2 KL(teacher || student)
+            + hard_weight * cross entropy(logits, targets)
+
+    with both distributions at the teacher's temperature over its listed tokens
+    and "any other token", summed over steps after weighting step t by
+    ``step_weight[t]`` (default: one over the rows with ``lengths > t``), as
+    ``DecoderHeadFn`` reduces its cross entropy.  Returns an fp32 scalar that
+    carries the gradient of the logits.  Indices outside the vocabulary raise
+    STATUS_BAD_TOKEN in ``status`` (see ``check_status``)."""
+    load()
+    require_device(logits, 'distill logits')
+    _dtype_code(logits, 'distill logits')
+    if logits.dim() != 3 or 0 in logits.shape:
+        raise ValueError(
+            f'logits have shape {tuple(logits.shape)}, expected [T, B, V]'
+        )
+    steps, batch, vocab = logits.shape
+    _check_vocab(vocab)
+    values, indices, rest, temperature = teacher
+    temperature = _check_temperature(temperature)
+    dev = logits.device
+    if indices.dim() != 3 or not 1 <= indices.shape[-1] <= _lib.TOP_MAX:
+        raise ValueError(
+            f'teacher indices have shape {tuple(indices.shape)}, expected '
+            f'[T, B, k] with k in 1..{_lib.TOP_MAX}'
+        )
+    shape = logits.shape[:2]
+    listed = shape + indices.shape[-1:]
+    values = _operand(values.detach(), 'teacher values', dev, listed,
+                      tuple(_lib.DTYPES))
+    indices = _operand(indices, 'teacher indices', dev, listed, (torch.int32, ))
+    if rest is not None:
+        rest = _operand(rest.detach(), 'teacher rest', dev, shape,
+                        (torch.float32, ))
+    hard_weight = float(hard_weight)
+    if not 0.0 <= hard_weight <= 1.0:
+        raise ValueError(f'hard_weight {hard_weight}: expected 0..1')
+    if targets is not None:
+        targets = _operand(targets, 'targets', dev, shape, (torch.int64, ))
+    elif hard_weight > 0:
+        raise ValueError('hard_weight needs targets')
+    if lengths is not None:
+        if lengths.dtype != torch.int32 or lengths.device != dev:
+            lengths = lengths.to(device=dev, dtype=torch.int32)
+        lengths = _operand(lengths, 'lengths', dev, (batch, ), (torch.int32, ))
+    if step_weight is not None:
+        step_weight = _operand(
+            step_weight.to(device=dev, dtype=torch.float32), 'step_weight',
+            dev, (steps, ), (torch.float32, )
+        )
+    return DistillLossFn.apply(
+        logits, values, indices, rest, temperature, targets, lengths,
+        hard_weight, step_weight, status
+    )
+
+
+class BeamStep(NamedTuple):
+    """One selection of ``beam_select``: of every batch row's new beams, best
+    first, the token i64[W,B], the beam it continues i32[W,B], the score
+    f64[W,B] and whether it has ended (bool[W,B], None if beams do not end)."""
+    tokens: torch.Tensor
+    parents: torch.Tensor
+    scores: torch.Tensor
+    finished: Optional[torch.Tensor] = None
+
+
+def beam_select(logits, scores, width=None, temperature=1.0, finished=None,
+                end_token=None):
+    """One step of a beam search over beams and vocabulary: of the K * V
+    candidates ``scores[k, b] + log_softmax(logits[k, b] / temperature)`` of
+    every batch row the ``width`` (default K) best, equal ones by beam, then
+    token.  ``logits[K,B,V]`` in fp32, bf16 or fp16 (rows k * B + b, the layout
+    of the beams' states), ``scores`` f64[K,B] with -inf for a slot that holds
+    no beam (at the start: every slot but the first).  ``finished`` bool[K,B]
+    with ``end_token``: a finished beam keeps its score and repeats
+    ``end_token``.  Returns a ``BeamStep``; ``reorder_states`` lets the states
+    follow.  A beam's own tokens are ranked by logit.  No gradient."""
+    lib = load()
+    require_device(logits, 'beam logits')
+    code = _dtype_code(logits, 'beam logits')
+    if logits.dim() != 3 or 0 in logits.shape:
+        raise ValueError(
+            f'logits have shape {tuple(logits.shape)}, expected [K, B, V]'
+        )
+    beams, batch, vocab = logits.shape
+    _check_vocab(vocab)
+    temperature = _check_temperature(temperature)
+    width = beams if width is None else int(width)
+    if not (1 <= beams <= _lib.BEAM_MAX and 1 <= width <= _lib.BEAM_MAX
+            and width <= beams * vocab):
+        raise ValueError(
+            f'{beams} beams and width {width}: expected 1..{_lib.BEAM_MAX}, '
+            f'the width within the {beams * vocab} candidates'
+        )
+    dev = logits.device
+    scores = _operand(scores, 'scores', dev, (beams, batch),
+                      (torch.float64, ))
+    if (finished is None) != (end_token is None):
+        raise ValueError('finished and end_token go together')
+    finished_out = None
+    if finished is not None:
+        finished = _operand(finished, 'finished', dev, (beams, batch),
+                            (torch.bool, ))
+        end_token = int(end_token)
+        if not 0 <= end_token < vocab:
+            raise ValueError(
+                f'end_token {end_token} outside the vocabulary of {vocab}'
+            )
+        finished_out = torch.empty((width, batch), dtype=torch.bool,
+                                   device=dev)
+    x2, _, ld = _rows2d(logits.detach(), 'beam logits')
+    tokens = torch.empty((width, batch), dtype=torch.int64, device=dev)
+    parents = torch.empty((width, batch), dtype=torch.int32, device=dev)
+    scores_out = torch.empty((width, batch), dtype=torch.float64, device=dev)
+    need = lib.pcm_beam_select_workspace_bytes(beams, batch, vocab, width)
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with _on(dev):
+        check(
+            lib.pcm_beam_select(
+                x2.data_ptr(), code, ld, scores.data_ptr(), ptr(finished),
+                beams, batch, vocab, width, temperature,
+                -1 if end_token is None else end_token, tokens.data_ptr(),
+                parents.data_ptr(), scores_out.data_ptr(), ptr(finished_out),
+                ptr(work), need, stream_ptr(dev)
+            ), 'pcm_beam_select'
+        )
+    return BeamStep(tokens, parents, scores_out, finished_out)
+
+
+def _state_view(t, row_dim, rows, what):
+    """PcmState of a tensor whose dimension ``row_dim`` is the beams' rows."""
+    dim = t.dim()
+    if not -dim <= row_dim < dim:
+        raise ValueError(f'{what}: row dimension {row_dim} of {dim}')
+    row_dim %= dim
+    shape, stride, size = t.shape, t.stride(), t.element_size()
+    if shape[row_dim] != rows:
+        raise ValueError(
+            f'{what} has {shape[row_dim]} rows, expected {rows}'
+        )
+    inner = 1   # elements of a row's piece, in one stretch
+    for d in range(dim - 1, row_dim, -1):
+        if shape[d] != 1 and stride[d] != inner:
+            raise ValueError(
+                f'{what}: the dimensions after its rows must be contiguous'
+            )
+        inner *= shape[d]
+    outer, outer_stride = 1, 0   # the dimensions before them, as one
+    for d in range(row_dim - 1, -1, -1):
+        if shape[d] == 1:
+            continue
+        if outer > 1 and stride[d] != outer * outer_stride:
+            raise ValueError(
+                f'{what}: the dimensions before its rows must be evenly spaced'
+            )
+        if outer == 1:
+            outer_stride = stride[d]
+        outer *= shape[d]
+    return _lib.PcmState(t.data_ptr(), outer, outer_stride * size,
+                         stride[row_dim] * size, inner * size)
+
+
+def reorder_states(parents, states, row_dims=0, status=None):
+    """Lets the states of beams follow them, IN PLACE and in one launch: with
+    ``parents`` i32[K,B] (``BeamStep.parents``), row ``k * B + b`` of every
+    tensor becomes what its row ``parents[k, b] * B + b`` was.  ``row_dims``:
+    the dimension of each tensor that holds the K * B rows, or one for all (the
+    StackGRU's hidden [L, K*B, H] has 1, its stack [K*B, D, W] has 0).  Any
+    element type; the dimensions after the rows must be contiguous, no two
+    tensors may share memory.  A parent outside [0, K) leaves its rows alone
+    and raises STATUS_BAD_PARENT in ``status`` (see ``check_status``)."""
+    lib = load()
+    require_device(parents, 'parents')
+    if parents.dtype != torch.int32 or parents.dim() != 2 \
+            or 0 in parents.shape:
+        raise ValueError('parents: expected int32[K, B]')
+    beams, batch = parents.shape
+    if beams > _lib.BEAM_MAX:
+        raise ValueError(f'{beams} beams: expected 1..{_lib.BEAM_MAX}')
+    if not 1 <= len(states) <= _lib.MAX_STATES:
+        raise ValueError(f'{len(states)} states: expected 1..'
+                         f'{_lib.MAX_STATES}')
+    if isinstance(row_dims, int):
+        row_dims = [row_dims] * len(states)
+    if len(row_dims) != len(states):
+        raise ValueError('row_dims: one for each state')
+    dev = parents.device
+    table = (_lib.PcmState * len(states))()
+    for i, (state, row_dim) in enumerate(zip(states, row_dims)):
+        if state.device != dev:
+            raise ValueError(
+                f'state {i} is on {state.device}, the parents on {dev}'
+            )
+        if state.requires_grad:
+            raise ValueError(f'state {i} requires a gradient')
+        table[i] = _state_view(state, row_dim, beams * batch, f'state {i}')
+    parents = parents.contiguous()
+    with _on(dev):
+        check(
+            lib.pcm_reorder_states(
+                parents.data_ptr(), beams, batch, table, len(states),
+                ptr(status), stream_ptr(dev)
+            ), 'pcm_reorder_states'
+        )
 
 
 def adam_step(param, grad, exp_avg, exp_avg_sq, lr, beta1, beta2, eps, step,

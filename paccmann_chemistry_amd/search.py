@@ -155,3 +155,41 @@ class BeamSearch(Search):
             for sample_beams in updated
         ]).permute(1, 0).to(self.device)
         return (token_beams, updated)
+
+
+class JointBeamSearch(Search):
+    """Beam search over beams AND vocabulary: every step keeps the best
+    ``beam_width`` of all beams' continuations, hidden states and stacks follow
+    the beams they belong to, and a beam that has produced the end token keeps
+    its score (the reference's BeamSearch, search.py:144-275, ranks
+    ``top_tokens`` per beam, leaves the states with their slots and never
+    ends).  ``generate_from_latent`` runs it on the device
+    (pcm_stackgru_generate_joint_beam); ``step`` is one selection."""
+
+    def __init__(self, beam_width: int = 3, temperature: float = 1.0):
+        super().__init__()
+        self.beam_width = beam_width
+        self.temperature = temperature
+
+    def start(self, batch_size: int, device=None) -> torch.Tensor:
+        """Scores f64[beam_width, B] before the first step: one beam."""
+        device = self.device if device is None else device
+        scores = torch.full((self.beam_width, batch_size), float('-inf'),
+                            dtype=torch.float64, device=device)
+        scores[0] = 0
+        return scores
+
+    def forward(self, logits: torch.Tensor) -> object:
+        raise NotImplementedError(
+            'JointBeamSearch needs the states to follow its beams: use step'
+        )
+
+    def step(self, logits: torch.Tensor, scores: torch.Tensor, finished=None,
+             end_token=None) -> object:
+        """One ``ops.beam_select`` over logits[K,B,V]: a ``BeamStep``."""
+        super().step(logits)
+        from .ops import beam_select
+        return beam_select(
+            logits, scores, self.beam_width, self.temperature, finished,
+            end_token
+        )

@@ -141,13 +141,17 @@ def train_vae(
     kl_growth=0.0015, input_keep=1., test_input_keep=0., start_index=2,
     end_index=3, generate_len=100, log_interval=100, eval_interval=200,
     save_interval=200, loss_tracker=None, logger=None, batch_mode='padded',
-    writer=None, persistent_optimizer=None
+    writer=None, persistent_optimizer=None, teacher=None, teacher_top=8,
+    teacher_temperature=2.0, hard_weight=0.5
 ):  # yapf: disable
     """training.py:70-325: one epoch.  The optimizer is re-created at the top
     of every epoch exactly as the reference does (training.py:132), unless the
     caller passes ``persistent_optimizer`` (not in the reference: an optimizer
     instance that keeps its moments across epochs and can be checkpointed with
-    ``save_checkpoint`` for a resume)."""
+    ``save_checkpoint`` for a resume).  With a ``teacher`` (a TeacherVAE of the
+    same vocabulary, not in the reference) the decoder's loss is distilled from
+    the teacher's ``teacher_top`` largest logits at ``teacher_temperature``,
+    ``hard_weight`` of it on the targets."""
     if loss_tracker is None:
         loss_tracker = {
             'test_loss_a': 10e4, 'test_rec_a': 10e4, 'test_kld_a': 10e4,
@@ -158,6 +162,8 @@ def train_vae(
     data_preparation = get_data_preparation(batch_mode)
     vae_model = model.to(device)
     vae_model.train()
+    if teacher is not None:
+        teacher = teacher.to(device).eval()
     train_loss = 0
     if persistent_optimizer is not None:
         optimizer = persistent_optimizer
@@ -178,9 +184,16 @@ def train_vae(
             end_index=end_index, device=device
         )
         optimizer.zero_grad()
-        decoder_loss, mu, logvar = vae_model(
-            encoder_seq, decoder_seq, target_seq
-        )
+        if teacher is None:
+            decoder_loss, mu, logvar = vae_model(
+                encoder_seq, decoder_seq, target_seq
+            )
+        else:
+            decoder_loss, mu, logvar = vae_model.distill(
+                encoder_seq, decoder_seq, target_seq,
+                teacher.teach(encoder_seq, decoder_seq, teacher_top,
+                              teacher_temperature), hard_weight
+            )
         loss, kl_div = vae_loss_function(
             decoder_loss, mu, logvar, kl_growth=kl_growth, step=global_step
         )

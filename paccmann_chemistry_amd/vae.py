@@ -12,10 +12,13 @@ from torch.nn.utils.rnn import PackedSequence
 from . import _lib
 from .hyperparams import OPTIMIZER_FACTORY
 from .ops import (
-    DecoderHeadFn, ReparamFn, check_status, linear, stackgru_generate,
-    stackgru_generate_beam
+    DecoderHeadFn, ReparamFn, check_status, distill_loss, linear,
+    stackgru_generate, stackgru_generate_beam, stackgru_generate_joint_beam,
+    top_logits
 )
-from .search import BeamSearch, GreedySearch, SamplingSearch
+from .search import (
+    BeamSearch, GreedySearch, JointBeamSearch, SamplingSearch
+)
 from .stack_rnn import StackGRU
 from .utils import packed_to_lengths
 
@@ -194,6 +197,59 @@ class StackGRUDecoder(StackGRU):
         targets, _ = packed_to_lengths(target_seq)
         return self._decode(tokens, targets, lengths, hidden, stack)
 
+    def _sequences(self, input_seq, target_seq):
+        """(tokens [T,B], targets [T,B] or None, lengths or None) of padded or
+        packed sequences."""
+        if isinstance(input_seq, PackedSequence):
+            tokens, lengths = packed_to_lengths(input_seq)
+            if target_seq is not None:
+                target_seq, _ = packed_to_lengths(target_seq)
+            return tokens, target_seq, lengths
+        return input_seq, target_seq, None
+
+    def _logits(self, latent_z, tokens, lengths):
+        hidden = self._latent_to_hidden(latent_z)
+        out, _, _ = self._run_sequence(tokens, lengths, hidden, None)
+        return linear(out, self.output_layer.weight, self.output_layer.bias)
+
+    def teacher_logits(self, latent_z, input_seq, k, temperature=1.0):
+        """What this decoder, as a teacher, says after every token of
+        ``input_seq``: ``TopLogits`` of shapes [T,B,k] (``ops.top_logits``),
+        for ``distill_step`` of a student.  latent_z as in
+        ``decoder_train_step``; no gradient."""
+        tokens, _, lengths = self._sequences(input_seq, None)
+        with torch.no_grad():
+            logits = self._logits(latent_z, tokens, lengths)
+            return top_logits(logits, k, temperature)
+
+    def distill_step(self, latent_z, input_seq, target_seq, teacher,
+                     hard_weight=0.5):
+        """``decoder_train_step`` with a teacher: the loss of
+        ``ops.distill_loss`` on this decoder's logits, ``hard_weight`` of it on
+        the targets (with 1 it is ``decoder_train_step``'s loss)."""
+        tokens, targets, lengths = self._sequences(input_seq, target_seq)
+        logits = self._logits(latent_z, tokens, lengths)
+        step_weight = None
+        if self.global_batch_loss:
+            from . import dp
+            step_weight = dp.global_step_weights(
+                lengths, tokens.shape[0], tokens.shape[1], logits.device
+            )
+        loss = distill_loss(
+            logits, teacher, targets=targets, lengths=lengths,
+            hard_weight=hard_weight, step_weight=step_weight,
+            status=self._status_word(logits.device)
+        )
+        self.logits = logits.detach()
+        # for monitoring, as in _decode
+        argmax = self.logits.argmax(-1).t()
+        if lengths is not None:
+            steps = torch.arange(tokens.shape[0], device=argmax.device)
+            running = steps < lengths.to(argmax.device).view(-1, 1)
+            argmax = torch.where(running, argmax, 0).float()
+        self.outputs = argmax
+        return loss
+
     def _decode(self, tokens, targets, lengths, hidden, stack):
         if stack is self.init_stack:
             stack = None
@@ -221,7 +277,9 @@ class StackGRUDecoder(StackGRU):
         """vae.py:391-489.  latent_z [1,B,Z]; prime_input i64[P]; returns
         i64[B, P+generate_len] (the prime included).  Greedy, sampling and
         beam search (which returns i64[B, generate_len], the best beam without
-        the prime, vae.py:485-488) each run in one fused generation call.
+        the prime, vae.py:485-488) each run in one fused generation call, as
+        does the joint beam search (the same shape; past its end token a
+        sequence repeats it).
         """
         if isinstance(search, type):
             search = search()
@@ -231,6 +289,10 @@ class StackGRUDecoder(StackGRU):
         if isinstance(search, BeamSearch):
             return self._generate_beam(
                 latent_z, prime_input, search, generate_len
+            )
+        if isinstance(search, JointBeamSearch):
+            return self._generate_joint_beam(
+                latent_z, prime_input, end_token, search, generate_len
             )
         if isinstance(search, GreedySearch):
             mode, temperature = _lib.SEARCH_GREEDY, 1.0
@@ -275,6 +337,27 @@ class StackGRUDecoder(StackGRU):
                 prime_input.view(-1), generate_len, search.beam_width,
                 search.top_tokens, search.temperature,
                 want_beams=return_beams,
+                status=self._status_word(hidden.device)
+            )
+
+
+    def _generate_joint_beam(self, latent_z, prime_input, end_token, search,
+                             generate_len, return_beams=False):
+        """JointBeamSearch in one fused call: i64[B, generate_len], the
+        best-scoring sequence of every row without the prime; with
+        ``return_beams`` also every beam i64[B, width, generate_len] and its
+        score f64[B, width], best first."""
+        batch_size = latent_z.shape[1]
+        end = None
+        if end_token is not None:
+            end = int(torch.as_tensor(end_token).view(-1)[0])
+        with torch.no_grad():
+            hidden = self._latent_to_hidden(latent_z)
+            return stackgru_generate_joint_beam(
+                self._dims(batch_size), self._weights(),
+                self.output_layer.weight, self.output_layer.bias, hidden,
+                prime_input.view(-1), generate_len, search.beam_width,
+                search.temperature, end_token=end, want_beams=return_beams,
                 status=self._status_word(hidden.device)
             )
 
@@ -378,6 +461,31 @@ class TeacherVAE(nn.Module):
         mu, logvar = self.encode(input_seq)
         latent_z = self.reparameterize(mu, logvar, eps).unsqueeze(0)
         decoder_loss = self.decode(latent_z, decoder_seq, target_seq)
+        return decoder_loss, mu, logvar
+
+    def _latent(self, input_seq, eps):
+        mu, logvar = self.encode(input_seq)
+        latent_z = self.reparameterize(mu, logvar, eps).unsqueeze(0)
+        return mu, logvar, latent_z.expand(self.decoder.n_layers, -1, -1)
+
+    def teach(self, input_seq, decoder_seq, k=8, temperature=2.0, eps=None):
+        """As a teacher: the ``TopLogits`` [T,B,k] of this model's decoder over
+        ``decoder_seq`` with the latent of ``input_seq``, for ``distill`` of a
+        student.  No gradient."""
+        with torch.no_grad():
+            _, _, latent_z = self._latent(input_seq, eps)
+            return self.decoder.teacher_logits(
+                latent_z, decoder_seq, k, temperature
+            )
+
+    def distill(self, input_seq, decoder_seq, target_seq, teacher,
+                hard_weight=0.5, eps=None):
+        """``forward`` with the decoder's loss distilled from a teacher's
+        ``TopLogits`` (``teach``): returns (decoder_loss, mu, logvar)."""
+        mu, logvar, latent_z = self._latent(input_seq, eps)
+        decoder_loss = self.decoder.distill_step(
+            latent_z, decoder_seq, target_seq, teacher, hard_weight
+        )
         return decoder_loss, mu, logvar
 
     def check_tokens(self):

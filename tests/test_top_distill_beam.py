@@ -1,0 +1,1286 @@
+"""Top logits, distillation, joint beam selection and state reordering against
+plain 64-bit implementations, at the sizes and masks where they can go wrong,
+their refusals, and the paths that run them together.
+
+Tolerances count roundings: EPS is half a step of fp32 (2^-24); a sum of n
+positive terms taken in chains of n / 64 (64 lanes at least share a row) is off
+by at most (n / 64 + 8) EPS, an exponential by |argument| + 2 of them.
+"""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+EPS = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8,
+        torch.float16: 2.0 ** -11}
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+gpu = pytest.mark.gpu
+
+
+def _dev():
+    return torch.device('cuda:0')
+
+
+def _gen(*numbers):
+    seed = 17
+    for n in numbers:
+        seed = (seed * 1000003 + int(n)) % (2 ** 31)
+    return torch.Generator().manual_seed(seed)
+
+
+# --------------------------------------------------------------------------
+# plain 64-bit implementations
+# --------------------------------------------------------------------------
+def ref_top(logits, k, tau):
+    x = logits.double().numpy()
+    rows, vocab = x.shape
+    values, places, rest = [], [], []
+    for row in x:
+        nan = np.isnan(row)
+        filled = np.where(nan, -np.inf, row)
+        order = np.lexsort((np.arange(vocab), -filled, nan))
+        values.append(row[order[:k]])
+        places.append(order[:k])
+        left = row[order[k:]] / tau
+        high = left.max() if left.size else -np.inf
+        if nan.any():
+            rest.append(np.nan)
+        elif np.isinf(high):
+            rest.append(high)
+        else:
+            rest.append(high + math.log(np.exp(left - high).sum()))
+    return (torch.from_numpy(np.array(values)),
+            torch.from_numpy(np.array(places)),
+            torch.tensor(rest, dtype=torch.float64))
+
+
+def _weights(steps, batch, lengths, step_weight):
+    running = torch.ones(steps, batch, dtype=torch.bool)
+    if lengths is not None:
+        running = torch.arange(steps)[:, None] < lengths[None, :]
+    if step_weight is None:
+        w = 1.0 / running.sum(1).clamp(min=1).double()
+    else:
+        w = step_weight.double()
+    return running.double() * w[:, None]
+
+
+def ref_distill(logits, values, indices, rest, tau, targets=None, lengths=None,
+                hard=0.0, step_weight=None):
+    """(loss, dlogits) by the definition, row by row, autograd in 64 bits."""
+    leaf = logits.double().clone().requires_grad_(True)
+    steps, batch, vocab = logits.shape
+    weights = _weights(steps, batch, lengths, step_weight)
+    total = torch.zeros((), dtype=torch.float64)
+    for t in range(steps):
+        for b in range(batch):
+            w = weights[t, b]
+            if w == 0:
+                continue
+            x = leaf[t, b] / tau
+            logq = torch.log_softmax(x, -1)
+            entries = [(int(i), float(v) / tau) for i, v in
+                       zip(indices[t, b], values[t, b].double())
+                       if 0 <= i < vocab]
+            other = torch.ones(vocab, dtype=torch.bool)
+            for i, _ in entries:
+                other[i] = False
+            said = torch.tensor([u for _, u in entries] + [
+                float(rest[t, b]) if rest is not None else -math.inf
+            ], dtype=torch.float64)
+            row = torch.zeros((), dtype=torch.float64)
+            if not bool((said == -math.inf).all()):
+                p = torch.softmax(said, 0)
+                logp = torch.log_softmax(said, 0)
+                outcomes = [logq[i] for i, _ in entries]
+                outcomes.append(torch.logsumexp(logq[other], 0)
+                                if bool(other.any()) else
+                                torch.tensor(-math.inf,
+                                             dtype=torch.float64))
+                for pj, lp, lq in zip(p, logp, outcomes):
+                    if pj > 0 or bool(torch.isnan(pj)):
+                        row = row + pj * (lp - lq)
+            row = (1 - hard) * tau * tau * row
+            if hard:
+                tg = min(max(int(targets[t, b]), 0), vocab - 1)
+                row = row - hard * torch.log_softmax(leaf[t, b], -1)[tg]
+            total = total + w * row
+    if not total.requires_grad:
+        return total, torch.zeros_like(leaf)
+    grad, = torch.autograd.grad(total, leaf)
+    return total.detach(), grad
+
+
+def ref_beam(logits, scores, width, tau, finished=None, end=None):
+    beams, batch, vocab = logits.shape
+    c = torch.full((beams, batch, vocab), -math.inf, dtype=torch.float64)
+    for k in range(beams):
+        for b in range(batch):
+            s = float(scores[k, b])
+            if finished is not None and bool(finished[k, b]):
+                c[k, b, end] = s if s == s else -math.inf
+                continue
+            x = logits[k, b].double()
+            if not s > -math.inf or bool(torch.isnan(x).any()) or \
+                    not math.isfinite(float(x.max())):
+                continue
+            x = x / tau
+            c[k, b] = s + (x - torch.logsumexp(x, 0))
+    flat = c.permute(1, 0, 2).reshape(batch, -1)
+    best, at = torch.sort(flat, dim=-1, descending=True, stable=True)
+    best, at = best[:, :width].t(), at[:, :width].t()
+    parents, tokens = at // vocab, at % vocab
+    done = None
+    if finished is not None:
+        done = finished.gather(0, parents) | (tokens == end)
+    return tokens, parents.int(), best, done
+
+
+def _strided(t, pad, dev):
+    """``t`` on the device as a view with a longer row stride at an odd
+    offset."""
+    shape = list(t.shape)
+    shape[-1] += pad
+    wide = torch.full(shape, float('nan'), dtype=t.dtype, device=dev)
+    view = wide[..., pad // 2: pad // 2 + t.shape[-1]]
+    view.copy_(t)
+    return view
+
+
+def _logits(shape, kind, dtype, g):
+    x = torch.randn(shape, generator=g) * 3
+    if kind == 'ties':
+        x = (x / 2).round()
+    elif kind == 'same':
+        x = torch.full(shape, -2.5)
+    elif kind == 'masked':     # most tokens are not allowed
+        keep = torch.rand(shape, generator=g) < 0.3
+        keep[..., -1] = True
+        x = torch.where(keep, x, -math.inf)
+    elif kind == 'lowest':     # masked with the type's lowest value
+        keep = torch.rand(shape, generator=g) < 0.3
+        x = torch.where(keep, x, torch.finfo(dtype).min)
+    elif kind == 'far':        # a list far above the others
+        x = x - 300
+        x[..., :3] += 500
+    elif kind == 'sorted':
+        x = x.sort(dim=-1, descending=True).values
+    elif kind == 'zeros':
+        x = torch.where(torch.rand(shape, generator=g) < 0.5, 0.0, -0.0)
+    return x.to(dtype)
+
+
+# --------------------------------------------------------------------------
+# refusals through the C ABI: before anything is launched
+# --------------------------------------------------------------------------
+def _host():
+    buf = (ctypes.c_double * 64)()
+    return ctypes.cast(buf, ctypes.c_void_p), buf
+
+
+def _refused(lib, rc, text):
+    assert rc != 0
+    assert text in lib.pcm_last_error().decode(), lib.pcm_last_error()
+
+
+def test_top_logits_refusals():
+    from paccmann_chemistry_amd import _lib
+    lib = _lib.load()
+    at, _keep = _host()
+
+    def call(logits=at, dtype=0, rows=2, ld=20, vocab=20, k=3, tau=1.0,
+             values=at):
+        return lib.pcm_top_logits(logits, dtype, rows, ld, vocab, k, tau,
+                                  values, at, at, None, 0, None)
+    _refused(lib, call(logits=None), 'null')
+    _refused(lib, call(values=None), 'null')
+    _refused(lib, call(dtype=3), 'dtype')
+    _refused(lib, call(rows=0), 'rows')
+    _refused(lib, call(vocab=0), 'rows')
+    _refused(lib, call(vocab=(1 << 18) + 1, ld=1 << 20), 'rows')
+    _refused(lib, call(ld=19), 'row stride')
+    _refused(lib, call(k=0), 'k=0')
+    _refused(lib, call(k=21), 'k=21')
+    _refused(lib, call(vocab=100, ld=100, k=65), 'k=65')
+    _refused(lib, call(tau=0.0), 'temperature')
+    _refused(lib, call(tau=float('nan')), 'temperature')
+
+
+def test_distill_refusals():
+    from paccmann_chemistry_amd import _lib
+    lib = _lib.load()
+    at, _keep = _host()
+
+    def call(logits=at, dtype=0, ld=20, values=at, vdtype=0, k=3, targets=at,
+             steps=2, batch=2, vocab=20, tau=1.0, hard=0.5):
+        return lib.pcm_distill_loss(
+            logits, dtype, ld, values, vdtype, at, None, k, targets, None,
+            None, steps, batch, vocab, tau, hard, at, None, at, None, None)
+    _refused(lib, call(logits=None), 'null')
+    _refused(lib, call(values=None), 'null')
+    _refused(lib, call(dtype=-1), 'dtype')
+    _refused(lib, call(vdtype=7), 'dtype')
+    _refused(lib, call(steps=0), 'shape')
+    _refused(lib, call(vocab=(1 << 18) + 1, ld=1 << 20), 'shape')
+    _refused(lib, call(steps=1 << 16, batch=1 << 16), 'rows')
+    _refused(lib, call(ld=3), 'row stride')
+    _refused(lib, call(k=0), 'k=0')
+    _refused(lib, call(k=65), 'k=65')
+    _refused(lib, call(tau=-1.0), 'temperature')
+    _refused(lib, call(hard=1.5), 'hard_weight')
+    _refused(lib, call(hard=float('nan')), 'hard_weight')
+    _refused(lib, call(targets=None), 'targets')
+    _refused(lib, lib.pcm_scale(None, 0, 4, at, None), 'bad args')
+    _refused(lib, lib.pcm_scale(at, 0, 0, at, None), 'bad args')
+    _refused(lib, lib.pcm_scale(at, 5, 4, at, None), 'dtype')
+    assert lib.pcm_distill_scratch_floats(0, 4) == 0
+    assert lib.pcm_distill_scratch_floats(3, 4) >= 15
+
+
+def test_beam_refusals():
+    from paccmann_chemistry_amd import _lib
+    lib = _lib.load()
+    at, _keep = _host()
+
+    def call(logits=at, dtype=0, ld=20, finished=at, beams=2, batch=2,
+             vocab=20, width=2, tau=1.0, end=3, done=at, work=at,
+             nbytes=1 << 30):
+        return lib.pcm_beam_select(
+            logits, dtype, ld, at, finished, beams, batch, vocab, width, tau,
+            end, at, at, at, done, work, nbytes, None)
+    _refused(lib, call(logits=None), 'null')
+    _refused(lib, call(dtype=9), 'dtype')
+    _refused(lib, call(beams=0), 'beams=0')
+    _refused(lib, call(beams=17), 'beams=17')
+    _refused(lib, call(width=17), 'width=17')
+    _refused(lib, call(beams=1, vocab=2, ld=2, width=3, end=1), 'candidates')
+    _refused(lib, call(batch=0), 'batch=0')
+    _refused(lib, call(vocab=0, ld=0), 'vocab=0')
+    _refused(lib, call(ld=19), 'row stride')
+    _refused(lib, call(tau=0.0), 'temperature')
+    _refused(lib, call(end=20), 'end_token')
+    _refused(lib, call(end=-1), 'end_token')
+    _refused(lib, call(done=None), 'finished_out')
+    _refused(lib, call(nbytes=0), 'workspace')
+    assert lib.pcm_beam_select_workspace_bytes(0, 1, 5, 1) == 0
+
+
+def test_reorder_refusals():
+    from paccmann_chemistry_amd import _lib
+    lib = _lib.load()
+    at, _keep = _host()
+    base = at.value
+
+    def call(states, beams=2, batch=2, parents=at):
+        table = (_lib.PcmState * max(1, len(states)))(
+            *[_lib.PcmState(*s) for s in states])
+        return lib.pcm_reorder_states(parents, beams, batch, table,
+                                      len(states), None, None)
+    good = (base, 1, 0, 16, 16)
+    _refused(lib, call([good], parents=None), 'null')
+    _refused(lib, call([good], beams=17), 'beams=17')
+    _refused(lib, call([good], beams=0), 'beams=0')
+    _refused(lib, call([good], batch=0), 'batch=0')
+    _refused(lib, call([]), '0 states')
+    _refused(lib, call([good] * 17), '17 states')
+    _refused(lib, call([(None, 1, 0, 16, 16)]), 'null')
+    _refused(lib, call([(base, -1, 0, 16, 16)]), 'negative')
+    _refused(lib, call([(base, 1, 0, 8, 16)]), 'share memory')
+    _refused(lib, call([(base, 1, 0, -16, 16)]), 'share memory')
+    _refused(lib, call([(base, 2, 32, 16, 16)]), 'share memory')
+    _refused(lib, call([good, (base + 32, 1, 0, 16, 16)]), 'another')
+
+
+def test_generation_refusals():
+    from paccmann_chemistry_amd import _lib
+    lib = _lib.load()
+    dims = _lib.make_dims(4, 20, 20, 32, 2, 7, 5, True)
+    at, _keep = _host()
+    weights = _lib.PcmStackGRUParams()
+
+    def call(end=3, tau=1.0, width=3, d=dims):
+        return lib.pcm_stackgru_generate_joint_beam(
+            ctypes.byref(d), ctypes.byref(weights), at, at, None, 0, at, 1, 4,
+            width, tau, end, at, None, None, at, 0, None, None)
+    _refused(lib, call(end=20), 'end_token')
+    _refused(lib, call(tau=0.0), 'temperature')
+    _refused(lib, call(width=17), 'beam_width')
+    assert lib.pcm_generate_joint_beam_workspace_bytes(
+        ctypes.byref(dims), 17, 4) == 0
+    assert lib.pcm_generate_joint_beam_workspace_bytes(
+        ctypes.byref(dims), 3, 4) > 0
+
+
+def test_host_tensors_are_refused():
+    import paccmann_chemistry_amd as P
+    from paccmann_chemistry_amd._lib import PaccmannHipError
+    x = torch.zeros(2, 2, 5)
+    with pytest.raises(PaccmannHipError):
+        P.top_logits(x, 2)
+    with pytest.raises(PaccmannHipError):
+        P.distill_loss(x, P.TopLogits(x, x.int()))
+    with pytest.raises(PaccmannHipError):
+        P.beam_select(x, x[..., 0].double())
+    with pytest.raises(PaccmannHipError):
+        P.reorder_states(torch.zeros(2, 2, dtype=torch.int32), [x])
+    with pytest.raises(NotImplementedError):
+        P.JointBeamSearch().forward(x)
+
+
+def test_distill_definition_by_differences():
+    """The 64-bit definition itself: its gradient against central differences,
+    and the two limits (no list: nothing; everything listed: the full KL)."""
+    g = _gen(5)
+    logits = torch.randn(2, 2, 9, generator=g).double()
+    values = torch.randn(2, 2, 4, generator=g).double()
+    indices = torch.tensor([[[0, 3, 8, -1], [2, 2, 7, 1]],
+                            [[5, 4, 3, 2], [1, 0, 8, -1]]])
+    rest = torch.randn(2, 2, generator=g).double()
+    targets = torch.tensor([[1, 2], [3, 8]])
+    args = (values, indices, rest, 2.0, targets, None, 0.3)
+    _, grad = ref_distill(logits, *args)
+    for at in ((0, 0, 0), (0, 1, 2), (0, 1, 4), (1, 0, 8), (1, 1, 8)):
+        step = torch.zeros_like(logits)
+        step[at] = 1e-5
+        up, _ = ref_distill(logits + step, *args)
+        down, _ = ref_distill(logits - step, *args)
+        # truncation 1e-10 of a third derivative of order 1, rounding 1e-16/1e-5
+        assert abs((up - down) / 2e-5 - grad[at]) < 1e-9
+    none = torch.full_like(indices, -1)
+    loss, grad = ref_distill(logits, values, none, None, 2.0)
+    assert loss == 0 and bool((grad == 0).all())
+    every = torch.arange(9).expand(2, 2, 9)
+    teacher = torch.randn(2, 2, 9, generator=g).double()
+    loss, _ = ref_distill(logits, teacher, every, None, 2.0)
+    p, q = torch.softmax(teacher / 2, -1), torch.log_softmax(logits / 2, -1)
+    want = 4 * (p * (p.log() - q)).sum(-1).mean(1).sum()
+    assert abs(loss - want) < 1e-12
+
+
+# --------------------------------------------------------------------------
+# top logits
+# --------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows,vocab,k,kind', [
+    (1, 1, 1, 'normal'), (5, 60, 8, 'normal'), (67, 60, 8, 'ties'),
+    (7, 60, 60, 'normal'), (3, 64, 64, 'ties'), (2, 63, 16, 'same'),
+    (130, 129, 16, 'normal'), (3, 128, 16, 'masked'), (70, 33, 1, 'zeros'),
+    (2, 1000, 33, 'ties'), (5, 513, 64, 'masked'), (3, 2049, 64, 'same'),
+    (2, 2048, 5, 'sorted'), (2, 5003, 1, 'lowest'), (3, 5003, 64, 'far'),
+    (2, 8192, 64, 'sorted'), (2, 33001, 17, 'masked'), (1, 70001, 64, 'ties'),
+    (2, 65536, 64, 'same'), (1, 131071, 7, 'normal'),
+    (1, 262144, 64, 'normal'), (300, 700, 4, 'normal'),
+])
+def test_top_logits(dtype, rows, vocab, k, kind):
+    import paccmann_chemistry_amd as P
+    g = _gen(rows, vocab, k)
+    x = _logits((rows, vocab), kind, dtype, g)
+    tau = 2.0 if vocab % 2 else 1.0
+    values, places, rest = ref_top(x, k, tau)
+    for pad in (0, 7):
+        xd = _strided(x, pad, _dev()) if pad else x.to(_dev())
+        top = P.top_logits(xd, k, tau)
+        assert top.values.dtype == dtype and top.temperature == tau
+        assert torch.equal(top.indices.cpu().long(), places)
+        assert torch.equal(top.values.cpu().double(), values)
+        got = top.rest.cpu().double()
+        # chains of the sum, arguments of the exponentials, the shift's product
+        tol = EPS * (vocab / 64 + 16 + 4 * rest.abs())
+        fine = torch.isfinite(rest)
+        assert torch.equal(got[~fine], rest[~fine])
+        assert bool(((got - rest).abs() <= tol)[fine].all())
+
+
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('vocab,k', [(60, 8), (700, 9), (9000, 40)])
+def test_top_logits_of_rows_that_are_not_numbers(dtype, vocab, k):
+    import paccmann_chemistry_amd as P
+    g = _gen(vocab)
+    x = _logits((6, vocab), 'normal', dtype, g)
+    x[0, 5] = math.nan
+    x[1, 7] = math.inf
+    x[2, :] = -math.inf
+    x[3, :] = math.nan
+    x[4, k:] = math.nan       # fewer numbers than the list is long
+    x[4, 0] = math.nan
+    x[5, :] = math.inf
+    values, places, rest = ref_top(x, k, 1.0)
+    top = P.top_logits(x.to(_dev()), k)
+    assert torch.equal(top.indices.cpu().long(), places)
+    assert torch.equal(torch.isnan(top.values.cpu()), torch.isnan(values))
+    assert torch.equal(torch.nan_to_num(top.values.cpu().double(), 9e9),
+                       torch.nan_to_num(values, 9e9))
+    got = top.rest.cpu().double()
+    assert torch.equal(torch.isnan(got), torch.isnan(rest))
+    assert bool((got == rest)[torch.isinf(rest)].all())
+    fine = torch.isfinite(rest)
+    assert bool(((got - rest).abs() <= EPS * (vocab / 64 + 64))[fine].all())
+
+
+@gpu
+def test_top_logits_shapes_and_refusals():
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    x = torch.randn(4, 3, 30, generator=_gen(1)).to(dev)
+    top = P.top_logits(x, 5)
+    assert top.values.shape == (4, 3, 5) and top.rest.shape == (4, 3)
+    one = P.top_logits(x[1, 2], 5)
+    assert torch.equal(one.indices, top.indices[1, 2])
+    turned = P.top_logits(x.transpose(0, 1), 5)
+    assert torch.equal(turned.indices, top.indices.transpose(0, 1))
+    column = P.top_logits(x.permute(2, 0, 1), 2)    # unit stride nowhere
+    assert torch.equal(column.values.cpu(), torch.sort(
+        x.permute(2, 0, 1).cpu(), -1, descending=True).values[..., :2])
+    empty = P.top_logits(x[:0], 5)
+    assert empty.values.shape == (0, 3, 5)
+    leaf = x.clone().requires_grad_(True)
+    assert not P.top_logits(leaf, 2).values.requires_grad
+    for bad in (0, 31, 65):
+        with pytest.raises(ValueError):
+            P.top_logits(x, bad)
+    with pytest.raises(ValueError):
+        P.top_logits(x, 3, temperature=0.0)
+    with pytest.raises(TypeError):
+        P.top_logits(x.double(), 3)
+    with pytest.raises(ValueError):
+        P.top_logits(torch.zeros(1, (1 << 18) + 1, device=dev), 3)
+
+
+# --------------------------------------------------------------------------
+# distillation
+# --------------------------------------------------------------------------
+def _distill_case(T, B, V, k, dtype, kind, rest, g, absent=True):
+    logits = _logits((T, B, V), kind, dtype, g)
+    teacher = torch.randn(T, B, V, generator=g) * 3
+    tau = 2.0
+    values, indices = torch.topk(teacher, k, dim=-1)
+    others = teacher.scatter(-1, indices, -math.inf)
+    rest_t = torch.logsumexp(others / tau, -1).float() if rest else None
+    indices = indices.int()
+    if absent and k > 1:
+        keep = torch.randint(1, k + 1, (T, B, 1), generator=g)
+        indices = torch.where(torch.arange(k) < keep, indices, -1).int()
+    return logits, values.to(dtype), indices, rest_t, tau
+
+
+def _check_distill(got_loss, got, ref_loss, ref, logits, weights, tau, hard,
+                   vocab, dtype):
+    live = torch.where(torch.isfinite(logits.double()), logits.double(), 0.0)
+    size = 4 + 2 * live.abs().amax(-1) / tau + 2 * math.log(vocab + 1) + 30
+    chain = EPS * (vocab / 64 + 64)
+    per_row = ((1 - hard) * tau * tau + hard * tau) * size * chain
+    tol = float((weights.abs() * per_row).sum()) + EPS * abs(float(ref_loss))
+    if abs(float(ref_loss)) > torch.finfo(torch.float32).max:
+        # masked with the type's lowest value: tau^2 p 3.4e38 / tau can pass
+        # 3.4028e38, and what rounds to infinity in 32 bits is one
+        assert float(got_loss) == float(ref_loss.float())
+    else:
+        assert abs(float(got_loss) - float(ref_loss)) <= tol
+    # q and p are at most 1, |x| exp(-|x|) at most 1 / e; then one rounding
+    room = weights.abs()[..., None] * ((1 - hard) * tau + hard) * chain
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    tol = room + HALF[dtype] * (ref.abs() + room) + tiny
+    assert bool(((got.double() - ref).abs() <= tol).all())
+
+
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('T,B,V,k,kind,rest,hard,ragged', [
+    (1, 1, 1, 1, 'normal', False, 0.0, False),
+    (1, 1, 2, 1, 'normal', True, 0.5, False),
+    (3, 5, 60, 8, 'normal', True, 0.5, True),
+    (9, 21, 60, 8, 'ties', True, 0.0, True),
+    (4, 7, 60, 60, 'normal', False, 0.25, False),
+    (2, 3, 64, 64, 'normal', False, 1.0, True),
+    (2, 3, 128, 5, 'lowest', True, 0.25, False),
+    (2, 3, 129, 5, 'normal', True, 0.5, True),
+    (2, 2, 601, 64, 'far', True, 0.25, False),
+    (1, 3, 1030, 17, 'normal', False, 0.0, False),
+    (1, 3, 2050, 17, 'normal', True, 0.0, False),
+    (2, 2, 5003, 33, 'normal', True, 0.25, True),
+    (1, 2, 33001, 64, 'normal', True, 0.25, False),
+    (1, 2, 65537, 9, 'normal', True, 0.5, False),
+    (1, 1, 140001, 9, 'normal', True, 0.5, False),
+])
+def test_distill(dtype, T, B, V, k, kind, rest, hard, ragged):
+    import paccmann_chemistry_amd as P
+    g = _gen(T, B, V, k)
+    logits, values, indices, rest_t, tau = _distill_case(
+        T, B, V, k, dtype, kind, rest, g)
+    targets = torch.randint(0, V, (T, B), generator=g)
+    targets[0, 0] = max(int(indices[0, 0, 0]), 0)   # a target that is listed
+    lengths = torch.randint(0, T + 1, (B, ), generator=g) if ragged else None
+    weights = _weights(T, B, lengths, None)
+    ref_loss, ref = ref_distill(logits, values, indices, rest_t, tau, targets,
+                                lengths, hard)
+    dev = _dev()
+    for pad in (0, 5):
+        xd = (_strided(logits, pad, dev) if pad else logits.to(dev))
+        if ragged:       # whatever inactive rows hold takes no part
+            stop = weights.to(dev) == 0
+            xd[stop] = math.nan
+        xd = xd.detach().requires_grad_(True)
+        teacher = P.TopLogits(
+            values.to(dev), indices.to(dev),
+            rest_t.to(dev) if rest_t is not None else None, tau)
+        loss = P.distill_loss(
+            xd, teacher, targets=targets.to(dev),
+            lengths=None if lengths is None else lengths.to(dev),
+            hard_weight=hard)
+        assert loss.dtype == torch.float32 and loss.dim() == 0
+        grad, = torch.autograd.grad(loss, xd)
+        assert grad.dtype == dtype and grad.shape == xd.shape
+        _check_distill(loss, grad.cpu(), ref_loss, ref, logits, weights, tau,
+                       hard, V, dtype)
+        if ragged:
+            assert bool((grad.cpu()[weights == 0] == 0).all())
+        with torch.no_grad():
+            alone = P.distill_loss(
+                xd, teacher, targets=targets.to(dev),
+                lengths=None if lengths is None else lengths.to(dev),
+                hard_weight=hard)
+        assert torch.equal(alone, loss.detach())
+
+
+@gpu
+@pytest.mark.parametrize('V', [60, 700, 5000])
+def test_distill_odd_teachers(V):
+    """A list with the same index twice, an empty one, one whose values are all
+    -inf, indices outside the vocabulary, no probability for the others, a
+    nearly complete list, step weights with a zero."""
+    import paccmann_chemistry_amd as P
+    g = _gen(V, 3)
+    T, B, k, tau = 3, 4, 6, 2.0
+    logits, values, indices, rest, _ = _distill_case(
+        T, B, V, k, torch.float32, 'normal', True, g, absent=False)
+    indices[0, 0] = torch.tensor([4, 9, 4, 4, 9, 1])
+    indices[0, 1] = -1
+    rest[0, 1] = -math.inf
+    values[0, 2] = -math.inf
+    rest[0, 2] = -math.inf
+    indices[0, 3, 2] = V
+    indices[1, 0, 5] = 2 ** 31 - 1
+    indices[1, 1] = -7
+    rest[1, 2] = -math.inf
+    values[1, 3, 0] = -math.inf
+    logits[2, 0] -= 60            # the others hold e-26 of the student
+    logits[2, 0, indices[2, 0].long()] += 60
+    rest[2, 0] = -40.0
+    targets = torch.randint(0, V, (T, B), generator=g)
+    step_weight = torch.tensor([0.7, 1.3, 0.4])
+    weights = _weights(T, B, None, step_weight)
+    ref_loss, ref = ref_distill(logits, values, indices, rest, tau, targets,
+                                None, 0.25, step_weight)
+    dev = _dev()
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    xd = logits.to(dev).requires_grad_(True)
+    teacher = P.TopLogits(values.to(dev), indices.to(dev), rest.to(dev), tau)
+    loss = P.distill_loss(xd, teacher, targets=targets.to(dev),
+                          hard_weight=0.25, step_weight=step_weight.to(dev),
+                          status=status)
+    grad, = torch.autograd.grad(loss, xd)
+    _check_distill(loss, grad.cpu(), ref_loss, ref, logits, weights, tau, 0.25,
+                   V, torch.float32)
+    from paccmann_chemistry_amd.ops import check_status
+    with pytest.raises(RuntimeError, match='index out of range'):
+        check_status(status)
+    # a step without weight takes no part, NaN or not
+    step_weight[1] = 0
+    broken = logits.clone()
+    broken[1] = math.nan
+    ref_loss, ref = ref_distill(logits, values, indices, rest, tau, targets,
+                                None, 0.25, step_weight)
+    xd = broken.to(dev).requires_grad_(True)
+    loss = P.distill_loss(xd, teacher, targets=targets.to(dev),
+                          hard_weight=0.25, step_weight=step_weight.to(dev))
+    grad, = torch.autograd.grad(loss, xd)
+    _check_distill(loss, grad.cpu(), ref_loss, ref, logits,
+                   _weights(T, B, None, step_weight), tau, 0.25, V,
+                   torch.float32)
+
+
+@gpu
+def test_distill_values_that_are_not_numbers():
+    """Infinities where the definition has them, NaN where it has none."""
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    for V in (60, 900, 5000):
+        g = _gen(V, 11)
+        logits, values, indices, rest, tau = _distill_case(
+            1, 6, V, 5, torch.float32, 'normal', True, g, absent=False)
+        logits[0, 0, indices[0, 0, 0].long()] = -math.inf   # p > 0, q = 0
+        logits[0, 1, 3] = math.nan
+        logits[0, 2] = -math.inf
+        values[0, 3, 1] = math.nan
+        rest[0, 4] = math.nan
+        lengths = torch.ones(6, dtype=torch.int32)
+        for b, what in enumerate(['inf', 'nan', 'nan', 'nan', 'nan', '']):
+            one = torch.zeros(6, dtype=torch.int32)
+            one[b] = lengths[b]
+            xd = logits.to(dev).requires_grad_(True)
+            loss = P.distill_loss(
+                xd, P.TopLogits(values.to(dev), indices.to(dev), rest.to(dev),
+                                tau), lengths=one.to(dev))
+            value = float(loss)
+            grad, = torch.autograd.grad(loss, xd)
+            others = [r for r in range(6) if r != b]
+            assert bool((grad[0, others] == 0).all())
+            if what == 'inf':
+                assert value == math.inf
+                assert bool(torch.isfinite(grad[0, b]).all())
+            elif what == 'nan':
+                assert math.isnan(value)
+            else:
+                assert math.isfinite(value)
+
+
+@gpu
+def test_distill_gradient_by_differences_and_scale():
+    """The kernel's gradient against differences of the kernel's own loss, and
+    an incoming gradient that is not one."""
+    import paccmann_chemistry_amd as P
+    g = _gen(77)
+    dev = _dev()
+    logits, values, indices, rest, tau = _distill_case(
+        2, 3, 40, 6, torch.float32, 'normal', True, g)
+    targets = torch.randint(0, 40, (2, 3), generator=g).to(dev)
+    teacher = P.TopLogits(values.to(dev), indices.to(dev), rest.to(dev), tau)
+
+    def f(x):
+        return P.distill_loss(x, teacher, targets=targets, hard_weight=0.5)
+    x = logits.to(dev).requires_grad_(True)
+    base, = torch.autograd.grad(f(x), x)
+    step = 2.0 ** -5
+    loss = float(f(x.detach()))
+    # 32-bit losses: their rounding over the step; the third derivative of a
+    # log-sum-exp is at most 1, times tau^2 / tau^3 and the step's square
+    tol = 8 * EPS * max(1.0, loss) * 40 / step + step * step
+    for at in ((0, 0, 1), (0, 2, 39), (1, 1, int(indices[1, 1, 0]))):
+        d = torch.zeros_like(x)
+        d[at] = step
+        up, down = float(f(x.detach() + d)), float(f(x.detach() - d))
+        assert abs((up - down) / (2 * step) - float(base[at])) <= tol
+    for factor in (1.0, -3.5, 0.0):
+        loss = f(x) * factor
+        grad, = torch.autograd.grad(loss, x)
+        assert bool(((grad - base * factor).abs()
+                     <= EPS * (base * factor).abs()).all())
+    loss = f(x)
+    torch.autograd.grad(loss, x, retain_graph=True)
+    with pytest.raises(RuntimeError, match='twice'):
+        torch.autograd.grad(loss, x)
+
+
+@gpu
+def test_distill_refusals_of_tensors():
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    x = torch.randn(2, 3, 10, device=dev)
+    v, i = x[..., :4].contiguous(), torch.zeros(2, 3, 4, dtype=torch.int32,
+                                                device=dev)
+    good = P.TopLogits(v, i)
+    P.distill_loss(x, good)
+    with pytest.raises(ValueError):
+        P.distill_loss(x[0], good)
+    with pytest.raises(ValueError):
+        P.distill_loss(x[:, :0], good)
+    with pytest.raises(ValueError):
+        P.distill_loss(x, P.TopLogits(v[:1], i))
+    with pytest.raises(TypeError):
+        P.distill_loss(x, P.TopLogits(v, i.long()))
+    with pytest.raises(TypeError):
+        P.distill_loss(x, P.TopLogits(v.double(), i))
+    with pytest.raises(ValueError):
+        P.distill_loss(x, P.TopLogits(v, i.cpu()))
+    with pytest.raises(ValueError):
+        P.distill_loss(x, P.TopLogits(v, i, x[0, :, 0]))
+    with pytest.raises(ValueError):
+        P.distill_loss(x, P.TopLogits(v, i, None, -1.0))
+    with pytest.raises(ValueError):
+        P.distill_loss(x, P.TopLogits(v[..., :0], i[..., :0]))
+    with pytest.raises(ValueError):
+        P.distill_loss(x, good, hard_weight=0.5)
+    with pytest.raises(ValueError):
+        P.distill_loss(x, good, hard_weight=2.0)
+    with pytest.raises(TypeError):
+        P.distill_loss(x, good, targets=i[..., 0], hard_weight=0.5)
+    with pytest.raises(ValueError):
+        P.distill_loss(x, good, lengths=torch.ones(2, device=dev))
+    with pytest.raises(ValueError):
+        P.distill_loss(x, good, step_weight=torch.ones(3, device=dev))
+    with pytest.raises(TypeError):
+        P.distill_loss(x.double(), good)
+
+
+# --------------------------------------------------------------------------
+# beam selection
+# --------------------------------------------------------------------------
+def _check_beam(step, want, logits):
+    tokens, parents, scores, done = want
+    assert torch.equal(step.parents.cpu(), parents)
+    assert torch.equal(step.tokens.cpu(), tokens)
+    got = step.scores.cpu()
+    fine = torch.isfinite(scores)
+    assert torch.equal(got[~fine], scores[~fine])
+    # the sum of exponentials in 64 bits, to 1.2e-11 of itself
+    assert bool(((got - scores).abs() <= 2e-11 + 1e-15 * scores.abs())
+                [fine].all())
+    if done is None:
+        assert step.finished is None
+    else:
+        assert torch.equal(step.finished.cpu(), done)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('K,B,V,W,kind,ends', [
+    (1, 1, 1, 1, 'normal', False), (1, 3, 60, 5, 'normal', False),
+    (3, 70, 60, 3, 'normal', True), (3, 5, 60, 16, 'masked', True),
+    (5, 2, 7, 5, 'normal', True), (16, 3, 60, 16, 'normal', False),
+    (2, 2, 2, 4, 'normal', True), (2, 3, 128, 2, 'zeros', True),
+    (4, 9, 129, 4, 'normal', True), (16, 2, 601, 16, 'masked', True),
+    (3, 2, 1000, 16, 'lowest', False), (8, 3, 5003, 8, 'normal', True),
+    (2, 2, 8192, 3, 'sorted', False), (4, 1, 131071, 4, 'normal', False),
+    (2, 1, 262144, 16, 'normal', True), (5, 130, 33, 5, 'far', False),
+    (1, 2, 70001, 16, 'normal', False),
+])
+def test_beam_select(dtype, K, B, V, W, kind, ends):
+    import paccmann_chemistry_amd as P
+    g = _gen(K, B, V, W)
+    logits = _logits((K, B, V), kind, dtype, g)
+    scores = -20 * torch.rand(K, B, generator=g, dtype=torch.float64)
+    scores[K - 1, 0] = -math.inf if K > 1 else -3.0
+    finished = torch.rand(K, B, generator=g) < 0.3 if ends else None
+    end = V - 1 if ends else None
+    tau = 0.8
+    want = ref_beam(logits, scores, W, tau, finished, end)
+    dev = _dev()
+    for pad in (0, 3):
+        xd = _strided(logits, pad, dev) if pad else logits.to(dev)
+        step = P.beam_select(
+            xd, scores.to(dev), width=W, temperature=tau,
+            finished=None if finished is None else finished.to(dev),
+            end_token=end)
+        _check_beam(step, want, logits)
+
+
+@gpu
+@pytest.mark.parametrize('V', [20, 60, 700, 6000])
+def test_beam_select_of_rows_without_a_distribution(V):
+    """Beams that are equal, slots without a beam, rows of NaN, +inf or
+    nothing: ties go to the lowest beam, then token."""
+    import paccmann_chemistry_amd as P
+    g = _gen(V, 2)
+    K, B = 6, 5
+    logits = _logits((K, B, V), 'normal', torch.float32, g)
+    scores = -20 * torch.rand(K, B, generator=g, dtype=torch.float64)
+    logits[:, 0] = logits[0, 0]
+    scores[:, 0] = scores[0, 0]        # the same beam six times
+    scores[1:, 1] = -math.inf          # the first step
+    logits[0, 1] = -math.inf           # ... with two tokens allowed
+    logits[0, 1, [3, 9]] = torch.tensor([1.0, 2.0])
+    logits[1, 2, 4] = math.nan
+    logits[2, 2, 4] = math.inf
+    logits[3, 2] = -math.inf
+    scores[4, 2] = math.nan
+    scores[:, 3] = -math.inf           # no beam at all
+    finished = torch.zeros(K, B, dtype=torch.bool)
+    finished[:, 4] = True              # all of them have ended
+    finished[1, 2] = True              # ... one with NaN for logits
+    dev = _dev()
+    want = ref_beam(logits, scores, K, 1.0, finished, 2)
+    step = P.beam_select(logits.to(dev), scores.to(dev),
+                         finished=finished.to(dev), end_token=2)
+    _check_beam(step, want, logits)
+    want = ref_beam(logits, scores, 2, 1.0)
+    step = P.beam_select(logits.to(dev), scores.to(dev), width=2)
+    _check_beam(step, want, logits)
+
+
+@gpu
+def test_beam_select_refusals_of_tensors():
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    x = torch.randn(2, 3, 10, device=dev)
+    s = torch.zeros(2, 3, dtype=torch.float64, device=dev)
+    f = torch.zeros(2, 3, dtype=torch.bool, device=dev)
+    P.beam_select(x, s)
+    with pytest.raises(ValueError):
+        P.beam_select(x[0], s)
+    with pytest.raises(ValueError):
+        P.beam_select(x, s[:1])
+    with pytest.raises(TypeError):
+        P.beam_select(x, s.float())
+    with pytest.raises(ValueError):
+        P.beam_select(x, s.cpu())
+    with pytest.raises(ValueError):
+        P.beam_select(x, s, finished=f)
+    with pytest.raises(ValueError):
+        P.beam_select(x, s, end_token=3)
+    with pytest.raises(ValueError):
+        P.beam_select(x, s, finished=f, end_token=10)
+    with pytest.raises(TypeError):
+        P.beam_select(x, s, finished=f.int(), end_token=3)
+    with pytest.raises(ValueError):
+        P.beam_select(x, s, width=17)
+    with pytest.raises(ValueError):
+        P.beam_select(x[:, :, :1], s, width=3)
+    with pytest.raises(ValueError):
+        P.beam_select(x.expand(2, 3, 10).repeat(9, 1, 1), s.repeat(9, 1))
+    with pytest.raises(ValueError):
+        P.beam_select(x, s, temperature=0)
+
+
+# --------------------------------------------------------------------------
+# states that follow their beams
+# --------------------------------------------------------------------------
+def _rows_of(parents):
+    beams, batch = parents.shape
+    return (parents.long() * batch + torch.arange(batch)).reshape(-1)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.int8,
+                                   torch.float64, torch.bool])
+@pytest.mark.parametrize('K,B,inner', [
+    (1, 1, (1, )), (2, 1, (7, )), (3, 5, (64, )), (5, 3, (25, 19)),
+    (16, 2, (33, )), (4, 300, (2, 3)), (7, 1, (4097, )), (2, 70000, (1, )),
+])
+def test_reorder_states(dtype, K, B, inner):
+    import paccmann_chemistry_amd as P
+    g = _gen(K, B, inner[0])
+    dev = _dev()
+    parents = torch.randint(0, K, (K, B), generator=g, dtype=torch.int32)
+    parents[:, 0] = torch.arange(K)            # nothing moves
+    if B > 1:
+        parents[:, 1] = K - 1                  # everything follows one
+    if B > 2:
+        parents[:, 2] = torch.arange(K).roll(1)
+    rows = _rows_of(parents)
+
+    def make(*shape):
+        return (torch.randn(*shape, generator=g) * 50).to(dtype)
+    first, last = make(K * B, *inner), make(2, 3, K * B, *inner)
+    a, b = first.to(dev), last.to(dev)
+    P.reorder_states(parents.to(dev), [a, b], [0, 2])
+    assert torch.equal(a.cpu(), first[rows])
+    assert torch.equal(b.cpu(), last[:, :, rows])
+
+
+@gpu
+def test_reorder_views_bad_parents_and_refusals():
+    import paccmann_chemistry_amd as P
+    from paccmann_chemistry_amd.ops import check_status
+    dev = _dev()
+    g = _gen(8)
+    K, B = 3, 4
+    parents = torch.randint(0, K, (K, B), generator=g, dtype=torch.int32)
+    rows = _rows_of(parents)
+    wide = torch.randn(2, K * B, 11, generator=g)
+    want = wide.clone()
+    want[:, :, 2:7] = wide[:, rows, 2:7]       # columns inside other data
+    got = wide.to(dev)
+    P.reorder_states(parents.to(dev), [got[:, :, 2:7]], 1)
+    assert torch.equal(got.cpu(), want)
+    turned = torch.randn(K * B, 2, 6, generator=g)    # outer within the row
+    got = turned.to(dev)
+    P.reorder_states(parents.to(dev), [got.transpose(0, 1)], 1)
+    assert torch.equal(got.cpu(), turned[rows])
+    spare = torch.randn(K * B + 3, 5, generator=g)    # rows behind the last
+    got = spare.to(dev)
+    P.reorder_states(parents.to(dev), [got[:K * B]])
+    assert torch.equal(got.cpu()[:K * B], spare[:K * B][rows])
+    assert torch.equal(got.cpu()[K * B:], spare[K * B:])
+    # parents outside leave their rows and are reported
+    bad = parents.clone()
+    bad[1, 2], bad[0, 0] = K, -1
+    fixed = bad.clone()
+    fixed[1, 2], fixed[0, 0] = 1, 0
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    x = torch.randn(K * B, 5, generator=g)
+    got = x.to(dev)
+    P.reorder_states(bad.to(dev), [got], status=status)
+    assert torch.equal(got.cpu(), x[_rows_of(fixed)])
+    with pytest.raises(RuntimeError, match='parents'):
+        check_status(status)
+    check_status(status)
+    p = parents.to(dev)
+    P.reorder_states(p, [got[:, :0], got])            # an empty one is fine
+    with pytest.raises(ValueError):
+        P.reorder_states(p.long(), [got])
+    with pytest.raises(ValueError):
+        P.reorder_states(p, [got[:5]])
+    with pytest.raises(ValueError):
+        P.reorder_states(p, [got], 2)
+    with pytest.raises(ValueError):
+        P.reorder_states(p, [got], [0, 0])
+    with pytest.raises(ValueError):
+        P.reorder_states(p, [])
+    with pytest.raises(ValueError):
+        P.reorder_states(p, [got.cpu()])
+    with pytest.raises(ValueError):
+        P.reorder_states(p, [torch.randn(12, 5, 6, device=dev)
+                             .transpose(1, 2)])
+    with pytest.raises(ValueError):
+        P.reorder_states(p, [got.requires_grad_(True)])
+    y = torch.randn(K * B, 5, device=dev)
+    with pytest.raises(P._lib.PaccmannHipError, match='memory'):
+        P.reorder_states(p, [y, y])
+    with pytest.raises(P._lib.PaccmannHipError, match='memory'):
+        P.reorder_states(p, [y[:1].expand(K * B, 5)])
+
+
+# --------------------------------------------------------------------------
+# together
+# --------------------------------------------------------------------------
+PARAMS = {
+    'latent_dim': 16, 'rnn_cell_size': 64, 'embedding_size': 37,
+    'vocab_size': 37, 'stack_width': 6, 'stack_depth': 5, 'n_layers': 2,
+    'dropout': 0.0, 'batch_size': 21, 'batch_mode': 'padded',
+    'embedding': 'one_hot', 'use_stack': True, 'bidirectional': False
+}
+
+
+def _vae(params, seed, scale=0.35):
+    import paccmann_chemistry_amd as P
+    from oracle import weights as W
+    sd = W.make_state_dict(params, seed, scale=scale)
+    vae = P.TeacherVAE(P.StackGRUEncoder(dict(params)),
+                       P.StackGRUDecoder(dict(params)))
+    vae.load_state_dict(sd)
+    return vae.to(_dev()), sd
+
+
+def _oracle_joint(sd, z, prime, G, params, width, tau, end):
+    from oracle import stackgru_oracle as O
+    p = O.sub_params(sd, 'decoder')
+    batch = z.shape[0]
+    h0 = z @ p['latent_to_hidden.weight'].t() + p['latent_to_hidden.bias']
+    hidden = h0.repeat(width, 1).unsqueeze(0).repeat(params['n_layers'], 1, 1)
+    _, stack = O._zeros_state(p, batch * width, params['stack_depth'])
+    use = params['use_stack']
+    for t in range(prime.numel() - 1):
+        _, hidden, stack = O.stackgru_step(
+            p, prime[t].repeat(batch * width), hidden, stack, use)
+    tokens = prime[-1].repeat(width, batch)
+    scores = torch.full((width, batch), -math.inf, dtype=torch.float64)
+    scores[0] = 0
+    done = torch.zeros(width, batch, dtype=torch.bool)
+    seqs = torch.zeros(width, batch, 0, dtype=torch.long)
+    for _ in range(G):
+        out, hidden, stack = O.stackgru_step(
+            p, tokens.reshape(-1), hidden, stack, use)
+        logits = out @ p['output_layer.weight'].t() + p['output_layer.bias']
+        logits = logits.view(width, batch, -1)
+        tokens, parents, scores, now = ref_beam(
+            logits, scores, width, tau, done if end is not None else None, end)
+        done = now if now is not None else done
+        rows = _rows_of(parents)
+        hidden, stack = hidden[:, rows], stack[rows]
+        seqs = seqs.view(width * batch, -1)[rows].view(width, batch, -1)
+        seqs = torch.cat([seqs, tokens[..., None]], -1)
+    return seqs.transpose(0, 1), scores.t()
+
+
+@gpu
+@pytest.mark.parametrize('width,end,layers,use_stack', [
+    (1, 3, 2, True), (3, 3, 2, True), (5, None, 2, True), (4, 3, 1, True),
+    (16, 3, 2, False)])
+def test_joint_beam_generation_matches_oracle(width, end, layers, use_stack):
+    """generate_from_latent(search=JointBeamSearch) against the oracle's steps
+    with the plain selection and gathered states."""
+    import paccmann_chemistry_amd as P
+    params = dict(PARAMS, n_layers=layers, use_stack=use_stack)
+    vae, sd = _vae(params, 88)
+    vae.eval()
+    z = torch.from_numpy(np.random.default_rng(89).standard_normal(
+        (21, 16)).astype(np.float32))
+    prime, G = torch.tensor([2, 7]), 9
+    search = P.JointBeamSearch(beam_width=width, temperature=0.9)
+    with torch.no_grad():
+        want, want_scores = _oracle_joint(sd, z, prime, G, params, width, 0.9,
+                                          end)
+    end_token = None if end is None else torch.tensor([end])
+    best = vae.decoder.generate_from_latent(
+        z.unsqueeze(0).to(_dev()), prime.to(_dev()), end_token, search=search,
+        generate_len=G)
+    vae.decoder._update_batch_size(21)
+    tokens, beams, scores = vae.decoder._generate_joint_beam(
+        z.unsqueeze(0).to(_dev()), prime.to(_dev()), end_token, search, G,
+        return_beams=True)
+    vae.check_tokens()
+    assert torch.equal(best, tokens)
+    assert torch.equal(beams.cpu(), want)
+    assert torch.equal(tokens.cpu(), want[:, 0])
+    # 32-bit logits on both sides, of order 10, over G steps
+    assert bool(((scores.cpu() - want_scores).abs() <= 1e-4 * G).all())
+    # the same from the operators, one call each
+    dec = vae.decoder
+    B = 21
+    with torch.no_grad():
+        hidden = dec._latent_to_hidden(z.unsqueeze(0).to(_dev()))
+        hidden = hidden.repeat(width, 1).expand(layers, -1, -1).contiguous()
+        stack = torch.zeros(B * width, 5, 6, device=_dev())
+        dec._update_batch_size(B * width)
+        _, hidden, stack = dec(prime[:1].repeat(B * width).to(_dev()), hidden,
+                               stack)
+        last = prime[1].repeat(width, B).to(_dev())
+        score = search.start(B, _dev())
+        done = torch.zeros(width, B, dtype=torch.bool, device=_dev())
+        for _ in range(G):
+            out, hidden, stack = dec(last.view(-1), hidden, stack)
+            logits = torch.nn.functional.linear(
+                out[0], dec.output_layer.weight, dec.output_layer.bias)
+            step = search.step(logits.view(width, B, -1), score,
+                               done if end is not None else None, end)
+            states = [hidden, stack] if use_stack else [hidden]
+            P.reorder_states(step.parents, states, [1, 0][:len(states)])
+            last, score = step.tokens, step.scores
+            done = step.finished if end is not None else done
+    assert bool(((score.t() - scores).abs() <= 1e-4 * G).all())
+    # tokens through TeacherVAE.generate: nothing from the end token on
+    if end is not None:
+        mols = list(vae.generate(z.unsqueeze(0).to(_dev()), prime.to(_dev()),
+                                 end_token.to(_dev()), generate_len=G,
+                                 search=search))
+        assert len(mols) == 21
+        assert all(end not in m.tolist() for m in mols)
+
+
+@gpu
+@pytest.mark.parametrize('mode', ['padded', 'packed'])
+def test_distillation_of_a_model(mode):
+    """TeacherVAE.teach and distill: with all the weight on the targets the
+    loss is the ordinary one; with a teacher, loss and every gradient are the
+    ones of the formula on the student's own logits."""
+    import paccmann_chemistry_amd as P
+    params = dict(PARAMS, batch_size=6, batch_mode=mode)
+    student, _ = _vae(params, 5)
+    teacher, _ = _vae(params, 6)
+    dev = _dev()
+    g = _gen(9)
+    lens = [9, 9, 7, 5, 2, 1]
+    seqs = [torch.randint(4, 37, (n, ), generator=g) for n in lens]
+    if mode == 'packed':
+        pack = torch.nn.utils.rnn.pack_sequence
+        enc = pack([s.to(dev) for s in seqs])
+        tgt = pack([s.roll(-1).to(dev) for s in seqs])
+        lengths = torch.tensor(lens)
+    else:
+        enc = torch.nn.utils.rnn.pad_sequence(seqs).to(dev)
+        tgt = enc.roll(-1, 0)
+        lengths = None
+    eps = torch.randn(6, 16, generator=g).to(dev)
+    top = teacher.teach(enc, enc, k=5, temperature=2.0, eps=eps)
+    assert top.values.shape == (9, 6, 5) and not top.values.requires_grad
+    plain, _, _ = student(enc, enc, tgt, eps=eps)
+    hard, _, _ = student.distill(enc, enc, tgt, top, hard_weight=1.0, eps=eps)
+    # two 32-bit losses of 9 steps of order 4
+    assert abs(float(plain) - float(hard)) <= 64 * EPS * float(plain)
+    for p in student.parameters():
+        p.grad = None
+    loss, _, _ = student.distill(enc, enc, tgt, top, hard_weight=0.3, eps=eps)
+    loss.backward()
+    student.check_tokens()
+    got = {n: p.grad.clone() for n, p in student.named_parameters()
+           if p.grad is not None}
+    logits = student.decoder.logits
+    targets = tgt if mode == 'padded' else \
+        torch.nn.utils.rnn.pad_packed_sequence(tgt)[0]
+    ref_loss, ref = ref_distill(
+        logits.cpu(), top.values.cpu(), top.indices.cpu(), top.rest.cpu(),
+        2.0, targets.cpu(), lengths, 0.3)
+    weights = _weights(9, 6, lengths, None)
+    chain = EPS * 128
+    assert abs(float(loss) - float(ref_loss)) <= float(
+        weights.sum()) * 4 * 40 * chain
+    # the same gradient sent through the same layers
+    for p in student.parameters():
+        p.grad = None
+    tokens, _, lengths_ = student.decoder._sequences(enc, None)
+    _, _, z = student._latent(enc, eps)
+    again = student.decoder._logits(z, tokens, lengths_)
+    again.backward(ref.float().to(dev))
+    for name, p in student.named_parameters():
+        if name in got:
+            want = p.grad
+            assert float((got[name] - want).abs().max()) <= \
+                1e-4 * float(want.abs().max()) + 1e-9, name
+    out = student.decoder.outputs
+    assert out.shape == (6, 9)
+
+
+@gpu
+def test_train_vae_with_a_teacher(tmp_path):
+    import logging
+    import os
+    import paccmann_chemistry_amd as P
+    from paccmann_chemistry_amd.training import train_vae
+    from paccmann_chemistry_amd.utils import collate_fn
+
+    class Language:
+        start_index, stop_index = 2, 3
+    for mode in ('packed', 'padded'):
+        params = dict(PARAMS, batch_size=8, batch_mode=mode)
+        student, _ = _vae(params, 5, scale=0.1)
+        teacher, before = _vae(params, 6)
+        g = _gen(21)
+        data = [torch.randint(4, 37, (int(n), ), generator=g)
+                for n in torch.randint(3, 12, (32, ), generator=g)]
+        loader = torch.utils.data.DataLoader(
+            data, batch_size=8, collate_fn=collate_fn, drop_last=True)
+        os.makedirs(tmp_path / mode / 'weights')
+        start = {k: v.clone() for k, v in student.state_dict().items()}
+        train_vae(0, student, loader, loader, Language(), str(tmp_path / mode),
+                  search=P.JointBeamSearch(2), log_interval=2, eval_interval=3,
+                  save_interval=3, generate_len=6, batch_mode=mode,
+                  logger=logging.getLogger('test'), teacher=teacher,
+                  teacher_top=4)
+        moved = [k for k, v in student.state_dict().items()
+                 if not torch.equal(v, start[k])]
+        assert len(moved) >= 30
+        assert all(torch.equal(v.cpu(), before[k].cpu())
+                   for k, v in teacher.state_dict().items())
+
+
+@gpu
+def test_other_streams_and_captured_replays():
+    """A serving step (top logits, selection, reordering) and a distillation
+    forward, captured once and replayed on new inputs between eager calls of
+    the same operators; and the same on a side stream."""
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    K, B, V = 3, 8, 700
+
+    def inputs(i):
+        g = _gen(i, 4)
+        return [torch.randn(K, B, V, generator=g).to(dev),
+                (-torch.rand(K, B, generator=g, dtype=torch.float64)).to(dev),
+                torch.randn(2, K * B, 33, generator=g).to(dev)]
+
+    def work(x, s, h):
+        top = P.top_logits(x, 5, 2.0)
+        step = P.beam_select(x, s, temperature=0.7)
+        P.reorder_states(step.parents, [h], 1)
+        loss = P.distill_loss(x, P.TopLogits(*top))
+        return [top.values, top.indices, top.rest, step.tokens, step.parents,
+                step.scores, h, loss]
+    want = []
+    for i in range(3):
+        want.append([t.clone() for t in work(*inputs(i))])
+    held = inputs(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = work(*inputs(1))
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want[1]):
+        assert torch.equal(a, b)
+    torch.cuda.synchronize()
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = work(*held)
+    held2 = inputs(1)
+    with torch.cuda.graph(other):
+        outs2 = work(*held2)
+    for i in (0, 1, 2, 1):
+        for t, new in zip(held, inputs(i)):
+            t.copy_(new)
+        for t, new in zip(held2, inputs(2 - i)):
+            t.copy_(new)
+        graph.replay()
+        other.replay()
+        eager = work(*inputs(i))
+        torch.cuda.synchronize()
+        for a, b, c in zip(outs, want[i], eager):
+            assert torch.equal(a, b) and torch.equal(c, b)
+        for a, b in zip(outs2, want[2 - i]):
+            assert torch.equal(a, b)
+
+
+@gpu
+def test_distill_training_step_in_a_graph():
+    """Forward and backward captured together, the leaf made before."""
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    g = _gen(31)
+    logits, values, indices, rest, tau = _distill_case(
+        3, 4, 700, 6, torch.float32, 'normal', True, g)
+    teacher = P.TopLogits(values.to(dev), indices.to(dev), rest.to(dev), tau)
+    x = logits.to(dev).requires_grad_(True)
+
+    def step():
+        return torch.autograd.grad(P.distill_loss(x, teacher), x)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grad = step()
+    for i in range(3):
+        new = torch.randn(3, 4, 700, generator=_gen(i)).to(dev)
+        with torch.no_grad():
+            x.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        leaf = new.clone().requires_grad_(True)
+        want, = torch.autograd.grad(P.distill_loss(leaf, teacher), leaf)
+        assert torch.equal(grad, want)
+
+
+@gpu
+def test_results_repeat_bit_for_bit():
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    for V, dtype in ((60, torch.float32), (9001, torch.bfloat16)):
+        g = _gen(V)
+        logits, values, indices, rest, tau = _distill_case(
+            4, 9, V, 8, dtype, 'normal', True, g)
+        indices[0, 0, 1] = indices[0, 0, 0]
+        x = logits.to(dev).requires_grad_(True)
+        teacher = P.TopLogits(values.to(dev), indices.to(dev), rest.to(dev),
+                              tau)
+        first = None
+        for _ in range(4):
+            loss = P.distill_loss(x, teacher)
+            grad, = torch.autograd.grad(loss, x)
+            top = P.top_logits(x, 8, tau)
+            now = [loss.detach(), grad, top.values, top.indices, top.rest]
+            first = first or now
+            assert all(torch.equal(a, b) for a, b in zip(first, now))
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """Logits and states of more than 2^31 elements, checked at their ends."""
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    rows, V = 8200, 262144           # 2.15e9 elements of 2 bytes
+    x = torch.empty(rows, V, dtype=torch.bfloat16, device=dev)
+    x.fill_(-1.0)
+    x[-1, -5:] = torch.tensor([1.0, 5.0, 3.0, 4.0, 2.0], device=dev)
+    x[0, 7] = 9.0
+    top = P.top_logits(x, 3)
+    assert top.indices[-1].tolist() == [V - 4, V - 2, V - 3]
+    assert top.indices[0].tolist() == [7, 0, 1]
+    assert top.indices[4100].tolist() == [0, 1, 2]
+    step = P.beam_select(x.view(2, rows // 2, V),
+                         torch.zeros(2, rows // 2, dtype=torch.float64,
+                                     device=dev))
+    assert step.tokens[0, -1].item() == V - 4
+    assert step.parents[0, -1].item() == 1
+    before = x[-1].clone()
+    parents = torch.tensor([[1] * (rows // 2), [1] * (rows // 2)],
+                           dtype=torch.int32, device=dev)
+    P.reorder_states(parents, [x])
+    assert torch.equal(x[rows // 2 - 1], before)
+    assert torch.equal(x[-1], before)
+    assert x[0, 7].item() == -1.0
