@@ -61,24 +61,177 @@ static __device__ __forceinline__ float key_value(double k) {
     return __int_as_float(__double2hiint(k));
 }
 
+
+// ---- lanes --------------------------------------------------------------------------
+// Value of lane ^ M.  Within a row of 16 lanes by DPP, across rows by the
+// row-swap instructions of gfx950: no LDS traffic, a few cycles each.
+template <int M>
+static __device__ __forceinline__ unsigned lane_xor(unsigned v) {
+    static_assert(M == 1 || M == 2 || M == 4 || M == 8 || M == 16 || M == 32,
+                  "one bit");
+    if constexpr (M == 1)          // quad_perm 1 0 3 2
+        return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);
+    else if constexpr (M == 2)     // quad_perm 2 3 0 1
+        return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);
+    else if constexpr (M == 4) {   // half-row mirror (^7), then quads (^3)
+        v = __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);
+        return __builtin_amdgcn_update_dpp(0, v, 0x1B, 0xf, 0xf, true);
+    } else if constexpr (M == 8)   // row rotation by 8
+        return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, true);
+    else if constexpr (M == 16) {  // [0] even rows of both, [1] odd rows
+        auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return (threadIdx.x & 16) ? r[0] : r[1];
+    } else {
+        auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return (threadIdx.x & 32) ? r[0] : r[1];
+    }
+}
+template <int M>
+static __device__ __forceinline__ float lane_xor(float v) {
+    return __uint_as_float(lane_xor<M>(__float_as_uint(v)));
+}
+template <int M>
+static __device__ __forceinline__ int lane_xor(int v) {
+    return (int)lane_xor<M>((unsigned)v);
+}
+template <int M>
+static __device__ __forceinline__ double lane_xor(double v) {
+    return __hiloint2double(lane_xor<M>(__double2hiint(v)),
+                            lane_xor<M>(__double2loint(v)));
+}
+
 // ---- wave reductions ----------------------------------------------------------------
-static __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+// every lane gets the result; the order of the sums is fixed
+static __device__ __forceinline__ float pcm_max(float a, float b) { return fmaxf(a, b); }
+static __device__ __forceinline__ double pcm_max(double a, double b) { return fmax(a, b); }
+template <typename T>
+static __device__ __forceinline__ T wave_max(T v) {
+    v = pcm_max(v, lane_xor<1>(v));
+    v = pcm_max(v, lane_xor<2>(v));
+    v = pcm_max(v, lane_xor<4>(v));
+    v = pcm_max(v, lane_xor<8>(v));
+    v = pcm_max(v, lane_xor<16>(v));
+    return pcm_max(v, lane_xor<32>(v));
+}
+template <typename T>
+static __device__ __forceinline__ T wave_sum(T v) {
+    v += lane_xor<1>(v);
+    v += lane_xor<2>(v);
+    v += lane_xor<4>(v);
+    v += lane_xor<8>(v);
+    v += lane_xor<16>(v);
+    return v + lane_xor<32>(v);
+}
+
+// ---- sorting 64 keys across a wave ------------------------------------------------------
+template <int STRIDE>
+static __device__ __forceinline__ double key_exchange(double v, bool keep_max) {
+    const double o = lane_xor<STRIDE>(v);
+    return keep_max ? fmax(v, o) : fmin(v, o);
+}
+template <int SIZE, int STRIDE>
+static __device__ __forceinline__ double key_sort_steps(double v, int lane) {
+    v = key_exchange<STRIDE>(v, ((lane & STRIDE) == 0) ==
+                                    ((lane & SIZE) == 0));
+    if constexpr (STRIDE > 1) v = key_sort_steps<SIZE, STRIDE / 2>(v, lane);
     return v;
 }
-static __device__ __forceinline__ double wave_max(double v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = fmax(v, __shfl_xor(v, off, 64));
-    return v;
+// a bitonic sequence, sorted: largest in lane 0
+static __device__ __forceinline__ double key_merge(double v, int lane) {
+    return key_sort_steps<64, 32>(v, lane);
 }
-static __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+static __device__ __forceinline__ double key_sort(double v, int lane) {
+    v = key_sort_steps<2, 1>(v, lane);
+    v = key_sort_steps<4, 2>(v, lane);
+    v = key_sort_steps<8, 4>(v, lane);
+    v = key_sort_steps<16, 8>(v, lane);
+    v = key_sort_steps<32, 16>(v, lane);
+    return key_merge(v, lane);
 }
-static __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+// value of one lane, known to all
+static __device__ __forceinline__ double key_lane(double v, int lane) {
+    return __hiloint2double(
+        __builtin_amdgcn_readlane(__double2hiint(v), lane),
+        __builtin_amdgcn_readlane(__double2loint(v), lane));
 }
+
+// ---- eight elements of a row in registers -----------------------------------------------
+// Kept as they lie in memory (16-bit types packed) and widened where they are
+// used.  A row starts at any element: the loads are 16 bytes wide and aligned to
+// the element only, which global memory takes.
+typedef unsigned row_u32x4 __attribute__((ext_vector_type(4)));
+typedef row_u32x4 row_u32x4_e2 __attribute__((aligned(2)));
+typedef row_u32x4 row_u32x4_e4 __attribute__((aligned(4)));
+template <int DT> struct Row8;
+template <> struct Row8<PCM_DTYPE_F32> {
+    row_u32x4 a, b;
+    __device__ __forceinline__ void load(const float *p) {
+        a = *(const row_u32x4_e4 *)p;
+        b = *(const row_u32x4_e4 *)(p + 4);
+    }
+    __device__ __forceinline__ void lowest() { a = b = 0xFF800000u; }
+    __device__ __forceinline__ void set(int i, float v) {
+        if (i < 4) a[i] = __float_as_uint(v); else b[i - 4] = __float_as_uint(v);
+    }
+    __device__ __forceinline__ float get(int i) const {
+        return __uint_as_float(i < 4 ? a[i] : b[i - 4]);
+    }
+};
+template <> struct Row8<PCM_DTYPE_BF16> {
+    row_u32x4 a;
+    __device__ __forceinline__ void load(const __bf16 *p) {
+        a = *(const row_u32x4_e2 *)p;
+    }
+    __device__ __forceinline__ void lowest() { a = 0xFF80FF80u; }
+    __device__ __forceinline__ void set(int i, __bf16 v) {
+        const unsigned u = __builtin_bit_cast(unsigned short, v);
+        a[i >> 1] = i & 1 ? (a[i >> 1] & 0xffffu) | (u << 16)
+                          : (a[i >> 1] & 0xffff0000u) | u;
+    }
+    __device__ __forceinline__ float get(int i) const {
+        return __uint_as_float(i & 1 ? a[i >> 1] & 0xffff0000u : a[i >> 1] << 16);
+    }
+};
+template <> struct Row8<PCM_DTYPE_F16> {
+    row_u32x4 a;
+    __device__ __forceinline__ void load(const _Float16 *p) {
+        a = *(const row_u32x4_e2 *)p;
+    }
+    __device__ __forceinline__ void lowest() { a = 0xFC00FC00u; }
+    __device__ __forceinline__ void set(int i, _Float16 v) {
+        const unsigned u = __builtin_bit_cast(unsigned short, v);
+        a[i >> 1] = i & 1 ? (a[i >> 1] & 0xffffu) | (u << 16)
+                          : (a[i >> 1] & 0xffff0000u) | u;
+    }
+    __device__ __forceinline__ float get(int i) const {
+        const unsigned short u =
+            (unsigned short)(i & 1 ? a[i >> 1] >> 16 : a[i >> 1]);
+        return (float)__builtin_bit_cast(_Float16, u);
+    }
+};
+
+// n elements of a row, dealt to NT threads in groups of eight: element j of
+// group g of thread tid is (g * NT + tid) * 8 + j.  What lies past n is -inf.
+template <int DT, int NT, int G> struct RowRegs {
+    Row8<DT> r[G];
+    static __device__ __forceinline__ int at(int g, int tid) {
+        return (g * NT + tid) * 8;
+    }
+    __device__ __forceinline__ void load(const typename RowType<DT>::T *p, int n,
+                                         int tid) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int e = at(g, tid);
+            if (e + 8 <= n) {
+                r[g].load(p + e);
+            } else {
+                r[g].lowest();
+                if (e < n) {
+#pragma unroll
+                    for (int j = 0; j < 7; ++j)
+                        if (e + j < n) r[g].set(j, p[e + j]);
+                }
+            }
+        }
+    }
+};

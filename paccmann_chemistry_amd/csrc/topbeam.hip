@@ -5,174 +5,518 @@
 
 namespace {
 
+// ---- the largest of a stretch -------------------------------------------------------
+// NT threads find the k <= 64 largest keys of n elements they hold in registers.
+// Only elements above -inf are looked at (NaN is not): where there are fewer
+// than k of them the caller fills up.
+//   1. every thread knows its own first maximum; the waves sort theirs (64
+//      keys, in registers) and merge them pairwise, keeping 64: the k-th largest
+//      of the threads' maxima is a lower bound of the k-th largest element;
+//   2. at most k threads hold anything at or above it: those append what they
+//      have (k * 8 G keys at most, k and a few as a rule) to a list in LDS;
+//   3. the list is sorted, 64 at a time.
+// Keys are distinct, so the result does not depend on the order in 2.
+template <int NT> struct TopLds {
+    double list[NT / 64][64];
+    int count;
+};
+
+// the 64 largest of the waves' sorted lists; in wave 0 afterwards
+template <int NT>
+__device__ __forceinline__ double merge_waves(double v, double (*list)[64],
+                                              int lane, int wave) {
+    if constexpr (NT > 64) {
+        for (int s = NT / 128; s > 0; s >>= 1) {
+            if (wave >= s && wave < 2 * s) list[wave][lane] = v;
+            __syncthreads();
+            if (wave < s)
+                v = key_merge(fmax(v, list[wave + s][63 - lane]), lane);
+        }
+    }
+    return v;
+}
+
+// sorted top 64 of n keys in memory (LDS or global); in wave 0 afterwards
+template <int NT>
+__device__ __forceinline__ double top_of_list(const double *keys, int n,
+                                              double (*list)[64], int lane,
+                                              int wave) {
+    double v = KEY_NONE;
+    for (int c = wave * 64; c < n; c += NT) {
+        const double x =
+            key_sort(c + lane < n ? keys[c + lane] : KEY_NONE, lane);
+        // both descending: turn one around
+        const double turned = __shfl(x, 63 - lane, 64);
+        v = c == wave * 64 ? x : key_merge(fmax(v, turned), lane);
+    }
+    if (n > 64) v = merge_waves<NT>(v, list, lane, wave);
+    return v;
+}
+
+// returns in wave 0: lane j holds the j-th largest key (KEY_NONE past `found`);
+// `found` (all threads): how many elements were at or above the bound.
+template <int DT, int NT, int G>
+__device__ __forceinline__ double top_of_regs(const RowRegs<DT, NT, G> &x,
+                                              int first, int k, TopLds<NT> &lds,
+                                              double *buf, int tid, int &found) {
+    const int lane = tid & 63, wave = tid >> 6;
+    float bv = -INFINITY;
+    int bi = 0;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = x.r[g].get(j);
+            if (v > bv) { bv = v; bi = x.at(g, tid) + j; }
+        }
+    if (tid == 0) lds.count = 0;
+    double key = bv > -INFINITY ? key_of(bv, first + bi) : KEY_NONE;
+    key = key_sort(key, lane);
+    key = merge_waves<NT>(key, lds.list, lane, wave);
+    double bound;
+    if constexpr (NT > 64) {
+        if (wave == 0 && lane == k - 1) lds.list[0][0] = key;
+        __syncthreads();
+        bound = lds.list[0][0];
+    } else {
+        bound = key_lane(key, k - 1);
+        __syncthreads();
+    }
+    const float bound_v = bound == KEY_NONE ? -INFINITY : key_value(bound);
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = x.r[g].get(j);
+            if (v >= bound_v && v > -INFINITY) {
+                const double e = key_of(v, first + x.at(g, tid) + j);
+                if (e >= bound) buf[atomicAdd(&lds.count, 1)] = e;
+            }
+        }
+    __syncthreads();
+    found = lds.count;
+    return top_of_list<NT>(buf, found, lds.list, lane, wave);
+}
+
+// block-wide maximum / sum, every thread gets it
+template <int NT, typename T>
+__device__ __forceinline__ T all_max(T v, T *red, int tid) {
+    v = wave_max(v);
+    if constexpr (NT > 64) {
+        __syncthreads();
+        if ((tid & 63) == 0) red[tid >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int i = 1; i < NT / 64; ++i) v = pcm_max(v, red[i]);
+    }
+    return v;
+}
+template <int NT, typename T>
+__device__ __forceinline__ T all_sum(T v, T *red, int tid) {
+    v = wave_sum(v);
+    if constexpr (NT > 64) {
+        __syncthreads();
+        if ((tid & 63) == 0) red[tid >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int i = 1; i < NT / 64; ++i) v += red[i];
+    }
+    return v;
+}
+
 // ---- top logits -------------------------------------------------------------------
-// One wave per row; the j-th largest key is the largest one below the (j-1)-th,
-// so nothing has to be marked.
+struct TopArgs {
+    const void *logits;
+    void *values;
+    int32_t *indices;
+    float *rest;
+    double *keys;        // split rows: [rows][parts][k]
+    float *part;         // ... [rows][parts][2]: maximum and sum of the others
+    long long ld;
+    int V, k, parts, len;   // len: elements of one part
+    float scale, inv_t;     // log2(e) / temperature; 1 / temperature
+};
+
+// Entries past the `found` numbers above -inf: the -inf ones by index, then the
+// NaN by index.  One wave; rare.
 template <int DT>
-__global__ __launch_bounds__(256) void top_logits_kernel(
-    const typename RowType<DT>::T *logits, long long rows, long long ld, int V,
-    int k, float scale, typename RowType<DT>::T *values, int32_t *indices,
-    float *rest) {
+__device__ void top_fill(const typename RowType<DT>::T *x, int V, int have, int k,
+                         typename RowType<DT>::T *values, int32_t *indices,
+                         int lane) {
     typedef RowType<DT> R;
-    const int lane = threadIdx.x & 63;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const typename R::T *x = logits + row * ld;
-    double prev = __builtin_inf();
-    for (int j = 0; j < k; ++j) {
-        double best = KEY_NONE;
-        for (int v = lane; v < V; v += 64) {
-            const double key = key_of(R::up(x[v]), v);
-            if (key < prev && key > best) best = key;
+    for (int nan = 0; nan < 2 && have < k; ++nan)
+        for (int c = 0; c < V && have < k; c += 64) {
+            const int v = c + lane;
+            const float xv = v < V ? R::up(x[v]) : 0.f;
+            const bool hit = v < V && (nan ? xv != xv : xv == -INFINITY);
+            const unsigned long long m = __ballot(hit);
+            const int at = have + __popcll(m & ((1ull << lane) - 1));
+            if (hit && at < k) {
+                values[at] = x[v];
+                indices[at] = v;
+            }
+            have += __popcll(m);
         }
-        prev = wave_max(best);
-        if (lane == 0) {
-            values[row * k + j] = R::down(key_value(prev));
-            indices[row * k + j] = key_index(prev);
+}
+
+__device__ __forceinline__ float top_rest(float m, float s, float inv_t) {
+    if (s != s) return s;
+    return isinf(m) ? m : m * inv_t + logf(s);
+}
+
+// One block per row, or per part of a row.
+template <int DT, int NT, int G>
+__global__ __launch_bounds__(NT) void top_kernel(TopArgs a) {
+    typedef RowType<DT> R;
+    typedef typename R::T T;
+    extern __shared__ double top_buf[];   // [k * 8 G]
+    __shared__ TopLds<NT> lds;
+    __shared__ float red[NT / 64];
+    __shared__ double s_last;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const long long row = blockIdx.x / a.parts;
+    const int part = (int)(blockIdx.x - row * a.parts), first = part * a.len;
+    const int n = min(a.len, a.V - first);
+    const T *x = (const T *)a.logits + row * a.ld;
+    RowRegs<DT, NT, G> regs;
+    regs.load(x + first, n, tid);
+    int found;
+    const double key =
+        top_of_regs<DT, NT, G>(regs, first, a.k, lds, top_buf, tid, found);
+    if (tid < 64) {
+        if (a.parts > 1) {
+            if (lane < a.k)
+                a.keys[(row * a.parts + part) * a.k + lane] = key;
+        } else {
+            T *values = (T *)a.values + row * a.k;
+            int32_t *indices = a.indices + row * a.k;
+            if (lane < min(found, a.k)) {
+                values[lane] = R::down(key_value(key));
+                indices[lane] = key_index(key);
+            }
+            if (found < a.k) top_fill<DT>(x, a.V, found, a.k, values, indices, lane);
         }
+        if (lane == a.k - 1) s_last = key;
     }
+    __syncthreads();
+    // the others: below the last one of the list (all of it, if it is not full)
+    const double last = s_last;
+    const float last_v = last == KEY_NONE ? -INFINITY : key_value(last);
+    const int last_i = last == KEY_NONE ? -1 : key_index(last) - first;
     float m = -INFINITY;
-    for (int v = lane; v < V; v += 64) {
-        const float xv = R::up(x[v]);
-        if (key_of(xv, v) < prev) m = fmaxf(m, xv);
-    }
-    m = wave_max(m);
-    float s = 0.f;
     bool nan = false;
-    for (int v = lane; v < V; v += 64) {
-        const float xv = R::up(x[v]);
-        nan |= xv != xv;
-        if (key_of(xv, v) < prev) s += exp2f((xv - m) * scale);
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = regs.r[g].get(j);
+            nan |= v != v;
+            if (v < last_v || (v == last_v && regs.at(g, tid) + j > last_i))
+                m = fmaxf(m, v);
+        }
+    m = all_max<NT>(nan ? INFINITY : m, red, tid);
+    float s = 0.f;
+    const float mm = isinf(m) ? 0.f : m;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = regs.r[g].get(j);
+            if (!(v > last_v || (v == last_v && regs.at(g, tid) + j <= last_i)))
+                s += __builtin_amdgcn_exp2f((v - mm) * a.scale);
+        }
+    s = all_sum<NT>(s, red, tid);
+    if (tid == 0) {
+        if (a.parts > 1) {
+            float *p = a.part + (row * a.parts + part) * 2;
+            p[0] = m;
+            p[1] = s;
+        } else {
+            a.rest[row] = top_rest(m, s, a.inv_t);
+        }
     }
-    s = wave_sum(s);
-    if (lane == 0)
-        rest[row] = __any(nan) ? NAN
-                    : isinf(m) ? m
-                               : m * (scale * 0.6931471805599453f) + logf(s);
-    else
-        (void)__any(nan);
+}
+
+// Joins the parts of a row: their lists into one, what did not get into it and
+// the parts' others into the row's.
+template <int DT>
+__global__ __launch_bounds__(1024) void top_join_kernel(TopArgs a) {
+    typedef RowType<DT> R;
+    typedef typename R::T T;
+    __shared__ double list[16][64];
+    __shared__ float red[16];
+    __shared__ double s_last;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const long long row = blockIdx.x;
+    const int n = a.parts * a.k;
+    const double *keys = a.keys + row * n;
+    const double key = top_of_list<1024>(keys, n, list, lane, wave);
+    if (wave == 0) {
+        T *values = (T *)a.values + row * a.k;
+        int32_t *indices = a.indices + row * a.k;
+        const int found = __popcll(__ballot(key > KEY_NONE && lane < a.k));
+        if (lane < found) {
+            values[lane] = R::down(key_value(key));
+            indices[lane] = key_index(key);
+        }
+        if (found < a.k)
+            top_fill<DT>((const T *)a.logits + row * a.ld, a.V, found, a.k,
+                         values, indices, lane);
+        if (lane == a.k - 1) s_last = key;
+    }
+    __syncthreads();
+    const double last = s_last;
+    float m = -INFINITY;
+    for (int i = tid; i < n; i += 1024)
+        if (keys[i] < last && keys[i] > KEY_NONE) m = fmaxf(m, key_value(keys[i]));
+    if (tid < a.parts) m = fmaxf(m, a.part[(row * a.parts + tid) * 2]);
+    m = all_max<1024>(m, red, tid);
+    const float mm = isinf(m) ? 0.f : m;
+    float s = 0.f;
+    for (int i = tid; i < n; i += 1024)
+        if (keys[i] < last && keys[i] > KEY_NONE)
+            s += __builtin_amdgcn_exp2f((key_value(keys[i]) - mm) * a.scale);
+    if (tid < a.parts) {
+        const float *p = a.part + (row * a.parts + tid) * 2;
+        const float pm = isinf(p[0]) ? 0.f : p[0];
+        // (a part without others has the sum 0)
+        if (p[1] != 0.f)
+            s += p[1] * __builtin_amdgcn_exp2f((pm - mm) * a.scale);
+    }
+    s = all_sum<1024>(s, red, tid);
+    if (tid == 0) a.rest[row] = top_rest(m, s, a.inv_t);
 }
 
 // ---- beam selection ---------------------------------------------------------------
-// First kernel: the `width` best tokens of every beam row by logit (the row's
-// normaliser does not change their order) with their scores in 64 bits.
-template <int DT>
-__global__ __launch_bounds__(256) void beam_rows_kernel(
-    const typename RowType<DT>::T *logits, long long ld, const double *scores,
-    const uint8_t *finished, int rows, int V, int width, double inv_t, int end,
-    double *cand, int32_t *ctok) {
-    typedef RowType<DT> R;
-    const int lane = threadIdx.x & 63;
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const double score = scores[row];
-    double *co = cand + (long long)row * width;
-    int32_t *to = ctok + (long long)row * width;
-    if (finished && finished[row]) {
-        // end_token, then the others in order
-        for (int j = lane; j < width; j += 64) {
-            int tok = j == 0 ? end : j - 1 + (j - 1 >= end ? 1 : 0);
-            co[j] = j == 0 && score == score ? score : -INFINITY;
-            to[j] = tok < V ? tok : -1;
-        }
-        return;
-    }
-    const typename R::T *x = logits + (long long)row * ld;
+struct BeamArgs {
+    const void *logits;
+    const double *scores;
+    const uint8_t *finished;
+    double *keys;       // [beams][batch][parts][width]
+    double *part;       // [beams][batch][parts][2]: maximum, sum (64 bits)
+    int64_t *tokens;
+    int32_t *parents;
+    double *scores_out;
+    uint8_t *finished_out;
+    long long ld;
+    int beams, batch, V, width, parts, len, end;
+    double inv_t, scale;   // 1 / temperature; log2(e) / temperature
+};
+
+// 2^t for t <= 0 in 64 bits, to 3e-13 of itself: rounded to the nearest integer
+// the rest is at most 1/2, where the Taylor series of exp(f ln 2) is off by
+// (ln 2 / 2)^11 / 11! after its tenth power.  18 instructions; beams compete
+// by the difference of two log-sum-exps, for which 32 bits are too few.
+__device__ __forceinline__ double exp2_64(double t) {
+    t = fmax(t, -1100.);
+    const double n = rint(t), f = (t - n) * 0.6931471805599453;
+    double p = 1. / 3628800.;
+    p = fma(p, f, 1. / 362880.);
+    p = fma(p, f, 1. / 40320.);
+    p = fma(p, f, 1. / 5040.);
+    p = fma(p, f, 1. / 720.);
+    p = fma(p, f, 1. / 120.);
+    p = fma(p, f, 1. / 24.);
+    p = fma(p, f, 1. / 6.);
+    p = fma(p, f, 0.5);
+    p = fma(p, f, 1.);
+    p = fma(p, f, 1.);
+    return ldexp(p, (int)n);
+}
+
+// Per beam row (or part of one): the `width` largest logits -- the row's
+// normaliser does not change their order -- and its maximum and sum.
+template <int DT, int NT, int G>
+__global__ __launch_bounds__(NT) void beam_rows_kernel(BeamArgs a) {
+    typedef typename RowType<DT>::T T;
+    extern __shared__ double beam_buf[];   // [width * 8 G]
+    __shared__ TopLds<NT> lds;
+    __shared__ float redf[NT / 64];
+    __shared__ double red[NT / 64];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const long long row = blockIdx.x / a.parts;
+    const int part = (int)(blockIdx.x - row * a.parts), first = part * a.len;
+    // (the join does not look at the rows of these)
+    if (!(a.scores[row] > -INFINITY) || (a.finished && a.finished[row])) return;
+    const int n = min(a.len, a.V - first);
+    RowRegs<DT, NT, G> regs;
+    regs.load((const T *)a.logits + row * a.ld + first, n, tid);
+    int found;
+    const double key = top_of_regs<DT, NT, G>(regs, first, a.width, lds,
+                                              beam_buf, tid, found);
+    if (tid < a.width) a.keys[(row * a.parts + part) * a.width + lane] = key;
     float m = -INFINITY;
-    bool bad = !(score > -INFINITY);
-    if (!bad) {
-        for (int v = lane; v < V; v += 64) {
-            const float xv = R::up(x[v]);
-            m = fmaxf(m, xv);
-            bad |= xv != xv;
+    bool nan = false;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = regs.r[g].get(j);
+            nan |= v != v;
+            m = fmaxf(m, v);
         }
-        m = wave_max(m);
-        bad = __any(bad) || isinf(m);
-    }
-    if (bad) {   // no beam here, or no distribution: every candidate is -inf
-        for (int j = lane; j < width; j += 64) {
-            co[j] = -INFINITY;
-            to[j] = j < V ? j : -1;
-        }
-        return;
-    }
+    m = all_max<NT>(nan ? INFINITY : m, redf, tid);
     double s = 0.;
-    for (int v = lane; v < V; v += 64)
-        s += exp(((double)R::up(x[v]) - (double)m) * inv_t);
-    s = wave_sum(s);
-    const double lse = (double)m * inv_t + log(s);
-    double prev = __builtin_inf();
-    for (int j = 0; j < width; ++j) {
-        double best = KEY_NONE;
-        for (int v = lane; v < V; v += 64) {
-            const double key = key_of(R::up(x[v]), v);
-            if (key < prev && key > best) best = key;
+    if (!isinf(m)) {
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                s += exp2_64(((double)regs.r[g].get(j) - (double)m) * a.scale);
+        s = all_sum<NT>(s, red, tid);
+    }
+    if (tid == 0) {
+        double *p = a.part + (row * a.parts + part) * 2;
+        p[0] = m;   // +inf: a NaN or +inf in this part, no distribution
+        p[1] = s;
+    }
+}
+
+// One block per batch row, one wave per beam: the beam's parts become `width`
+// candidates with their scores; wave 0 ranks those of all beams (256 at most,
+// four per lane) by score, then beam and token.
+__global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
+    __shared__ double s_c[PCM_BEAM_MAX * PCM_BEAM_MAX];
+    __shared__ int s_f[PCM_BEAM_MAX * PCM_BEAM_MAX];
+    const int lane = threadIdx.x & 63;
+    const int k = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.x, W = a.width;
+    const long long row = (long long)k * a.batch + b;
+    const double score = a.scores[row];
+    const bool done = a.finished && a.finished[row];
+    int tok = -1;
+    double c = -INFINITY;
+    if (done) {
+        // end_token, then the others in order
+        tok = lane == 0 ? a.end : lane - 1 + (lane - 1 >= a.end ? 1 : 0);
+        if (lane == 0 && score == score) c = score;
+    } else {
+        double m = -INFINITY;
+        if (score > -INFINITY)
+            for (int p = lane; p < a.parts; p += 64)
+                m = fmax(m, a.part[(row * a.parts + p) * 2]);
+        m = wave_max(m);
+        tok = lane;   // a row without a distribution: the tokens in order
+        if (!isinf(m)) {
+            double s = 0.;
+            for (int p = lane; p < a.parts; p += 64) {
+                const double *q = a.part + (row * a.parts + p) * 2;
+                if (q[1] != 0.) s += q[1] * exp2_64((q[0] - m) * a.scale);
+            }
+            s = wave_sum(s);
+            const double lse = m * a.inv_t + log(s);
+            const double *keys = a.keys + row * a.parts * W;
+            const int n = a.parts * W;
+            double key = KEY_NONE;
+            for (int at = 0; at < n; at += 64) {
+                double x = at + lane < n ? keys[at + lane] : KEY_NONE;
+                if (a.parts > 1) x = key_sort(x, lane);
+                const double turned = __shfl(x, 63 - lane, 64);
+                key = at == 0 ? x : key_merge(fmax(key, turned), lane);
+            }
+            const bool real = key > KEY_NONE && lane < W;
+            const int found = __popcll(__ballot(real));
+            if (real) {
+                tok = key_index(key);
+                c = score + ((double)key_value(key) * a.inv_t - lse);
+            } else if (lane < W) {
+                // fewer tokens above -inf: the lowest ones that are not listed
+                int want = lane - found, t = 0;
+                for (;; ++t) {
+                    bool listed = false;
+                    for (int j = 0; j < found; ++j)
+                        listed |= key_index(key_lane(key, j)) == t;
+                    if (!listed && want-- == 0) break;
+                    if (t >= 2 * PCM_BEAM_MAX) break;
+                }
+                tok = t;
+            }
         }
-        prev = wave_max(best);
+    }
+    if (lane < W) {
+        s_c[k * W + lane] = c;
+        s_f[k * W + lane] = tok < a.V ? k * a.V + tok : 0x7fffffff;
+    }
+    __syncthreads();
+    if (k != 0) return;
+    const int n = a.beams * W;
+    double cc[4];
+    int f[4];   // beam * V + token, 0x7fffffff where there is no candidate
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int at = lane + 64 * i;
+        f[i] = at < n ? s_f[at] : 0x7fffffff;
+        cc[i] = f[i] != 0x7fffffff ? s_c[at] : -INFINITY;
+    }
+    for (int j = 0; j < W; ++j) {
+        double bc = cc[0];
+        int bf = f[0];
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+            if (cc[i] > bc || (cc[i] == bc && f[i] < bf)) { bc = cc[i]; bf = f[i]; }
+        const double best = wave_max(bc);
+        // the lowest of those with this score
+        unsigned cand = bc == best ? (unsigned)bf : 0x7fffffffu;
+        cand = min(cand, lane_xor<1>(cand));
+        cand = min(cand, lane_xor<2>(cand));
+        cand = min(cand, lane_xor<4>(cand));
+        cand = min(cand, lane_xor<8>(cand));
+        cand = min(cand, lane_xor<16>(cand));
+        cand = min(cand, lane_xor<32>(cand));
+        bf = (int)cand;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (f[i] == bf) { cc[i] = -INFINITY; f[i] = 0x7fffffff; }
         if (lane == 0) {
-            const bool none = j >= V;
-            co[j] = none ? -INFINITY
-                         : score + ((double)key_value(prev) * inv_t - lse);
-            to[j] = none ? -1 : key_index(prev);
+            const int from = bf / a.V, t = bf - from * a.V;
+            const long long o = (long long)j * a.batch + b;
+            a.tokens[o] = t;
+            a.parents[o] = from;
+            a.scores_out[o] = best;
+            if (a.finished_out)
+                a.finished_out[o] =
+                    (a.finished && a.finished[(long long)from * a.batch + b]) ||
+                    t == a.end;
         }
     }
 }
 
-// Second kernel: one wave per batch row ranks the beams * width survivors (at
-// most 256: four per lane).
-__global__ __launch_bounds__(256) void beam_join_kernel(
-    const double *cand, const int32_t *ctok, const uint8_t *finished, int beams,
-    int batch, int V, int width, int end, int64_t *tokens, int32_t *parents,
-    double *scores_out, uint8_t *finished_out) {
-    const int lane = threadIdx.x & 63;
-    const int b = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (b >= batch) return;
-    double c[4];
-    int f[4];   // k * V + token, 0x7fffffff where there is no candidate
-    const int n = beams * width;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int at = lane + 64 * i;
-        c[i] = KEY_NONE;
-        f[i] = 0x7fffffff;
-        if (at < n) {
-            const int k = at / width, j = at - k * width;
-            const long long o = ((long long)k * batch + b) * width + j;
-            const int tok = ctok[o];
-            if (tok >= 0) {
-                c[i] = cand[o];
-                f[i] = k * V + tok;
-            }
-        }
+// How a row of V logits is dealt out: `parts` blocks of `len` elements each.
+// A block holds its elements in registers (65536 at most).  Few rows leave most
+// of the 256 CUs idle, so long ones are split until there are about 512 blocks
+// or a part is down to 4096 elements; the join costs one more launch.
+struct RowPlan {
+    int parts, len;
+};
+RowPlan row_plan(long long rows, int V) {
+    RowPlan p;
+    long long parts = (V + 65535) / 65536;
+    if (rows < 256) {
+        long long want = 512 / rows, most = V / 4096;
+        if (want > most) want = most;
+        if (want > 64) want = 64;
+        if (want > parts) parts = want;
     }
-    for (int j = 0; j < width; ++j) {
-        double bc = c[0];
-        int bf = f[0];
-#pragma unroll
-        for (int i = 1; i < 4; ++i)
-            if (c[i] > bc || (c[i] == bc && f[i] < bf)) { bc = c[i]; bf = f[i]; }
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) {
-            const double oc = __shfl_xor(bc, off, 64);
-            const int of = __shfl_xor(bf, off, 64);
-            if (oc > bc || (oc == bc && of < bf)) { bc = oc; bf = of; }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (f[i] == bf) { c[i] = KEY_NONE; f[i] = 0x7fffffff; }
-        if (lane == 0) {
-            const int k = bf / V, tok = bf - k * V;
-            const long long o = (long long)j * batch + b;
-            tokens[o] = tok;
-            parents[o] = k;
-            scores_out[o] = bc;
-            if (finished_out)
-                finished_out[o] =
-                    (finished && finished[(long long)k * batch + b]) ||
-                    tok == end;
-        }
-    }
+    p.len = (int)((V + parts - 1) / parts);
+    p.len = (p.len + 7) / 8 * 8;
+    p.parts = (V + p.len - 1) / p.len;
+    return p;
 }
+// run `call` with the constants NT (threads) and G (groups of eight per thread)
+// for a stretch of `len` elements
+#define PCM_BY_LENGTH(len, call)                                         \
+    do {                                                                 \
+        if ((len) <= 512) { constexpr int NT = 64, G = 1; call; }        \
+        else if ((len) <= 1024) { constexpr int NT = 64, G = 2; call; }  \
+        else if ((len) <= 2048) { constexpr int NT = 256, G = 1; call; } \
+        else if ((len) <= 4096) { constexpr int NT = 256, G = 2; call; } \
+        else if ((len) <= 8192) { constexpr int NT = 256, G = 4; call; } \
+        else if ((len) <= 16384) { constexpr int NT = 512, G = 4; call; } \
+        else if ((len) <= 32768) { constexpr int NT = 1024, G = 4; call; } \
+        else { constexpr int NT = 1024, G = 8; call; }                   \
+    } while (0)
 
 // ---- states follow their beams ------------------------------------------------------
 struct ReorderArgs {
@@ -285,8 +629,10 @@ void pcm_launch_beam_trace(const int64_t *tokens, const int32_t *parents,
 extern "C" {
 
 size_t pcm_top_logits_workspace_bytes(int64_t rows, int32_t vocab, int32_t k) {
-    (void)rows; (void)vocab; (void)k;
-    return 0;
+    if (rows < 1 || vocab < 1 || vocab > PCM_MAX_VOCAB || k < 1) return 0;
+    const RowPlan p = row_plan(rows, vocab);
+    if (p.parts == 1) return 0;
+    return (size_t)rows * p.parts * (k * sizeof(double) + 2 * sizeof(float));
 }
 
 int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
@@ -312,23 +658,40 @@ int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
     const size_t need = pcm_top_logits_workspace_bytes(rows, vocab, k);
     PCM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), PCM_ENOMEM,
                 "top_logits: workspace %zu < %zu bytes", workspace_bytes, need);
+    PCM_REQUIRE(((uintptr_t)workspace & 7) == 0, PCM_EINVAL,
+                "top_logits: workspace must be 8-byte aligned");
     hipStream_t st = (hipStream_t)stream;
-    const float scale = (float)(1.4426950408889634 / temperature);
-    PCM_BY_DTYPE(dtype, {
-        typedef RowType<DT>::T T;
-        hipLaunchKernelGGL(top_logits_kernel<DT>,
-                           dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st,
-                           (const T *)logits, (long long)rows, (long long)ld,
-                           vocab, k, scale, (T *)values, indices, rest);
-    });
+    const RowPlan plan = row_plan(rows, vocab);
+    TopArgs a;
+    a.logits = logits; a.values = values; a.indices = indices; a.rest = rest;
+    a.keys = (double *)workspace;
+    a.part = plan.parts > 1
+                 ? (float *)(a.keys + (size_t)rows * plan.parts * k) : nullptr;
+    a.ld = ld; a.V = vocab; a.k = k; a.parts = plan.parts; a.len = plan.len;
+    a.scale = (float)(1.4426950408889634 / temperature);
+    a.inv_t = (float)(1.0 / temperature);
+    PCM_REQUIRE(rows * plan.parts < (1ll << 31), PCM_EINVAL,
+                "top_logits: too many rows");
+    PCM_BY_DTYPE(dtype, PCM_BY_LENGTH(plan.len, {
+        hipLaunchKernelGGL((top_kernel<DT, NT, G>),
+                           dim3((unsigned)(rows * plan.parts)), dim3(NT),
+                           (size_t)k * 8 * G * sizeof(double), st, a);
+    }));
+    if (plan.parts > 1)
+        PCM_BY_DTYPE(dtype, {
+            hipLaunchKernelGGL(top_join_kernel<DT>, dim3((unsigned)rows),
+                               dim3(1024), 0, st, a);
+        });
     return pcm_check_launch("top_logits");
 }
 
 size_t pcm_beam_select_workspace_bytes(int32_t beams, int32_t batch,
                                        int32_t vocab, int32_t width) {
-    (void)vocab;
-    if (beams < 1 || batch < 1 || width < 1) return 0;
-    return (size_t)beams * batch * width * (sizeof(double) + sizeof(int32_t));
+    if (beams < 1 || batch < 1 || width < 1 || vocab < 1 ||
+        vocab > PCM_MAX_VOCAB)
+        return 0;
+    const size_t rows = (size_t)beams * batch;
+    return rows * row_plan(rows, vocab).parts * (width + 2) * sizeof(double);
 }
 
 int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
@@ -369,19 +732,27 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
     PCM_REQUIRE(((uintptr_t)workspace & 7) == 0, PCM_EINVAL,
                 "beam_select: workspace must be 8-byte aligned");
     hipStream_t st = (hipStream_t)stream;
-    const int rows = beams * batch;
-    double *cand = (double *)workspace;
-    int32_t *ctok = (int32_t *)(cand + (size_t)rows * width);
-    PCM_BY_DTYPE(dtype, {
-        typedef RowType<DT>::T T;
-        hipLaunchKernelGGL(beam_rows_kernel<DT>, dim3((rows + 3) / 4), dim3(256),
-                           0, st, (const T *)logits, (long long)ld, scores,
-                           finished, rows, vocab, width, 1.0 / temperature,
-                           end_token, cand, ctok);
-    });
-    hipLaunchKernelGGL(beam_join_kernel, dim3((batch + 3) / 4), dim3(256), 0, st,
-                       cand, ctok, finished, beams, batch, vocab, width,
-                       end_token, tokens, parents, scores_out, finished_out);
+    const long long rows = (long long)beams * batch;
+    const RowPlan plan = row_plan(rows, vocab);
+    PCM_REQUIRE(rows * plan.parts < (1ll << 31), PCM_EINVAL,
+                "beam_select: too many rows");
+    BeamArgs a;
+    a.logits = logits; a.scores = scores; a.finished = finished;
+    a.keys = (double *)workspace;
+    a.part = a.keys + (size_t)rows * plan.parts * width;
+    a.tokens = tokens; a.parents = parents; a.scores_out = scores_out;
+    a.finished_out = finished_out;
+    a.ld = ld; a.beams = beams; a.batch = batch; a.V = vocab; a.width = width;
+    a.parts = plan.parts; a.len = plan.len; a.end = end_token;
+    a.inv_t = 1.0 / temperature;
+    a.scale = 1.4426950408889634 / temperature;
+    PCM_BY_DTYPE(dtype, PCM_BY_LENGTH(plan.len, {
+        hipLaunchKernelGGL((beam_rows_kernel<DT, NT, G>),
+                           dim3((unsigned)(rows * plan.parts)), dim3(NT),
+                           (size_t)width * 8 * G * sizeof(double), st, a);
+    }));
+    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)batch), dim3(64 * beams),
+                       0, st, a);
     return pcm_check_launch("beam_select");
 }
 
