@@ -27,14 +27,14 @@ static inline bool pcm_dtype_known(int dtype) {
     return dtype >= PCM_DTYPE_F32 && dtype <= PCM_DTYPE_F16;
 }
 // run `call` with the constant DT equal to a dtype code
-#define PCM_BY_DTYPE(dtype, call)                                    \
+#define PCM_BY_DTYPE(dtype, ...)                                     \
     do {                                                             \
         if ((dtype) == PCM_DTYPE_F32) {                              \
-            constexpr int DT = PCM_DTYPE_F32; call;                  \
+            constexpr int DT = PCM_DTYPE_F32; __VA_ARGS__;                  \
         } else if ((dtype) == PCM_DTYPE_BF16) {                      \
-            constexpr int DT = PCM_DTYPE_BF16; call;                 \
+            constexpr int DT = PCM_DTYPE_BF16; __VA_ARGS__;                 \
         } else {                                                     \
-            constexpr int DT = PCM_DTYPE_F16; call;                  \
+            constexpr int DT = PCM_DTYPE_F16; __VA_ARGS__;                  \
         }                                                            \
     } while (0)
 
@@ -123,6 +123,34 @@ static __device__ __forceinline__ T wave_sum(T v) {
     return v + lane_xor<32>(v);
 }
 
+// block-wide maximum / sum, every thread gets it
+template <int NT, typename T>
+static __device__ __forceinline__ T all_max(T v, T *red, int tid) {
+    v = wave_max(v);
+    if constexpr (NT > 64) {
+        __syncthreads();
+        if ((tid & 63) == 0) red[tid >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int i = 1; i < NT / 64; ++i) v = pcm_max(v, red[i]);
+    }
+    return v;
+}
+template <int NT, typename T>
+static __device__ __forceinline__ T all_sum(T v, T *red, int tid) {
+    v = wave_sum(v);
+    if constexpr (NT > 64) {
+        __syncthreads();
+        if ((tid & 63) == 0) red[tid >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int i = 1; i < NT / 64; ++i) v += red[i];
+    }
+    return v;
+}
+
 // ---- sorting 64 keys across a wave ------------------------------------------------------
 template <int STRIDE>
 static __device__ __forceinline__ double key_exchange(double v, bool keep_max) {
@@ -170,6 +198,17 @@ template <> struct Row8<PCM_DTYPE_F32> {
         b = *(const row_u32x4_e4 *)(p + 4);
     }
     __device__ __forceinline__ void lowest() { a = b = 0xFF800000u; }
+    __device__ __forceinline__ void drop(int i) { set(i, -INFINITY); }
+    static __device__ __forceinline__ void store(float *p, const float *v) {
+        row_u32x4 x, y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = __float_as_uint(v[i]);
+            y[i] = __float_as_uint(v[4 + i]);
+        }
+        *(row_u32x4_e4 *)p = x;
+        *(row_u32x4_e4 *)(p + 4) = y;
+    }
     __device__ __forceinline__ void set(int i, float v) {
         if (i < 4) a[i] = __float_as_uint(v); else b[i - 4] = __float_as_uint(v);
     }
@@ -183,6 +222,19 @@ template <> struct Row8<PCM_DTYPE_BF16> {
         a = *(const row_u32x4_e2 *)p;
     }
     __device__ __forceinline__ void lowest() { a = 0xFF80FF80u; }
+    __device__ __forceinline__ void drop(int i) { set(i, (__bf16)-INFINITY); }
+    static __device__ __forceinline__ void store(__bf16 *p, const float *v) {
+        row_u32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned short lo =
+                __builtin_bit_cast(unsigned short, (__bf16)v[2 * i]);
+            const unsigned short hi =
+                __builtin_bit_cast(unsigned short, (__bf16)v[2 * i + 1]);
+            x[i] = lo | (unsigned)hi << 16;
+        }
+        *(row_u32x4_e2 *)p = x;
+    }
     __device__ __forceinline__ void set(int i, __bf16 v) {
         const unsigned u = __builtin_bit_cast(unsigned short, v);
         a[i >> 1] = i & 1 ? (a[i >> 1] & 0xffffu) | (u << 16)
@@ -198,6 +250,19 @@ template <> struct Row8<PCM_DTYPE_F16> {
         a = *(const row_u32x4_e2 *)p;
     }
     __device__ __forceinline__ void lowest() { a = 0xFC00FC00u; }
+    __device__ __forceinline__ void drop(int i) { set(i, (_Float16)-INFINITY); }
+    static __device__ __forceinline__ void store(_Float16 *p, const float *v) {
+        row_u32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned short lo =
+                __builtin_bit_cast(unsigned short, (_Float16)v[2 * i]);
+            const unsigned short hi =
+                __builtin_bit_cast(unsigned short, (_Float16)v[2 * i + 1]);
+            x[i] = lo | (unsigned)hi << 16;
+        }
+        *(row_u32x4_e2 *)p = x;
+    }
     __device__ __forceinline__ void set(int i, _Float16 v) {
         const unsigned u = __builtin_bit_cast(unsigned short, v);
         a[i >> 1] = i & 1 ? (a[i >> 1] & 0xffffu) | (u << 16)

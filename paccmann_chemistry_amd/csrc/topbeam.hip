@@ -98,34 +98,6 @@ __device__ __forceinline__ double top_of_regs(const RowRegs<DT, NT, G> &x,
     return top_of_list<NT>(buf, found, lds.list, lane, wave);
 }
 
-// block-wide maximum / sum, every thread gets it
-template <int NT, typename T>
-__device__ __forceinline__ T all_max(T v, T *red, int tid) {
-    v = wave_max(v);
-    if constexpr (NT > 64) {
-        __syncthreads();
-        if ((tid & 63) == 0) red[tid >> 6] = v;
-        __syncthreads();
-        v = red[0];
-#pragma unroll
-        for (int i = 1; i < NT / 64; ++i) v = pcm_max(v, red[i]);
-    }
-    return v;
-}
-template <int NT, typename T>
-__device__ __forceinline__ T all_sum(T v, T *red, int tid) {
-    v = wave_sum(v);
-    if constexpr (NT > 64) {
-        __syncthreads();
-        if ((tid & 63) == 0) red[tid >> 6] = v;
-        __syncthreads();
-        v = red[0];
-#pragma unroll
-        for (int i = 1; i < NT / 64; ++i) v += red[i];
-    }
-    return v;
-}
-
 // ---- top logits -------------------------------------------------------------------
 struct TopArgs {
     const void *logits;
