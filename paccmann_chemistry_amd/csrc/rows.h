@@ -187,6 +187,7 @@ static __device__ __forceinline__ double key_lane(double v, int lane) {
 // Kept as they lie in memory (16-bit types packed) and widened where they are
 // used.  A row starts at any element: the loads are 16 bytes wide and aligned to
 // the element only, which global memory takes.
+typedef unsigned row_u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned row_u32x4 __attribute__((ext_vector_type(4)));
 typedef row_u32x4 row_u32x4_e2 __attribute__((aligned(2)));
 typedef row_u32x4 row_u32x4_e4 __attribute__((aligned(4)));

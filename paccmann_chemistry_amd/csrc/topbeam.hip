@@ -491,42 +491,71 @@ RowPlan row_plan(long long rows, int V) {
     } while (0)
 
 // ---- states follow their beams ------------------------------------------------------
+struct ReorderState {
+    char *data;
+    long long outer_stride, row_stride;
+    unsigned units, per_row;   // of 16 .. 1 bytes: of all outer indices; of one
+    unsigned magic, shift;     // o = unit / per_row
+    int bytes;                 // of a unit
+};
 struct ReorderArgs {
     const int32_t *parents;
     int32_t *status;
     int beams, batch, count;
-    int split;                        // blocks per batch row
-    int unit[PCM_MAX_STATES];         // bytes a thread moves at once
-    long long chunks[PCM_MAX_STATES]; // units of all outer indices of one row
-    long long per_row[PCM_MAX_STATES];
-    pcm_state s[PCM_MAX_STATES];
+    int split;                 // blocks per batch row
+    ReorderState s[PCM_MAX_STATES];
 };
 
-// A thread owns one unit of one batch row in ALL beams: it loads what every
-// beam will hold before it stores any of it, so the move is in place whatever
-// the parents are.
-template <typename U>
-__device__ void reorder_unit(char *at, long long beam_stride, const int *par,
-                             int beams) {
-    U v[PCM_BEAM_MAX];
+// A thread owns the same units of one batch row in ALL beams: it loads what
+// every beam will hold before it stores any of it, so the move is in place
+// whatever the parents are.  K bounds the beams (the arrays stay in registers),
+// N units are in flight at once; the parents are the same for the whole block,
+// so a beam that keeps its row costs a scalar branch.
+template <typename U, int K, int N>
+__device__ __forceinline__ void reorder_units(const ReorderState &s, int b,
+                                              long long beam_stride,
+                                              const int (&par)[K], unsigned first,
+                                              unsigned step) {
+    for (unsigned c0 = first; c0 < s.units; c0 += N * step) {
+        U v[N][K];
+        char *at[N];
 #pragma unroll
-    for (int k = 0; k < PCM_BEAM_MAX; ++k)
-        if (k < beams && par[k] != k)
-            v[k] = *(const U *)(at + par[k] * beam_stride);
+        for (int n = 0; n < N; ++n) {
+            const unsigned c = c0 + n * step;
+            const unsigned o = s.per_row == s.units ? 0u
+                               : s.per_row == 1 ? c
+                               : __umulhi(c, s.magic) >> s.shift;
+            at[n] = s.data + (long long)o * s.outer_stride +
+                    (long long)b * s.row_stride +
+                    (long long)(c - o * s.per_row) * sizeof(U);
+            if (c < s.units) {
 #pragma unroll
-    for (int k = 0; k < PCM_BEAM_MAX; ++k)
-        if (k < beams && par[k] != k) *(U *)(at + k * beam_stride) = v[k];
+                for (int k = 0; k < K; ++k)
+                    if (par[k] != k) v[n][k] = *(const U *)(at[n] + par[k] * beam_stride);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (c0 + n * step < s.units) {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (par[k] != k) *(U *)(at[n] + k * beam_stride) = v[n][k];
+            }
+    }
 }
 
+template <int K>
 __global__ __launch_bounds__(256) void reorder_kernel(ReorderArgs a) {
+    constexpr int N = K <= 4 ? 4 : K <= 8 ? 2 : 1;
     const int b = blockIdx.x / a.split, part = blockIdx.x - b * a.split;
-    int par[PCM_BEAM_MAX];
+    int par[K];
     bool moves = false;
 #pragma unroll
-    for (int k = 0; k < PCM_BEAM_MAX; ++k) {
+    for (int k = 0; k < K; ++k) {
         par[k] = k;
         if (k < a.beams) {
-            const int p = a.parents[(long long)k * a.batch + b];
+            const int p = __builtin_amdgcn_readfirstlane(
+                a.parents[(long long)k * a.batch + b]);
             if (p >= 0 && p < a.beams) par[k] = p;
             else if (a.status && threadIdx.x == 0 && part == 0)
                 atomicOr(a.status, PCM_STATUS_BAD_PARENT);
@@ -534,21 +563,16 @@ __global__ __launch_bounds__(256) void reorder_kernel(ReorderArgs a) {
         }
     }
     if (!moves) return;
+    const unsigned first = part * 256 + threadIdx.x, step = a.split * 256;
     for (int i = 0; i < a.count; ++i) {
-        const pcm_state &s = a.s[i];
+        const ReorderState &s = a.s[i];
         const long long stride = s.row_stride * a.batch;
-        for (long long c = (long long)part * 256 + threadIdx.x;
-             c < a.chunks[i]; c += (long long)a.split * 256) {
-            const long long o = c / a.per_row[i], e = c - o * a.per_row[i];
-            char *at = (char *)s.data + o * s.outer_stride +
-                       b * s.row_stride + e * a.unit[i];
-            switch (a.unit[i]) {
-            case 16: reorder_unit<uint4>(at, stride, par, a.beams); break;
-            case 8: reorder_unit<uint2>(at, stride, par, a.beams); break;
-            case 4: reorder_unit<unsigned>(at, stride, par, a.beams); break;
-            case 2: reorder_unit<unsigned short>(at, stride, par, a.beams); break;
-            default: reorder_unit<unsigned char>(at, stride, par, a.beams); break;
-            }
+        switch (s.bytes) {
+        case 16: reorder_units<row_u32x4, K, N>(s, b, stride, par, first, step); break;
+        case 8: reorder_units<row_u32x2, K, N>(s, b, stride, par, first, step); break;
+        case 4: reorder_units<unsigned, K, N>(s, b, stride, par, first, step); break;
+        case 2: reorder_units<unsigned short, K, N>(s, b, stride, par, first, step); break;
+        default: reorder_units<unsigned char, K, N>(s, b, stride, par, first, step); break;
         }
     }
 }
@@ -777,11 +801,27 @@ int pcm_reorder_states(const int32_t *parents, int32_t beams, int32_t batch,
             (unsigned long long)s.row_stride |
             (s.outer > 1 ? (unsigned long long)s.outer_stride : 0ull);
         while (bits & (unit - 1)) unit >>= 1;
-        a.s[n] = s;
-        a.unit[n] = unit;
-        a.per_row[n] = s.row_bytes / unit;
-        a.chunks[n] = a.per_row[n] * s.outer;
-        most = a.chunks[n] > most ? a.chunks[n] : most;
+        const long long per_row = s.row_bytes / unit;
+        const long long units = per_row * s.outer;
+        PCM_REQUIRE(units < (1ll << 30), PCM_EINVAL,
+                    "reorder_states: state %d has rows of %lld pieces of %d "
+                    "bytes (2^30 at most)", i, units, unit);
+        ReorderState &q = a.s[n];
+        q.data = (char *)s.data;
+        q.outer_stride = s.outer > 1 ? s.outer_stride : 0;
+        q.row_stride = s.row_stride;
+        q.units = (unsigned)units;
+        q.per_row = (unsigned)per_row;
+        q.bytes = unit;
+        // c / per_row for c < 2^31: a multiplication by ceil(2^(32 + l) / per_row),
+        // 2^l < per_row <= 2^(l + 1)
+        int l = 0;
+        while ((2ll << l) < per_row) ++l;
+        q.shift = l;
+        q.magic = per_row > 1
+                      ? (unsigned)(((1ull << (32 + l)) + per_row - 1) / per_row)
+                      : 0;
+        most = units > most ? units : most;
         a.count = n + 1;
     }
     // enough blocks per batch row to spread a small batch over the chip
@@ -790,8 +830,16 @@ int pcm_reorder_states(const int32_t *parents, int32_t beams, int32_t batch,
     if (split > want) split = want;
     if (split < 1) split = 1;
     a.split = (int)split;
-    hipLaunchKernelGGL(reorder_kernel, dim3((unsigned)(split * batch)),
-                       dim3(256), 0, (hipStream_t)stream, a);
+    const dim3 grid((unsigned)(split * batch));
+#define PCM_REORDER(K) \
+    hipLaunchKernelGGL(reorder_kernel<K>, grid, dim3(256), 0, (hipStream_t)stream, a)
+    if (beams <= 2) PCM_REORDER(2);
+    else if (beams <= 3) PCM_REORDER(3);
+    else if (beams <= 4) PCM_REORDER(4);
+    else if (beams <= 6) PCM_REORDER(6);
+    else if (beams <= 8) PCM_REORDER(8);
+    else PCM_REORDER(16);
+#undef PCM_REORDER
     return pcm_check_launch("reorder_states");
 }
 
