@@ -98,6 +98,100 @@ __device__ __forceinline__ double top_of_regs(const RowRegs<DT, NT, G> &x,
     return top_of_list<NT>(buf, found, lds.list, lane, wave);
 }
 
+// ---- the largest of a short row ---------------------------------------------------
+// LPR lanes share a row, each sorts what it holds into a list of KT by insertion
+// (two instructions per place: v_max_f64, v_min_f64), then the lanes' lists are
+// merged pairwise; every lane ends with the row's list.  A row of 60 costs about
+// 30 instructions of a wave this way (16 rows in it) against 800 for a wave per
+// row.  All elements are ranked, -inf and NaN too.
+template <int KT> struct ShortTop {
+    double l[KT];
+    __device__ __forceinline__ void add(double key) {
+#pragma unroll
+        for (int j = 0; j < KT; ++j) {
+            const double hi = fmax(l[j], key);
+            key = fmin(l[j], key);
+            l[j] = hi;
+        }
+    }
+    template <int M> __device__ __forceinline__ void merge() {
+        double o[KT];
+#pragma unroll
+        for (int j = 0; j < KT; ++j) o[j] = lane_xor<M>(l[j]);
+#pragma unroll
+        for (int j = 0; j < KT; ++j) l[j] = fmax(l[j], o[KT - 1 - j]);
+#pragma unroll
+        for (int s = KT / 2; s > 0; s >>= 1)
+#pragma unroll
+            for (int j = 0; j < KT; ++j)
+                if ((j & s) == 0) {
+                    const double hi = fmax(l[j], l[j + s]);
+                    l[j + s] = fmin(l[j], l[j + s]);
+                    l[j] = hi;
+                }
+    }
+    template <int DT, int LPR, int G>
+    __device__ __forceinline__ void of(const RowRegs<DT, LPR, G> &x, int V,
+                                       int sub) {
+#pragma unroll
+        for (int j = 0; j < KT; ++j) l[j] = KEY_NONE;
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int at = x.at(g, sub) + j;
+                const double key = key_of(x.r[g].get(j), at);
+                add(at < V ? key : KEY_NONE);
+            }
+        merge<1>();
+        merge<2>();
+        if constexpr (LPR == 16) {
+            merge<4>();
+            merge<8>();
+        }
+    }
+};
+// reductions over the LPR lanes of a row
+template <int LPR, typename T>
+__device__ __forceinline__ T row_max(T v) {
+    v = pcm_max(v, lane_xor<1>(v));
+    v = pcm_max(v, lane_xor<2>(v));
+    if constexpr (LPR == 16) {
+        v = pcm_max(v, lane_xor<4>(v));
+        v = pcm_max(v, lane_xor<8>(v));
+    }
+    return v;
+}
+template <int LPR, typename T>
+__device__ __forceinline__ T row_sum(T v) {
+    v += lane_xor<1>(v);
+    v += lane_xor<2>(v);
+    if constexpr (LPR == 16) {
+        v += lane_xor<4>(v);
+        v += lane_xor<8>(v);
+    }
+    return v;
+}
+// run the call with the constants LPR (lanes per row), G (groups of eight per
+// lane) and KT (list) for rows of V <= 512 and lists of k <= 16
+#define PCM_BY_SHORT_LIST(k, ...)                                     \
+    do {                                                              \
+        if ((k) <= 4) { constexpr int KT = 4; __VA_ARGS__; }          \
+        else if ((k) <= 8) { constexpr int KT = 8; __VA_ARGS__; }     \
+        else { constexpr int KT = 16; __VA_ARGS__; }                  \
+    } while (0)
+#define PCM_BY_SHORT(V, k, ...)                                               \
+    do {                                                                      \
+        if ((V) <= 64) {                                                      \
+            constexpr int LPR = 4, G = 2; PCM_BY_SHORT_LIST(k, __VA_ARGS__);  \
+        } else if ((V) <= 128) {                                              \
+            constexpr int LPR = 4, G = 4; PCM_BY_SHORT_LIST(k, __VA_ARGS__);  \
+        } else {                                                              \
+            constexpr int LPR = 16, G = 4; PCM_BY_SHORT_LIST(k, __VA_ARGS__); \
+        }                                                                     \
+    } while (0)
+constexpr int SHORT_ROW = 512, SHORT_LIST = 16;
+
 // ---- top logits -------------------------------------------------------------------
 struct TopArgs {
     const void *logits;
@@ -136,6 +230,59 @@ __device__ void top_fill(const typename RowType<DT>::T *x, int V, int have, int 
 __device__ __forceinline__ float top_rest(float m, float s, float inv_t) {
     if (s != s) return s;
     return isinf(m) ? m : m * inv_t + logf(s);
+}
+
+// Rows of at most 512, lists of at most 16.
+template <int DT, int LPR, int G, int KT>
+__global__ __launch_bounds__(256) void top_short_kernel(TopArgs a, long long rows) {
+    typedef RowType<DT> R;
+    typedef typename R::T T;
+    const int sub = threadIdx.x % LPR;
+    const long long row =
+        (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+    if (row >= rows) return;   // (all lanes of a row)
+    RowRegs<DT, LPR, G> x;
+    x.load((const T *)a.logits + row * a.ld, a.V, sub);
+    ShortTop<KT> top;
+    top.template of<DT, LPR, G>(x, a.V, sub);
+    T *values = (T *)a.values + row * a.k;
+    int32_t *indices = a.indices + row * a.k;
+    double last = top.l[0];
+#pragma unroll
+    for (int j = 0; j < KT; ++j)
+        if (j < a.k) {
+            last = top.l[j];
+            if (j % LPR == sub) {
+                values[j] = R::down(key_value(last));
+                indices[j] = key_index(last);
+            }
+        }
+    const float last_v = key_value(last);
+    const int last_i = key_index(last);
+    float m = -INFINITY;
+    bool nan = false;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = x.r[g].get(j);
+            nan |= v != v;
+            if (v < last_v || (v == last_v && x.at(g, sub) + j > last_i))
+                m = fmaxf(m, v);
+        }
+    m = row_max<LPR>(nan ? INFINITY : m);
+    const float mm = isinf(m) ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = x.r[g].get(j);
+            if (!(v > last_v || (v == last_v && x.at(g, sub) + j <= last_i)))
+                s += __builtin_amdgcn_exp2f((v - mm) * a.scale);
+        }
+    s = row_sum<LPR>(s);
+    if (sub == 0) a.rest[row] = top_rest(m, s, a.inv_t);
 }
 
 // One block per row, or per part of a row.
@@ -455,6 +602,93 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
     }
 }
 
+// Short rows, everything in one launch: a block takes 64 / LPR batch rows, one
+// wave per beam; a candidate's place is the number of better ones.
+template <int DT, int LPR, int G, int KT>
+__global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
+    typedef typename RowType<DT>::T T;
+    constexpr int RB = 64 / LPR;
+    extern __shared__ double beam_c[];        // [RB][beams * width] scores
+    const int per = a.beams * a.width;
+    int *beam_f = (int *)(beam_c + RB * per); // ... beam * V + token
+    const int lane = threadIdx.x & 63, sub = lane % LPR, rb = lane / LPR;
+    const int k = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.x * RB + rb;
+    if (b < a.batch) {
+        const long long row = (long long)k * a.batch + b;
+        const double score = a.scores[row];
+        const bool done = a.finished && a.finished[row];
+        double lse = 0.;
+        bool live = !done && score > -INFINITY;
+        ShortTop<KT> top;
+        if (live) {
+            RowRegs<DT, LPR, G> x;
+            x.load((const T *)a.logits + row * a.ld, a.V, sub);
+            top.template of<DT, LPR, G>(x, a.V, sub);
+            bool nan = false;
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float v = x.r[g].get(j);
+                    nan |= v != v;
+                }
+            // (the list's first is the maximum; a NaN anywhere ends the row)
+            const float m = row_max<LPR>(nan ? INFINITY : key_value(top.l[0]));
+            live = !isinf(m);
+            if (live) {
+                double s = 0.;
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        s += exp2_64(((double)x.r[g].get(j) - (double)m) *
+                                     a.scale);
+                s = row_sum<LPR>(s);
+                lse = (double)m * a.inv_t + log(s);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+            if (j < a.width && j % LPR == sub) {
+                int tok = j;   // a row without a distribution: tokens in order
+                double c = -INFINITY;
+                if (done) {    // end_token, then the others in order
+                    tok = j == 0 ? a.end : j - 1 + (j - 1 >= a.end ? 1 : 0);
+                    if (j == 0 && score == score) c = score;
+                } else if (live) {
+                    tok = top.l[j] > KEY_NONE ? key_index(top.l[j]) : a.V;
+                    c = score + ((double)key_value(top.l[j]) * a.inv_t - lse);
+                }
+                const int at = rb * per + k * a.width + j;
+                beam_c[at] = tok < a.V ? c : -INFINITY;
+                beam_f[at] = tok < a.V ? k * a.V + tok : 0x7fffffff;
+            }
+    }
+    __syncthreads();
+    const int rows = min(RB, a.batch - (int)blockIdx.x * RB);
+    for (int i = threadIdx.x; i < rows * per; i += blockDim.x) {
+        const int r = i / per;
+        const double c = beam_c[i];
+        const int f = beam_f[i];
+        int place = 0;
+        for (int j = r * per; j < (r + 1) * per; ++j)
+            place += beam_c[j] > c || (beam_c[j] == c && beam_f[j] < f);
+        if (place < a.width) {
+            const int from = f / a.V, t = f - from * a.V;
+            const int bb = blockIdx.x * RB + r;
+            const long long o = (long long)place * a.batch + bb;
+            a.tokens[o] = t;
+            a.parents[o] = from;
+            a.scores_out[o] = c;
+            if (a.finished_out)
+                a.finished_out[o] =
+                    (a.finished && a.finished[(long long)from * a.batch + bb]) ||
+                    t == a.end;
+        }
+    }
+}
+
 // How a row of V logits is dealt out: `parts` blocks of `len` elements each.
 // A block holds its elements in registers (65536 at most).  Few rows leave most
 // of the 256 CUs idle, so long ones are split until there are about 512 blocks
@@ -478,16 +712,16 @@ RowPlan row_plan(long long rows, int V) {
 }
 // run `call` with the constants NT (threads) and G (groups of eight per thread)
 // for a stretch of `len` elements
-#define PCM_BY_LENGTH(len, call)                                         \
+#define PCM_BY_LENGTH(len, ...)                                          \
     do {                                                                 \
-        if ((len) <= 512) { constexpr int NT = 64, G = 1; call; }        \
-        else if ((len) <= 1024) { constexpr int NT = 64, G = 2; call; }  \
-        else if ((len) <= 2048) { constexpr int NT = 256, G = 1; call; } \
-        else if ((len) <= 4096) { constexpr int NT = 256, G = 2; call; } \
-        else if ((len) <= 8192) { constexpr int NT = 256, G = 4; call; } \
-        else if ((len) <= 16384) { constexpr int NT = 512, G = 4; call; } \
-        else if ((len) <= 32768) { constexpr int NT = 1024, G = 4; call; } \
-        else { constexpr int NT = 1024, G = 8; call; }                   \
+        if ((len) <= 512) { constexpr int NT = 64, G = 1; __VA_ARGS__; }        \
+        else if ((len) <= 1024) { constexpr int NT = 64, G = 2; __VA_ARGS__; }  \
+        else if ((len) <= 2048) { constexpr int NT = 256, G = 1; __VA_ARGS__; } \
+        else if ((len) <= 4096) { constexpr int NT = 256, G = 2; __VA_ARGS__; } \
+        else if ((len) <= 8192) { constexpr int NT = 256, G = 4; __VA_ARGS__; } \
+        else if ((len) <= 16384) { constexpr int NT = 512, G = 4; __VA_ARGS__; } \
+        else if ((len) <= 32768) { constexpr int NT = 1024, G = 4; __VA_ARGS__; } \
+        else { constexpr int NT = 1024, G = 8; __VA_ARGS__; }                   \
     } while (0)
 
 // ---- states follow their beams ------------------------------------------------------
@@ -668,6 +902,15 @@ int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
     a.inv_t = (float)(1.0 / temperature);
     PCM_REQUIRE(rows * plan.parts < (1ll << 31), PCM_EINVAL,
                 "top_logits: too many rows");
+    if (vocab <= SHORT_ROW && k <= SHORT_LIST) {
+        PCM_BY_DTYPE(dtype, PCM_BY_SHORT(vocab, k, {
+            constexpr int per_block = 256 / LPR;
+            hipLaunchKernelGGL((top_short_kernel<DT, LPR, G, KT>),
+                               dim3((unsigned)((rows + per_block - 1) / per_block)),
+                               dim3(256), 0, st, a, (long long)rows);
+        }));
+        return pcm_check_launch("top_logits");
+    }
     PCM_BY_DTYPE(dtype, PCM_BY_LENGTH(plan.len, {
         hipLaunchKernelGGL((top_kernel<DT, NT, G>),
                            dim3((unsigned)(rows * plan.parts)), dim3(NT),
@@ -686,6 +929,7 @@ size_t pcm_beam_select_workspace_bytes(int32_t beams, int32_t batch,
     if (beams < 1 || batch < 1 || width < 1 || vocab < 1 ||
         vocab > PCM_MAX_VOCAB)
         return 0;
+    if (vocab <= SHORT_ROW) return 0;
     const size_t rows = (size_t)beams * batch;
     return rows * row_plan(rows, vocab).parts * (width + 2) * sizeof(double);
 }
@@ -723,7 +967,7 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
                 "in [0, %d), got %d", vocab, end_token);
     const size_t need =
         pcm_beam_select_workspace_bytes(beams, batch, vocab, width);
-    PCM_REQUIRE(workspace && workspace_bytes >= need, PCM_ENOMEM,
+    PCM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), PCM_ENOMEM,
                 "beam_select: workspace %zu < %zu bytes", workspace_bytes, need);
     PCM_REQUIRE(((uintptr_t)workspace & 7) == 0, PCM_EINVAL,
                 "beam_select: workspace must be 8-byte aligned");
@@ -742,6 +986,17 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
     a.parts = plan.parts; a.len = plan.len; a.end = end_token;
     a.inv_t = 1.0 / temperature;
     a.scale = 1.4426950408889634 / temperature;
+    if (vocab <= SHORT_ROW) {
+        PCM_BY_DTYPE(dtype, PCM_BY_SHORT(vocab, width, {
+            constexpr int per_block = 64 / LPR;
+            const size_t lds = (size_t)per_block * beams * width *
+                               (sizeof(double) + sizeof(int));
+            hipLaunchKernelGGL((beam_short_kernel<DT, LPR, G, KT>),
+                               dim3((unsigned)((batch + per_block - 1) / per_block)),
+                               dim3(64 * beams), lds, st, a);
+        }));
+        return pcm_check_launch("beam_select");
+    }
     PCM_BY_DTYPE(dtype, PCM_BY_LENGTH(plan.len, {
         hipLaunchKernelGGL((beam_rows_kernel<DT, NT, G>),
                            dim3((unsigned)(rows * plan.parts)), dim3(NT),
