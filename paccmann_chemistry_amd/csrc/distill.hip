@@ -313,7 +313,8 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
 // -- a group of eight elements is one byte of it -- and become -inf in the
 // registers, so the passes see the others only.
 template <int DT, int NT, int G, bool HARD, bool KEEP>
-__global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
+__global__ __launch_bounds__(NT, KEEP ? row_waves(DT, NT, G) : 8) void
+distill_row_kernel(DistillArgs a) {
     typedef RowType<DT> R;
     typedef typename R::T T;
     extern __shared__ unsigned marks[];   // a bit per element
@@ -381,15 +382,12 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
             }
         }
         const unsigned bits = mark8[g * NT + tid];
-        if (bits) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (bits >> j & 1) q.drop(j);
-        }
+        if (bits) q.drop(bits);
     };
     if (KEEP) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
+            regs.r[g].touch();
             group(g, regs.r[g]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) m = fmaxf(m, regs.r[g].get(j));
@@ -458,7 +456,10 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
     };
     if (KEEP) {
 #pragma unroll
-        for (int g = 0; g < G; ++g) add(regs.r[g]);
+        for (int g = 0; g < G; ++g) {
+            regs.r[g].touch();
+            add(regs.r[g]);
+        }
     } else {
         for (int g = 0; g < groups; ++g) {
             Row8<DT> q;
@@ -502,7 +503,10 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
     };
     if (KEEP) {
 #pragma unroll
-        for (int g = 0; g < G; ++g) write(g, regs.r[g]);
+        for (int g = 0; g < G; ++g) {
+            regs.r[g].touch();
+            write(g, regs.r[g]);
+        }
     } else {
         for (int g = 0; g < groups; ++g) {
             Row8<DT> q;

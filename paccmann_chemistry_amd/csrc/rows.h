@@ -199,7 +199,16 @@ template <> struct Row8<PCM_DTYPE_F32> {
         b = *(const row_u32x4_e4 *)(p + 4);
     }
     __device__ __forceinline__ void lowest() { a = b = 0xFF800000u; }
-    __device__ __forceinline__ void drop(int i) { set(i, -INFINITY); }
+    // -inf in the places of the bits
+    __device__ __forceinline__ void drop(unsigned bits) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (bits >> i & 1) set(i, -INFINITY);
+    }
+    // what is derived from the elements is derived after this: a pass over a row
+    // that touches each group before it uses it neither keeps values widened by an
+    // earlier pass in registers nor widens all groups at once
+    __device__ __forceinline__ void touch() { asm volatile("" : "+v"(a), "+v"(b)); }
     static __device__ __forceinline__ void store(float *p, const float *v) {
         row_u32x4 x, y;
 #pragma unroll
@@ -223,7 +232,12 @@ template <> struct Row8<PCM_DTYPE_BF16> {
         a = *(const row_u32x4_e2 *)p;
     }
     __device__ __forceinline__ void lowest() { a = 0xFF80FF80u; }
-    __device__ __forceinline__ void drop(int i) { set(i, (__bf16)-INFINITY); }
+    __device__ __forceinline__ void drop(unsigned bits) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (bits >> i & 1) set(i, (__bf16)-INFINITY);
+    }
+    __device__ __forceinline__ void touch() { asm volatile("" : "+v"(a)); }
     static __device__ __forceinline__ void store(__bf16 *p, const float *v) {
         row_u32x4 x;
 #pragma unroll
@@ -251,7 +265,12 @@ template <> struct Row8<PCM_DTYPE_F16> {
         a = *(const row_u32x4_e2 *)p;
     }
     __device__ __forceinline__ void lowest() { a = 0xFC00FC00u; }
-    __device__ __forceinline__ void drop(int i) { set(i, (_Float16)-INFINITY); }
+    __device__ __forceinline__ void drop(unsigned bits) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (bits >> i & 1) set(i, (_Float16)-INFINITY);
+    }
+    __device__ __forceinline__ void touch() { asm volatile("" : "+v"(a)); }
     static __device__ __forceinline__ void store(_Float16 *p, const float *v) {
         row_u32x4 x;
 #pragma unroll
@@ -275,6 +294,13 @@ template <> struct Row8<PCM_DTYPE_F16> {
         return (float)__builtin_bit_cast(_Float16, u);
     }
 };
+
+// Waves per SIMD that a kernel is to leave room for: two blocks of 1024 threads
+// per CU where the row takes at most 32 registers of the 64 that this leaves, so
+// that one block loads while the other computes.
+constexpr int row_waves(int dt, int nt, int g) {
+    return nt * (dt == PCM_DTYPE_F32 ? 2 * g : g) <= 8192 ? 8 : 4;
+}
 
 // n elements of a row, dealt to NT threads in groups of eight: element j of
 // group g of thread tid is (g * NT + tid) * 8 + j.  What lies past n is -inf.

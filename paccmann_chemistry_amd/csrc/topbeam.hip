@@ -6,20 +6,63 @@
 namespace {
 
 // ---- the largest of a stretch -------------------------------------------------------
-// NT threads find the k <= 64 largest keys of n elements they hold in registers.
-// Only elements above -inf are looked at (NaN is not): where there are fewer
-// than k of them the caller fills up.
-//   1. every thread knows its own first maximum; the waves sort theirs (64
-//      keys, in registers) and merge them pairwise, keeping 64: the k-th largest
-//      of the threads' maxima is a lower bound of the k-th largest element;
-//   2. at most k threads hold anything at or above it: those append what they
-//      have (k * 8 G keys at most, k and a few as a rule) to a list in LDS;
+// NT threads find the k <= 64 largest keys of n elements in one pass over memory
+// and a second look at the few threads that hold them.  Only elements above
+// -inf are looked at (NaN is not): where there are fewer than k of them the caller
+// fills up.
+//   1. in the pass every thread keeps its maximum and the group of eight where
+//      it first appeared: the key (maximum, last index of that group) is not above
+//      the thread's largest one.  The waves sort theirs (64, in registers) and
+//      merge them pairwise, keeping 64: the k-th largest is a bound that k
+//      elements reach, all of them in the (at most) k threads whose own key does;
+//   2. a wave reads such a thread's elements again, one per lane, and appends
+//      those at or above the bound to a list in LDS: k and a few as a rule;
 //   3. the list is sorted, 64 at a time.
-// Keys are distinct, so the result does not depend on the order in 2.
+// Keys are distinct, so the order in 2 does not matter, and ties take no special
+// path.  A list that overflows (k - 1 threads full of large elements) is made
+// by k passes instead.
+constexpr int top_room(int nt) { return nt == 64 ? 256 : 1024; }
 template <int NT> struct TopLds {
     double list[NT / 64][64];
-    int count;
+    double buf[top_room(NT)];
+    int held[64];    // threads that reach the bound
+    int holders, count;
 };
+
+// every group of eight elements of the stretch, f(elements, group): thread tid
+// has the groups at (g * NT + tid) * 8; four loads in flight
+template <int DT, int NT, typename F>
+__device__ __forceinline__ void each_group(const typename RowType<DT>::T *p, int n,
+                                           int tid, F f) {
+    constexpr int U = 4;
+    int g = 0;
+    for (; (g + U) * NT * 8 <= n; g += U) {
+        Row8<DT> q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u].load(p + ((g + u) * NT + tid) * 8);
+#pragma unroll
+        for (int u = 0; u < U; ++u) f(q[u], g + u);
+    }
+    for (; g * NT * 8 < n; ++g) {
+        const int e = (g * NT + tid) * 8;
+        Row8<DT> q;
+        if (e + 8 <= n) {
+            q.load(p + e);
+        } else {
+            q.lowest();
+#pragma unroll
+            for (int j = 0; j < 7; ++j)
+                if (e + j < n) q.set(j, p[e + j]);
+        }
+        f(q, g);
+    }
+}
+// element of thread `holder` that `lane` looks at when a wave reads eight of its
+// groups from g0 on
+template <int NT>
+__device__ __forceinline__ int held_at(int g0, int holder, int lane) {
+    return ((g0 + (lane >> 3)) * NT + holder) * 8 + (lane & 7);
+}
 
 // the 64 largest of the waves' sorted lists; in wave 0 afterwards
 template <int NT>
@@ -53,49 +96,80 @@ __device__ __forceinline__ double top_of_list(const double *keys, int n,
     return v;
 }
 
-// returns in wave 0: lane j holds the j-th largest key (KEY_NONE past `found`);
-// `found` (all threads): how many elements were at or above the bound.
-template <int DT, int NT, int G>
-__device__ __forceinline__ double top_of_regs(const RowRegs<DT, NT, G> &x,
-                                              int first, int k, TopLds<NT> &lds,
-                                              double *buf, int tid, int &found) {
-    const int lane = tid & 63, wave = tid >> 6;
-    float bv = -INFINITY;
-    int bi = 0;
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float v = x.r[g].get(j);
-            if (v > bv) { bv = v; bi = x.at(g, tid) + j; }
-        }
-    if (tid == 0) lds.count = 0;
-    double key = bv > -INFINITY ? key_of(bv, first + bi) : KEY_NONE;
+// the k-th largest of one key per thread, known to all
+template <int NT>
+__device__ __forceinline__ double bound_of(double key, int k, TopLds<NT> &lds,
+                                           int lane, int wave) {
     key = key_sort(key, lane);
     key = merge_waves<NT>(key, lds.list, lane, wave);
-    double bound;
     if constexpr (NT > 64) {
         if (wave == 0 && lane == k - 1) lds.list[0][0] = key;
         __syncthreads();
-        bound = lds.list[0][0];
+        key = lds.list[0][0];
     } else {
-        bound = key_lane(key, k - 1);
-        __syncthreads();
+        key = key_lane(key, k - 1);
     }
-    const float bound_v = bound == KEY_NONE ? -INFINITY : key_value(bound);
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float v = x.r[g].get(j);
-            if (v >= bound_v && v > -INFINITY) {
-                const double e = key_of(v, first + x.at(g, tid) + j);
-                if (e >= bound) buf[atomicAdd(&lds.count, 1)] = e;
+    __syncthreads();   // (lds.count, and the lists are free again)
+    return key;
+}
+
+// Steps 1 (from the threads' maxima on) to 3.  bv, bg: the thread's maximum and
+// the group where it first appeared.  Returns in wave 0: lane j holds the j-th
+// largest key (KEY_NONE past `found`).  `slot`: the thread's place among the
+// holders, -1 if it holds none of the k largest.
+template <int DT, int NT>
+__device__ __forceinline__ double top_of_threads(
+    const typename RowType<DT>::T *p, int n, int first, int k, float bv, int bg,
+    TopLds<NT> &lds, int tid, int &found, int &slot) {
+    typedef RowType<DT> R;
+    const int lane = tid & 63, wave = tid >> 6;
+    if (tid == 0) lds.count = lds.holders = 0;
+    const double key = bv > -INFINITY
+                           ? key_of(bv, first + (bg * NT + tid) * 8 + 7)
+                           : KEY_NONE;
+    const double bound = bound_of<NT>(key, k, lds, lane, wave);
+    slot = -1;
+    if (key > KEY_NONE && key >= bound) {
+        slot = atomicAdd(&lds.holders, 1);
+        lds.held[slot] = tid;
+    }
+    __syncthreads();
+    const int holders = lds.holders;
+    for (int i = wave; i < holders; i += NT / 64) {
+        const int holder = lds.held[i];
+        for (int g0 = 0; g0 * NT * 8 < n; g0 += 8) {
+            const int e = held_at<NT>(g0, holder, lane);
+            const float v = e < n ? R::up(p[e]) : -INFINITY;
+            if (v > -INFINITY) {
+                const double ek = key_of(v, first + e);
+                if (ek >= bound) {
+                    const int at = atomicAdd(&lds.count, 1);
+                    if (at < top_room(NT)) lds.buf[at] = ek;
+                }
             }
         }
+    }
     __syncthreads();
     found = lds.count;
-    return top_of_list<NT>(buf, found, lds.list, lane, wave);
+    if (found > top_room(NT)) {
+        double prev = __builtin_inf();
+        for (int j = 0; j < k; ++j) {
+            double best = KEY_NONE;
+            for (int g = 0; g * NT * 8 < n; ++g)
+                for (int i = 0; i < 8; ++i) {
+                    const int e = (g * NT + tid) * 8 + i;
+                    if (e >= n) break;
+                    const float v = R::up(p[e]);
+                    const double ek = key_of(v, first + e);
+                    if (v > -INFINITY && ek < prev && ek > best) best = ek;
+                }
+            prev = all_max<NT>(best, &lds.list[0][0], tid);
+            if (tid == 0) lds.buf[j] = prev;
+        }
+        __syncthreads();
+        found = k;   // (there were more than that)
+    }
+    return top_of_list<NT>(lds.buf, found, lds.list, lane, wave);
 }
 
 // ---- the largest of a short row ---------------------------------------------------
@@ -285,25 +359,45 @@ __global__ __launch_bounds__(256) void top_short_kernel(TopArgs a, long long row
     if (sub == 0) a.rest[row] = top_rest(m, s, a.inv_t);
 }
 
-// One block per row, or per part of a row.
-template <int DT, int NT, int G>
-__global__ __launch_bounds__(NT) void top_kernel(TopArgs a) {
+// One block per row, or per part of a row.  The sum of the others is taken in the
+// same pass, by thread and over everything, relative to the thread's running
+// maximum; a wave takes the sums of the threads that hold listed elements again,
+// without those.  (The whole row's sum minus the listed ones' would lose what
+// the others are when the list holds nearly all of it.)
+template <int DT, int NT>
+__global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
     typedef RowType<DT> R;
     typedef typename R::T T;
-    extern __shared__ double top_buf[];   // [k * 8 G]
     __shared__ TopLds<NT> lds;
-    __shared__ float red[NT / 64];
+    __shared__ float red[NT / 64], red2[NT / 64], s_m[64], s_s[64];
     __shared__ double s_last;
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const long long row = blockIdx.x / a.parts;
     const int part = (int)(blockIdx.x - row * a.parts), first = part * a.len;
     const int n = min(a.len, a.V - first);
-    const T *x = (const T *)a.logits + row * a.ld;
-    RowRegs<DT, NT, G> regs;
-    regs.load(x + first, n, tid);
-    int found;
-    const double key =
-        top_of_regs<DT, NT, G>(regs, first, a.k, lds, top_buf, tid, found);
+    const T *x = (const T *)a.logits + row * a.ld, *p = x + first;
+    float m = -INFINITY, s = 0.f;
+    int bg = 0;
+    each_group<DT, NT>(p, n, tid, [&](const Row8<DT> &q, int g) {
+        float v[8], gm = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = q.get(j);
+            gm = fmaxf(gm, v[j]);
+        }
+        if (gm > m) {
+            if (m > -INFINITY) s *= __builtin_amdgcn_exp2f((m - gm) * a.scale);
+            m = gm;
+            bg = g;
+        }
+        const float mm = isinf(m) ? 0.f : m;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            s += __builtin_amdgcn_exp2f((v[j] - mm) * a.scale);
+    });
+    int found, slot;
+    const double key = top_of_threads<DT, NT>(p, n, first, a.k, m, bg, lds, tid,
+                                              found, slot);
     if (tid < 64) {
         if (a.parts > 1) {
             if (lane < a.k)
@@ -320,40 +414,52 @@ __global__ __launch_bounds__(NT) void top_kernel(TopArgs a) {
         if (lane == a.k - 1) s_last = key;
     }
     __syncthreads();
-    // the others: below the last one of the list (all of it, if it is not full)
+    // the holders' others: below the list's last (none if it is not full)
     const double last = s_last;
-    const float last_v = last == KEY_NONE ? -INFINITY : key_value(last);
-    const int last_i = last == KEY_NONE ? -1 : key_index(last) - first;
-    float m = -INFINITY;
-    bool nan = false;
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float v = regs.r[g].get(j);
+    const int holders = lds.holders;
+    for (int i = wave; i < holders; i += NT / 64) {
+        const int holder = lds.held[i];
+        float om = -INFINITY, os = 0.f;
+        bool nan = false;
+        for (int g0 = 0; g0 * NT * 8 < n; g0 += 8) {
+            const int e = held_at<NT>(g0, holder, lane);
+            const float v = e < n ? R::up(p[e]) : -INFINITY;
             nan |= v != v;
-            if (v < last_v || (v == last_v && regs.at(g, tid) + j > last_i))
-                m = fmaxf(m, v);
+            if (v > -INFINITY && key_of(v, first + e) < last) om = fmaxf(om, v);
         }
-    m = all_max<NT>(nan ? INFINITY : m, red, tid);
-    float s = 0.f;
-    const float mm = isinf(m) ? 0.f : m;
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float v = regs.r[g].get(j);
-            if (!(v > last_v || (v == last_v && regs.at(g, tid) + j <= last_i)))
-                s += __builtin_amdgcn_exp2f((v - mm) * a.scale);
+        om = wave_max(om);
+        const float mm = isinf(om) ? 0.f : om;
+        for (int g0 = 0; g0 * NT * 8 < n; g0 += 8) {
+            const int e = held_at<NT>(g0, holder, lane);
+            const float v = e < n ? R::up(p[e]) : -INFINITY;
+            if (v > -INFINITY && key_of(v, first + e) < last)
+                os += __builtin_amdgcn_exp2f((v - mm) * a.scale);
         }
-    s = all_sum<NT>(s, red, tid);
+        os = wave_sum(os);
+        nan = __any(nan);
+        if (lane == 0) {
+            s_m[i] = om;
+            s_s[i] = nan ? NAN : os;
+        }
+    }
+    __syncthreads();
+    if (slot >= 0) {
+        m = s_m[slot];
+        s = s_s[slot];
+    }
+    const float mx = all_max<NT>(m, red, tid);
+    const float mm = isinf(mx) ? 0.f : mx;
+    // (a thread without others has the sum 0, or NaN)
+    const float mt = isinf(m) ? 0.f : m;
+    s = all_sum<NT>(s == 0.f ? 0.f : s * __builtin_amdgcn_exp2f((mt - mm) * a.scale),
+                    red2, tid);
     if (tid == 0) {
         if (a.parts > 1) {
-            float *p = a.part + (row * a.parts + part) * 2;
-            p[0] = m;
-            p[1] = s;
+            float *q = a.part + (row * a.parts + part) * 2;
+            q[0] = mx;
+            q[1] = s;
         } else {
-            a.rest[row] = top_rest(m, s, a.inv_t);
+            a.rest[row] = top_rest(mx, s, a.inv_t);
         }
     }
 }
@@ -446,11 +552,11 @@ __device__ __forceinline__ double exp2_64(double t) {
 }
 
 // Per beam row (or part of one): the `width` largest logits -- the row's
-// normaliser does not change their order -- and its maximum and sum.
-template <int DT, int NT, int G>
-__global__ __launch_bounds__(NT) void beam_rows_kernel(BeamArgs a) {
+// normaliser does not change their order -- and its maximum and sum, in one
+// pass.
+template <int DT, int NT>
+__global__ __launch_bounds__(NT, 8) void beam_rows_kernel(BeamArgs a) {
     typedef typename RowType<DT>::T T;
-    extern __shared__ double beam_buf[];   // [width * 8 G]
     __shared__ TopLds<NT> lds;
     __shared__ float redf[NT / 64];
     __shared__ double red[NT / 64];
@@ -460,36 +566,42 @@ __global__ __launch_bounds__(NT) void beam_rows_kernel(BeamArgs a) {
     // (the join does not look at the rows of these)
     if (!(a.scores[row] > -INFINITY) || (a.finished && a.finished[row])) return;
     const int n = min(a.len, a.V - first);
-    RowRegs<DT, NT, G> regs;
-    regs.load((const T *)a.logits + row * a.ld + first, n, tid);
-    int found;
-    const double key = top_of_regs<DT, NT, G>(regs, first, a.width, lds,
-                                              beam_buf, tid, found);
-    if (tid < a.width) a.keys[(row * a.parts + part) * a.width + lane] = key;
+    const T *p = (const T *)a.logits + row * a.ld + first;
     float m = -INFINITY;
+    int bg = 0;
     bool nan = false;
-#pragma unroll
-    for (int g = 0; g < G; ++g)
+    double s = 0.;
+    each_group<DT, NT>(p, n, tid, [&](const Row8<DT> &q, int g) {
+        float v[8], gm = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float v = regs.r[g].get(j);
-            nan |= v != v;
-            m = fmaxf(m, v);
+            v[j] = q.get(j);
+            gm = fmaxf(gm, v[j]);
+            nan |= v[j] != v[j];
         }
-    m = all_max<NT>(nan ? INFINITY : m, redf, tid);
-    double s = 0.;
-    if (!isinf(m)) {
+        if (gm > m) {
+            if (m > -INFINITY) s *= exp2_64(((double)m - (double)gm) * a.scale);
+            m = gm;
+            bg = g;
+        }
+        const double mm = m == -INFINITY ? 0. : (double)m;
 #pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                s += exp2_64(((double)regs.r[g].get(j) - (double)m) * a.scale);
-        s = all_sum<NT>(s, red, tid);
-    }
+        for (int j = 0; j < 8; ++j)
+            s += exp2_64(((double)v[j] - mm) * a.scale);
+    });
+    int found, slot;
+    const double key = top_of_threads<DT, NT>(p, n, first, a.width, m, bg, lds,
+                                              tid, found, slot);
+    if (tid < a.width) a.keys[(row * a.parts + part) * a.width + lane] = key;
+    const float mx = all_max<NT>(nan ? INFINITY : m, redf, tid);
+    if (!isinf(mx))
+        s = all_sum<NT>(m == -INFINITY
+                            ? 0. : s * exp2_64(((double)m - (double)mx) * a.scale),
+                        red, tid);
     if (tid == 0) {
-        double *p = a.part + (row * a.parts + part) * 2;
-        p[0] = m;   // +inf: a NaN or +inf in this part, no distribution
-        p[1] = s;
+        double *q = a.part + (row * a.parts + part) * 2;
+        q[0] = mx;   // +inf: a NaN or +inf in this part, no distribution
+        q[1] = isinf(mx) ? 0. : s;
     }
 }
 
@@ -690,15 +802,15 @@ __global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
 }
 
 // How a row of V logits is dealt out: `parts` blocks of `len` elements each.
-// A block holds its elements in registers (65536 at most).  Few rows leave most
-// of the 256 CUs idle, so long ones are split until there are about 512 blocks
-// or a part is down to 4096 elements; the join costs one more launch.
+// Few rows leave most of the 256 CUs idle, so long ones are split until there
+// are about 512 blocks or a part is down to 4096 elements; the join costs one more
+// launch.
 struct RowPlan {
     int parts, len;
 };
 RowPlan row_plan(long long rows, int V) {
     RowPlan p;
-    long long parts = (V + 65535) / 65536;
+    long long parts = 1;
     if (rows < 256) {
         long long want = 512 / rows, most = V / 4096;
         if (want > most) want = most;
@@ -710,18 +822,12 @@ RowPlan row_plan(long long rows, int V) {
     p.parts = (V + p.len - 1) / p.len;
     return p;
 }
-// run `call` with the constants NT (threads) and G (groups of eight per thread)
-// for a stretch of `len` elements
-#define PCM_BY_LENGTH(len, ...)                                          \
-    do {                                                                 \
-        if ((len) <= 512) { constexpr int NT = 64, G = 1; __VA_ARGS__; }        \
-        else if ((len) <= 1024) { constexpr int NT = 64, G = 2; __VA_ARGS__; }  \
-        else if ((len) <= 2048) { constexpr int NT = 256, G = 1; __VA_ARGS__; } \
-        else if ((len) <= 4096) { constexpr int NT = 256, G = 2; __VA_ARGS__; } \
-        else if ((len) <= 8192) { constexpr int NT = 256, G = 4; __VA_ARGS__; } \
-        else if ((len) <= 16384) { constexpr int NT = 512, G = 4; __VA_ARGS__; } \
-        else if ((len) <= 32768) { constexpr int NT = 1024, G = 4; __VA_ARGS__; } \
-        else { constexpr int NT = 1024, G = 8; __VA_ARGS__; }                   \
+// run the call with the constant NT (threads) for a stretch of `len` elements
+#define PCM_BY_LENGTH(len, ...)                              \
+    do {                                                     \
+        if ((len) <= 1024) { constexpr int NT = 64; __VA_ARGS__; }        \
+        else if ((len) <= 16384) { constexpr int NT = 256; __VA_ARGS__; } \
+        else { constexpr int NT = 512; __VA_ARGS__; }        \
     } while (0)
 
 // ---- states follow their beams ------------------------------------------------------
@@ -912,9 +1018,9 @@ int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
         return pcm_check_launch("top_logits");
     }
     PCM_BY_DTYPE(dtype, PCM_BY_LENGTH(plan.len, {
-        hipLaunchKernelGGL((top_kernel<DT, NT, G>),
-                           dim3((unsigned)(rows * plan.parts)), dim3(NT),
-                           (size_t)k * 8 * G * sizeof(double), st, a);
+        hipLaunchKernelGGL((top_kernel<DT, NT>),
+                           dim3((unsigned)(rows * plan.parts)), dim3(NT), 0, st,
+                           a);
     }));
     if (plan.parts > 1)
         PCM_BY_DTYPE(dtype, {
@@ -998,9 +1104,9 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
         return pcm_check_launch("beam_select");
     }
     PCM_BY_DTYPE(dtype, PCM_BY_LENGTH(plan.len, {
-        hipLaunchKernelGGL((beam_rows_kernel<DT, NT, G>),
-                           dim3((unsigned)(rows * plan.parts)), dim3(NT),
-                           (size_t)width * 8 * G * sizeof(double), st, a);
+        hipLaunchKernelGGL((beam_rows_kernel<DT, NT>),
+                           dim3((unsigned)(rows * plan.parts)), dim3(NT), 0, st,
+                           a);
     }));
     hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)batch), dim3(64 * beams),
                        0, st, a);
