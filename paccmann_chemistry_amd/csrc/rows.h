@@ -123,6 +123,27 @@ static __device__ __forceinline__ T wave_sum(T v) {
     return v + lane_xor<32>(v);
 }
 
+// reductions over the LPR lanes of a row
+template <int LPR, typename T>
+static __device__ __forceinline__ T row_max(T v) {
+    v = pcm_max(v, lane_xor<1>(v));
+    v = pcm_max(v, lane_xor<2>(v));
+    if constexpr (LPR == 16) {
+        v = pcm_max(v, lane_xor<4>(v));
+        v = pcm_max(v, lane_xor<8>(v));
+    }
+    return v;
+}
+template <int LPR, typename T>
+static __device__ __forceinline__ T row_sum(T v) {
+    v += lane_xor<1>(v);
+    v += lane_xor<2>(v);
+    if constexpr (LPR == 16) {
+        v += lane_xor<4>(v);
+        v += lane_xor<8>(v);
+    }
+    return v;
+}
 // block-wide maximum / sum, every thread gets it
 template <int NT, typename T>
 static __device__ __forceinline__ T all_max(T v, T *red, int tid) {
@@ -205,10 +226,16 @@ template <> struct Row8<PCM_DTYPE_F32> {
         for (int i = 0; i < 8; ++i)
             if (bits >> i & 1) set(i, -INFINITY);
     }
-    // what is derived from the elements is derived after this: a pass over a row
-    // that touches each group before it uses it neither keeps values widened by an
-    // earlier pass in registers nor widens all groups at once
-    __device__ __forceinline__ void touch() { asm volatile("" : "+v"(a), "+v"(b)); }
+    // What is derived from the elements is derived after this, and after what has
+    // gone into `so_far` (or to memory): a pass over a row that touches each group
+    // before it uses it neither keeps values widened by an earlier pass in
+    // registers nor widens all groups at once.
+    __device__ __forceinline__ void touch(float &so_far) {
+        asm volatile("" : "+v"(a), "+v"(b), "+v"(so_far));
+    }
+    __device__ __forceinline__ void touch() {
+        asm volatile("" : "+v"(a), "+v"(b) : : "memory");
+    }
     static __device__ __forceinline__ void store(float *p, const float *v) {
         row_u32x4 x, y;
 #pragma unroll
@@ -237,7 +264,12 @@ template <> struct Row8<PCM_DTYPE_BF16> {
         for (int i = 0; i < 8; ++i)
             if (bits >> i & 1) set(i, (__bf16)-INFINITY);
     }
-    __device__ __forceinline__ void touch() { asm volatile("" : "+v"(a)); }
+    __device__ __forceinline__ void touch(float &so_far) {
+        asm volatile("" : "+v"(a), "+v"(so_far));
+    }
+    __device__ __forceinline__ void touch() {
+        asm volatile("" : "+v"(a) : : "memory");
+    }
     static __device__ __forceinline__ void store(__bf16 *p, const float *v) {
         row_u32x4 x;
 #pragma unroll
@@ -270,7 +302,12 @@ template <> struct Row8<PCM_DTYPE_F16> {
         for (int i = 0; i < 8; ++i)
             if (bits >> i & 1) set(i, (_Float16)-INFINITY);
     }
-    __device__ __forceinline__ void touch() { asm volatile("" : "+v"(a)); }
+    __device__ __forceinline__ void touch(float &so_far) {
+        asm volatile("" : "+v"(a), "+v"(so_far));
+    }
+    __device__ __forceinline__ void touch() {
+        asm volatile("" : "+v"(a) : : "memory");
+    }
     static __device__ __forceinline__ void store(_Float16 *p, const float *v) {
         row_u32x4 x;
 #pragma unroll
@@ -327,3 +364,38 @@ template <int DT, int NT, int G> struct RowRegs {
         }
     }
 };
+
+// elements e .. e + 7 of n, -inf past the end
+template <int DT>
+static __device__ __forceinline__ void load_group(
+    Row8<DT> &q, const typename RowType<DT>::T *p, int n, int e) {
+    if (e + 8 <= n) {
+        q.load(p + e);
+    } else {
+        q.lowest();
+#pragma unroll
+        for (int j = 0; j < 7; ++j)
+            if (e + j < n) q.set(j, p[e + j]);
+    }
+}
+
+// every group of eight elements of the stretch, f(elements, group): thread tid
+// has the groups at (g * NT + tid) * 8; four loads in flight
+template <int DT, int NT, typename F>
+static __device__ __forceinline__ void each_group(const typename RowType<DT>::T *p, int n,
+                                           int tid, F f) {
+    constexpr int U = 4;
+    int g = 0;
+    for (; (g + U) * NT * 8 <= n; g += U) {
+        Row8<DT> q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u].load(p + ((g + u) * NT + tid) * 8);
+#pragma unroll
+        for (int u = 0; u < U; ++u) f(q[u], g + u);
+    }
+    for (; g * NT * 8 < n; ++g) {
+        Row8<DT> q;
+        load_group(q, p, n, (g * NT + tid) * 8);
+        f(q, g);
+    }
+}

@@ -16,7 +16,8 @@ namespace {
 //      merge them pairwise, keeping 64: the k-th largest is a bound that k
 //      elements reach, all of them in the (at most) k threads whose own key does;
 //   2. a wave reads such a thread's elements again, one per lane, and appends
-//      those at or above the bound to a list in LDS: k and a few as a rule;
+//      those at or above the bound to a list in LDS: k and a few as a rule (ONE: a
+//      thread has a single group, still in its registers, and does so itself);
 //   3. the list is sorted, 64 at a time.
 // Keys are distinct, so the order in 2 does not matter, and ties take no special
 // path.  A list that overflows (k - 1 threads full of large elements) is made
@@ -29,34 +30,6 @@ template <int NT> struct TopLds {
     int holders, count;
 };
 
-// every group of eight elements of the stretch, f(elements, group): thread tid
-// has the groups at (g * NT + tid) * 8; four loads in flight
-template <int DT, int NT, typename F>
-__device__ __forceinline__ void each_group(const typename RowType<DT>::T *p, int n,
-                                           int tid, F f) {
-    constexpr int U = 4;
-    int g = 0;
-    for (; (g + U) * NT * 8 <= n; g += U) {
-        Row8<DT> q[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) q[u].load(p + ((g + u) * NT + tid) * 8);
-#pragma unroll
-        for (int u = 0; u < U; ++u) f(q[u], g + u);
-    }
-    for (; g * NT * 8 < n; ++g) {
-        const int e = (g * NT + tid) * 8;
-        Row8<DT> q;
-        if (e + 8 <= n) {
-            q.load(p + e);
-        } else {
-            q.lowest();
-#pragma unroll
-            for (int j = 0; j < 7; ++j)
-                if (e + j < n) q.set(j, p[e + j]);
-        }
-        f(q, g);
-    }
-}
 // element of thread `holder` that `lane` looks at when a wave reads eight of its
 // groups from g0 on
 template <int NT>
@@ -79,15 +52,16 @@ __device__ __forceinline__ double merge_waves(double v, double (*list)[64],
     return v;
 }
 
-// sorted top 64 of n keys in memory (LDS or global); in wave 0 afterwards
-template <int NT>
+// sorted top 64 of n keys in memory (LDS or global; SORTED: every 64 of them are);
+// in wave 0 afterwards
+template <int NT, bool SORTED = false>
 __device__ __forceinline__ double top_of_list(const double *keys, int n,
                                               double (*list)[64], int lane,
                                               int wave) {
     double v = KEY_NONE;
     for (int c = wave * 64; c < n; c += NT) {
-        const double x =
-            key_sort(c + lane < n ? keys[c + lane] : KEY_NONE, lane);
+        double x = c + lane < n ? keys[c + lane] : KEY_NONE;
+        if (!SORTED) x = key_sort(x, lane);
         // both descending: turn one around
         const double turned = __shfl(x, 63 - lane, 64);
         v = c == wave * 64 ? x : key_merge(fmax(v, turned), lane);
@@ -117,10 +91,10 @@ __device__ __forceinline__ double bound_of(double key, int k, TopLds<NT> &lds,
 // the group where it first appeared.  Returns in wave 0: lane j holds the j-th
 // largest key (KEY_NONE past `found`).  `slot`: the thread's place among the
 // holders, -1 if it holds none of the k largest.
-template <int DT, int NT>
+template <int DT, int NT, bool ONE>
 __device__ __forceinline__ double top_of_threads(
-    const typename RowType<DT>::T *p, int n, int first, int k, float bv, int bg,
-    TopLds<NT> &lds, int tid, int &found, int &slot) {
+    const typename RowType<DT>::T *p, const Row8<DT> &q, int n, int first, int k,
+    float bv, int bg, TopLds<NT> &lds, int tid, int &found, int &slot) {
     typedef RowType<DT> R;
     const int lane = tid & 63, wave = tid >> 6;
     if (tid == 0) lds.count = lds.holders = 0;
@@ -130,11 +104,24 @@ __device__ __forceinline__ double top_of_threads(
     const double bound = bound_of<NT>(key, k, lds, lane, wave);
     slot = -1;
     if (key > KEY_NONE && key >= bound) {
-        slot = atomicAdd(&lds.holders, 1);
-        lds.held[slot] = tid;
+        if (ONE) {
+            slot = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float v = q.get(j);
+                const double ek = key_of(v, first + tid * 8 + j);
+                if (v > -INFINITY && ek >= bound) {
+                    const int at = atomicAdd(&lds.count, 1);
+                    if (at < top_room(NT)) lds.buf[at] = ek;
+                }
+            }
+        } else {
+            slot = atomicAdd(&lds.holders, 1);
+            lds.held[slot] = tid;
+        }
     }
     __syncthreads();
-    const int holders = lds.holders;
+    const int holders = lds.holders;   // (ONE: 0)
     for (int i = wave; i < holders; i += NT / 64) {
         const int holder = lds.held[i];
         for (int g0 = 0; g0 * NT * 8 < n; g0 += 8) {
@@ -225,27 +212,6 @@ template <int KT> struct ShortTop {
         }
     }
 };
-// reductions over the LPR lanes of a row
-template <int LPR, typename T>
-__device__ __forceinline__ T row_max(T v) {
-    v = pcm_max(v, lane_xor<1>(v));
-    v = pcm_max(v, lane_xor<2>(v));
-    if constexpr (LPR == 16) {
-        v = pcm_max(v, lane_xor<4>(v));
-        v = pcm_max(v, lane_xor<8>(v));
-    }
-    return v;
-}
-template <int LPR, typename T>
-__device__ __forceinline__ T row_sum(T v) {
-    v += lane_xor<1>(v);
-    v += lane_xor<2>(v);
-    if constexpr (LPR == 16) {
-        v += lane_xor<4>(v);
-        v += lane_xor<8>(v);
-    }
-    return v;
-}
 // run the call with the constants LPR (lanes per row), G (groups of eight per
 // lane) and KT (list) for rows of V <= 512 and lists of k <= 16
 #define PCM_BY_SHORT_LIST(k, ...)                                     \
@@ -272,7 +238,7 @@ struct TopArgs {
     void *values;
     int32_t *indices;
     float *rest;
-    double *keys;        // split rows: [rows][parts][k]
+    double *keys;        // split rows: [rows][parts][64]
     float *part;         // ... [rows][parts][2]: maximum and sum of the others
     long long ld;
     int V, k, parts, len;   // len: elements of one part
@@ -364,7 +330,7 @@ __global__ __launch_bounds__(256) void top_short_kernel(TopArgs a, long long row
 // maximum; a wave takes the sums of the threads that hold listed elements again,
 // without those.  (The whole row's sum minus the listed ones' would lose what
 // the others are when the list holds nearly all of it.)
-template <int DT, int NT>
+template <int DT, int NT, bool ONE>
 __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
     typedef RowType<DT> R;
     typedef typename R::T T;
@@ -378,7 +344,8 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
     const T *x = (const T *)a.logits + row * a.ld, *p = x + first;
     float m = -INFINITY, s = 0.f;
     int bg = 0;
-    each_group<DT, NT>(p, n, tid, [&](const Row8<DT> &q, int g) {
+    Row8<DT> own;
+    auto pass = [&](const Row8<DT> &q, int g) {
         float v[8], gm = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -394,14 +361,20 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             s += __builtin_amdgcn_exp2f((v[j] - mm) * a.scale);
-    });
+    };
+    if (ONE) {
+        load_group(own, p, n, tid * 8);
+        pass(own, 0);
+    } else {
+        each_group<DT, NT>(p, n, tid, pass);
+    }
     int found, slot;
-    const double key = top_of_threads<DT, NT>(p, n, first, a.k, m, bg, lds, tid,
-                                              found, slot);
+    const double key = top_of_threads<DT, NT, ONE>(p, own, n, first, a.k, m, bg,
+                                                   lds, tid, found, slot);
     if (tid < 64) {
         if (a.parts > 1) {
-            if (lane < a.k)
-                a.keys[(row * a.parts + part) * a.k + lane] = key;
+            a.keys[(row * a.parts + part) * 64 + lane] =
+                lane < a.k ? key : KEY_NONE;
         } else {
             T *values = (T *)a.values + row * a.k;
             int32_t *indices = a.indices + row * a.k;
@@ -442,10 +415,30 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
             s_s[i] = nan ? NAN : os;
         }
     }
-    __syncthreads();
-    if (slot >= 0) {
-        m = s_m[slot];
-        s = s_s[slot];
+    if (ONE) {
+        if (slot >= 0) {
+            m = -INFINITY;
+            bool take[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float v = own.get(j);
+                take[j] = v != v || (v > -INFINITY &&
+                                     key_of(v, first + tid * 8 + j) < last);
+                if (take[j]) m = fmaxf(m, v);
+            }
+            const float mm = isinf(m) ? 0.f : m;
+            s = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (take[j])
+                    s += __builtin_amdgcn_exp2f((own.get(j) - mm) * a.scale);
+        }
+    } else {
+        __syncthreads();
+        if (slot >= 0) {
+            m = s_m[slot];
+            s = s_s[slot];
+        }
     }
     const float mx = all_max<NT>(m, red, tid);
     const float mm = isinf(mx) ? 0.f : mx;
@@ -475,9 +468,9 @@ __global__ __launch_bounds__(1024) void top_join_kernel(TopArgs a) {
     __shared__ double s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const long long row = blockIdx.x;
-    const int n = a.parts * a.k;
+    const int n = a.parts * 64;
     const double *keys = a.keys + row * n;
-    const double key = top_of_list<1024>(keys, n, list, lane, wave);
+    const double key = top_of_list<1024, true>(keys, n, list, lane, wave);
     if (wave == 0) {
         T *values = (T *)a.values + row * a.k;
         int32_t *indices = a.indices + row * a.k;
@@ -554,7 +547,7 @@ __device__ __forceinline__ double exp2_64(double t) {
 // Per beam row (or part of one): the `width` largest logits -- the row's
 // normaliser does not change their order -- and its maximum and sum, in one
 // pass.
-template <int DT, int NT>
+template <int DT, int NT, bool ONE>
 __global__ __launch_bounds__(NT, 8) void beam_rows_kernel(BeamArgs a) {
     typedef typename RowType<DT>::T T;
     __shared__ TopLds<NT> lds;
@@ -571,7 +564,8 @@ __global__ __launch_bounds__(NT, 8) void beam_rows_kernel(BeamArgs a) {
     int bg = 0;
     bool nan = false;
     double s = 0.;
-    each_group<DT, NT>(p, n, tid, [&](const Row8<DT> &q, int g) {
+    Row8<DT> own;
+    auto pass = [&](const Row8<DT> &q, int g) {
         float v[8], gm = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -588,10 +582,16 @@ __global__ __launch_bounds__(NT, 8) void beam_rows_kernel(BeamArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             s += exp2_64(((double)v[j] - mm) * a.scale);
-    });
+    };
+    if (ONE) {
+        load_group(own, p, n, tid * 8);
+        pass(own, 0);
+    } else {
+        each_group<DT, NT>(p, n, tid, pass);
+    }
     int found, slot;
-    const double key = top_of_threads<DT, NT>(p, n, first, a.width, m, bg, lds,
-                                              tid, found, slot);
+    const double key = top_of_threads<DT, NT, ONE>(p, own, n, first, a.width, m,
+                                                   bg, lds, tid, found, slot);
     if (tid < a.width) a.keys[(row * a.parts + part) * a.width + lane] = key;
     const float mx = all_max<NT>(nan ? INFINITY : m, redf, tid);
     if (!isinf(mx))
@@ -822,14 +822,22 @@ RowPlan row_plan(long long rows, int V) {
     p.parts = (V + p.len - 1) / p.len;
     return p;
 }
-// run the call with the constant NT (threads) for a stretch of `len` elements
-#define PCM_BY_LENGTH(len, ...)                              \
-    do {                                                     \
-        if ((len) <= 1024) { constexpr int NT = 64; __VA_ARGS__; }        \
-        else if ((len) <= 16384) { constexpr int NT = 256; __VA_ARGS__; } \
-        else { constexpr int NT = 512; __VA_ARGS__; }        \
+// run the call with the constants NT (threads) and ONE (a group of eight per
+// thread) for a stretch of `len` elements
+#define PCM_BY_LENGTH(len, ...)                                                \
+    do {                                                                       \
+        if ((len) <= 512) {                                                    \
+            constexpr int NT = 64; constexpr bool ONE = true; __VA_ARGS__;     \
+        } else if ((len) <= 2048) {                                            \
+            constexpr int NT = 256; constexpr bool ONE = true; __VA_ARGS__;    \
+        } else if ((len) <= 4096) {                                            \
+            constexpr int NT = 512; constexpr bool ONE = true; __VA_ARGS__;    \
+        } else if ((len) <= 8192) {                                            \
+            constexpr int NT = 1024; constexpr bool ONE = true; __VA_ARGS__;   \
+        } else {                                                               \
+            constexpr int NT = 512; constexpr bool ONE = false; __VA_ARGS__;   \
+        }                                                                      \
     } while (0)
-
 // ---- states follow their beams ------------------------------------------------------
 struct ReorderState {
     char *data;
@@ -968,7 +976,7 @@ size_t pcm_top_logits_workspace_bytes(int64_t rows, int32_t vocab, int32_t k) {
     if (rows < 1 || vocab < 1 || vocab > PCM_MAX_VOCAB || k < 1) return 0;
     const RowPlan p = row_plan(rows, vocab);
     if (p.parts == 1) return 0;
-    return (size_t)rows * p.parts * (k * sizeof(double) + 2 * sizeof(float));
+    return (size_t)rows * p.parts * (64 * sizeof(double) + 2 * sizeof(float));
 }
 
 int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
@@ -1002,7 +1010,7 @@ int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
     a.logits = logits; a.values = values; a.indices = indices; a.rest = rest;
     a.keys = (double *)workspace;
     a.part = plan.parts > 1
-                 ? (float *)(a.keys + (size_t)rows * plan.parts * k) : nullptr;
+                 ? (float *)(a.keys + (size_t)rows * plan.parts * 64) : nullptr;
     a.ld = ld; a.V = vocab; a.k = k; a.parts = plan.parts; a.len = plan.len;
     a.scale = (float)(1.4426950408889634 / temperature);
     a.inv_t = (float)(1.0 / temperature);
@@ -1018,7 +1026,7 @@ int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
         return pcm_check_launch("top_logits");
     }
     PCM_BY_DTYPE(dtype, PCM_BY_LENGTH(plan.len, {
-        hipLaunchKernelGGL((top_kernel<DT, NT>),
+        hipLaunchKernelGGL((top_kernel<DT, NT, ONE>),
                            dim3((unsigned)(rows * plan.parts)), dim3(NT), 0, st,
                            a);
     }));
@@ -1104,7 +1112,7 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
         return pcm_check_launch("beam_select");
     }
     PCM_BY_DTYPE(dtype, PCM_BY_LENGTH(plan.len, {
-        hipLaunchKernelGGL((beam_rows_kernel<DT, NT>),
+        hipLaunchKernelGGL((beam_rows_kernel<DT, NT, ONE>),
                            dim3((unsigned)(rows * plan.parts)), dim3(NT), 0, st,
                            a);
     }));
