@@ -181,7 +181,8 @@ PROTOTYPES = {
     ),
     'pcm_reorder_states': (
         ctypes.c_int,
-        [_VP, _I32, _I32, ctypes.POINTER(PcmState), _I32, _VP, _VP]
+        # (pcm_state is five 64-bit words: an array of them, or of PcmState)
+        [_VP, _I32, _I32, _VP, _I32, _VP, _VP]
     ),
     'pcm_generate_joint_beam_workspace_bytes': (_SZ, [_DIMS_P, _I32, _I32]),
     'pcm_stackgru_generate_joint_beam': (

@@ -523,26 +523,39 @@ struct BeamArgs {
     double inv_t, scale;   // 1 / temperature; log2(e) / temperature
 };
 
-// 2^t for t <= 0 in 64 bits, to 3e-13 of itself: rounded to the nearest integer
-// the rest is at most 1/2, where the Taylor series of exp(f ln 2) is off by
-// (ln 2 / 2)^11 / 11! after its tenth power.  18 instructions; beams compete
-// by the difference of two log-sum-exps, for which 32 bits are too few.
+// 2^t for -1020 <= t <= 0 in 64 bits, to 7e-12 of itself: beams compete by the
+// difference of two log-sum-exps, for which 32 bits are too few.  Rounded to
+// the nearest integer n (by adding 1.5 * 2^52: n is then the low word too) the
+// rest f is at most 1/2, where the Taylor series of exp(f ln 2) is off by
+// (ln 2 / 2)^10 / 10! after its ninth power; n goes into the exponent's bits.
+// Additions and fused multiplications only.
 __device__ __forceinline__ double exp2_64(double t) {
-    t = fmax(t, -1100.);
-    const double n = rint(t), f = (t - n) * 0.6931471805599453;
-    double p = 1. / 3628800.;
-    p = fma(p, f, 1. / 362880.);
-    p = fma(p, f, 1. / 40320.);
-    p = fma(p, f, 1. / 5040.);
-    p = fma(p, f, 1. / 720.);
-    p = fma(p, f, 1. / 120.);
-    p = fma(p, f, 1. / 24.);
-    p = fma(p, f, 1. / 6.);
-    p = fma(p, f, 0.5);
+    const double big = 6755399441055744.0;
+    const double r = t + big, f = t - (r - big);
+    constexpr double L = 0.69314718055994530942;
+    double p = L * L * L * L * L * L * L * L * L / 362880.;
+    p = fma(p, f, L * L * L * L * L * L * L * L / 40320.);
+    p = fma(p, f, L * L * L * L * L * L * L / 5040.);
+    p = fma(p, f, L * L * L * L * L * L / 720.);
+    p = fma(p, f, L * L * L * L * L / 120.);
+    p = fma(p, f, L * L * L * L / 24.);
+    p = fma(p, f, L * L * L / 6.);
+    p = fma(p, f, L * L / 2.);
+    p = fma(p, f, L);
     p = fma(p, f, 1.);
-    p = fma(p, f, 1.);
-    return ldexp(p, (int)n);
+    return __hiloint2double(__double2hiint(p) + (__double2loint(r) << 20),
+                            __double2loint(p));
 }
+// exp of logits relative to a maximum m (finite): (v - m) / temperature, in powers
+// of two; what is below 2^-1000 counts as 2^-1000
+struct Exp64 {
+    double scale, shift;
+    __device__ __forceinline__ Exp64(double scale_, float m)
+        : scale(scale_), shift(-(double)m * scale_) {}
+    __device__ __forceinline__ double operator()(float v) const {
+        return exp2_64(fmax(fma((double)v, scale, shift), -1000.));
+    }
+};
 
 // Per beam row (or part of one): the `width` largest logits -- the row's
 // normaliser does not change their order -- and its maximum and sum, in one
@@ -574,14 +587,16 @@ __global__ __launch_bounds__(NT, 8) void beam_rows_kernel(BeamArgs a) {
             nan |= v[j] != v[j];
         }
         if (gm > m) {
-            if (m > -INFINITY) s *= exp2_64(((double)m - (double)gm) * a.scale);
+            if (m > -INFINITY) s *= Exp64(a.scale, gm)(m);
             m = gm;
             bg = g;
         }
-        const double mm = m == -INFINITY ? 0. : (double)m;
+        // (without any element above -inf yet, or with a +inf: not used)
+        const Exp64 e(a.scale, isinf(m) ? 0.f : m);
+        double sum = 0.;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            s += exp2_64(((double)v[j] - mm) * a.scale);
+        for (int j = 0; j < 8; ++j) sum += e(v[j]);
+        if (m > -INFINITY) s += sum;
     };
     if (ONE) {
         load_group(own, p, n, tid * 8);
@@ -595,9 +610,7 @@ __global__ __launch_bounds__(NT, 8) void beam_rows_kernel(BeamArgs a) {
     if (tid < a.width) a.keys[(row * a.parts + part) * a.width + lane] = key;
     const float mx = all_max<NT>(nan ? INFINITY : m, redf, tid);
     if (!isinf(mx))
-        s = all_sum<NT>(m == -INFINITY
-                            ? 0. : s * exp2_64(((double)m - (double)mx) * a.scale),
-                        red, tid);
+        s = all_sum<NT>(m == -INFINITY ? 0. : s * Exp64(a.scale, mx)(m), red, tid);
     if (tid == 0) {
         double *q = a.part + (row * a.parts + part) * 2;
         q[0] = mx;   // +inf: a NaN or +inf in this part, no distribution
@@ -615,8 +628,16 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
     const int k = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.x, W = a.width;
     const long long row = (long long)k * a.batch + b;
+    // everything a beam needs is asked for at once (rows that are not looked at
+    // hold whatever the workspace held)
     const double score = a.scores[row];
     const bool done = a.finished && a.finished[row];
+    const double *keys = a.keys + row * a.parts * W;
+    const double *part = a.part + row * a.parts * 2;
+    const int n = a.parts * W;
+    double key = lane < n ? keys[lane] : KEY_NONE;
+    const double pm = lane < a.parts ? part[2 * lane] : -INFINITY;
+    const double ps = lane < a.parts ? part[2 * lane + 1] : 0.;
     int tok = -1;
     double c = -INFINITY;
     if (done) {
@@ -624,28 +645,17 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
         tok = lane == 0 ? a.end : lane - 1 + (lane - 1 >= a.end ? 1 : 0);
         if (lane == 0 && score == score) c = score;
     } else {
-        double m = -INFINITY;
-        if (score > -INFINITY)
-            for (int p = lane; p < a.parts; p += 64)
-                m = fmax(m, a.part[(row * a.parts + p) * 2]);
-        m = wave_max(m);
+        const double m = score > -INFINITY ? wave_max(pm) : -INFINITY;
         tok = lane;   // a row without a distribution: the tokens in order
         if (!isinf(m)) {
-            double s = 0.;
-            for (int p = lane; p < a.parts; p += 64) {
-                const double *q = a.part + (row * a.parts + p) * 2;
-                if (q[1] != 0.) s += q[1] * exp2_64((q[0] - m) * a.scale);
-            }
-            s = wave_sum(s);
+            const double s = wave_sum(
+                ps > 0. ? ps * Exp64(a.scale, (float)m)((float)pm) : 0.);
             const double lse = m * a.inv_t + log(s);
-            const double *keys = a.keys + row * a.parts * W;
-            const int n = a.parts * W;
-            double key = KEY_NONE;
-            for (int at = 0; at < n; at += 64) {
-                double x = at + lane < n ? keys[at + lane] : KEY_NONE;
-                if (a.parts > 1) x = key_sort(x, lane);
-                const double turned = __shfl(x, 63 - lane, 64);
-                key = at == 0 ? x : key_merge(fmax(key, turned), lane);
+            if (a.parts > 1) key = key_sort(key, lane);
+            for (int at = 64; at < n; at += 64) {
+                const double x =
+                    key_sort(at + lane < n ? keys[at + lane] : KEY_NONE, lane);
+                key = key_merge(fmax(key, __shfl(x, 63 - lane, 64)), lane);
             }
             const bool real = key > KEY_NONE && lane < W;
             const int found = __popcll(__ballot(real));
@@ -672,13 +682,13 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
     }
     __syncthreads();
     if (k != 0) return;
-    const int n = a.beams * W;
+    const int all = a.beams * W;
     double cc[4];
     int f[4];   // beam * V + token, 0x7fffffff where there is no candidate
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int at = lane + 64 * i;
-        f[i] = at < n ? s_f[at] : 0x7fffffff;
+        f[i] = at < all ? s_f[at] : 0x7fffffff;
         cc[i] = f[i] != 0x7fffffff ? s_c[at] : -INFINITY;
     }
     for (int j = 0; j < W; ++j) {
@@ -749,13 +759,12 @@ __global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
             const float m = row_max<LPR>(nan ? INFINITY : key_value(top.l[0]));
             live = !isinf(m);
             if (live) {
+                const Exp64 e(a.scale, m);
                 double s = 0.;
 #pragma unroll
                 for (int g = 0; g < G; ++g)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        s += exp2_64(((double)x.r[g].get(j) - (double)m) *
-                                     a.scale);
+                    for (int j = 0; j < 8; ++j) s += e(x.r[g].get(j));
                 s = row_sum<LPR>(s);
                 lse = (double)m * a.inv_t + log(s);
             }

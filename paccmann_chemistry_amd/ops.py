@@ -4,6 +4,7 @@ torch is used for device memory, streams and the autograd graph only; every
 arithmetic operation of the path runs in libpaccmann_hip.so.
 """
 import ctypes
+import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -697,6 +698,10 @@ def stackgru_generate_joint_beam(
 
 # --------------------------------------------------------------------------
 # top logits, distillation, joint beam search
+#
+# A serving loop or a small batch is bound by what a call costs on the host, so
+# what is well-formed passes one comparison per tensor here and only the rest is
+# looked at for what is wrong with it.
 # --------------------------------------------------------------------------
 class _Here:
     """A context that is nothing: the device is current already."""
@@ -718,6 +723,11 @@ def _on(device):
     return torch.cuda.device(device)
 
 
+def _stream(device):
+    """``stream_ptr`` without the Python object around it (2 us)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _dtype_code(t, what):
     code = _lib.DTYPES.get(t.dtype)
     if code is None:
@@ -727,7 +737,7 @@ def _dtype_code(t, what):
     return code
 
 
-def _operand(t, what, device, shape, dtypes):
+def _operand(t, what, device, shape, *dtypes):
     """``t`` on ``device``, of that shape and one of those types, dense."""
     if t.device != device:
         raise ValueError(f'{what} is on {t.device}, the logits on {device}')
@@ -738,7 +748,15 @@ def _operand(t, what, device, shape, dtypes):
         raise ValueError(
             f'{what} has shape {tuple(t.shape)}, expected {tuple(shape)}'
         )
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _rows_of(x, what):
+    """(tensor kept alive, rows, row stride) of ``x[..., V]``."""
+    if x.is_contiguous():
+        vocab = x.shape[-1]
+        return x, x.numel() // vocab, vocab
+    return _rows2d(x, what)
 
 
 def _check_temperature(temperature):
@@ -786,13 +804,13 @@ def top_logits(logits, k, temperature=1.0):
             f'k={k}: expected 1..{min(vocab, _lib.TOP_MAX)} '
             f'(vocabulary {vocab})'
         )
-    logits = logits.detach()
     dev, lead = logits.device, logits.shape[:-1]
-    values = torch.empty(lead + (k, ), dtype=logits.dtype, device=dev)
-    indices = torch.empty(lead + (k, ), dtype=torch.int32, device=dev)
+    listed = lead + (k, )
+    values = torch.empty(listed, dtype=logits.dtype, device=dev)
+    indices = torch.empty(listed, dtype=torch.int32, device=dev)
     rest = torch.empty(lead, dtype=torch.float32, device=dev)
     if rest.numel():
-        x2, rows, ld = _rows2d(logits, 'top logits')
+        x2, rows, ld = _rows_of(logits.detach(), 'top logits')
         need = lib.pcm_top_logits_workspace_bytes(rows, vocab, k)
         work = None
         if need:
@@ -802,10 +820,39 @@ def top_logits(logits, k, temperature=1.0):
                 lib.pcm_top_logits(
                     x2.data_ptr(), code, rows, ld, vocab, k, temperature,
                     values.data_ptr(), indices.data_ptr(), rest.data_ptr(),
-                    ptr(work), need, stream_ptr(dev)
+                    ptr(work), need, _stream(dev)
                 ), 'pcm_top_logits'
             )
     return TopLogits(values, indices, rest, temperature)
+
+
+def _distill(logits, want, args):
+    """pcm_distill_loss on checked operands: (loss, dlogits or None)."""
+    (code, vocab, values, indices, rest, temperature, targets, lengths,
+     hard_weight, step_weight, status) = args
+    lib = load()
+    steps, batch, _ = logits.shape
+    dev = logits.device
+    x2, _, ld = _rows_of(logits, 'distill logits')
+    loss = torch.empty((), device=dev)
+    dlogits = None
+    if want:
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    scratch = torch.empty(
+        lib.pcm_distill_scratch_floats(steps, batch), device=dev
+    )
+    with _on(dev):
+        check(
+            lib.pcm_distill_loss(
+                x2.data_ptr(), code, ld, values.data_ptr(),
+                _lib.DTYPES[values.dtype], indices.data_ptr(), ptr(rest),
+                indices.shape[-1], ptr(targets), ptr(lengths),
+                ptr(step_weight), steps, batch, vocab, temperature,
+                hard_weight, loss.data_ptr(), ptr(dlogits),
+                scratch.data_ptr(), ptr(status), _stream(dev)
+            ), 'pcm_distill_loss'
+        )
+    return loss, dlogits
 
 
 class DistillLossFn(torch.autograd.Function):
@@ -813,33 +860,10 @@ class DistillLossFn(torch.autograd.Function):
     the loss and multiplied by the incoming one in ``backward``."""
 
     @staticmethod
-    def forward(ctx, logits, values, indices, rest, temperature, targets,
-                lengths, hard_weight, step_weight, status):
-        lib = load()
-        steps, batch, vocab = logits.shape
-        dev = logits.device
-        x2, _, ld = _rows2d(logits, 'distill logits')
-        want = ctx.needs_input_grad[0]
-        loss = torch.empty((), device=dev)
-        dlogits = torch.empty(
-            (steps, batch, vocab), dtype=logits.dtype, device=dev
-        ) if want else None
-        scratch = torch.empty(
-            lib.pcm_distill_scratch_floats(steps, batch), device=dev
-        )
-        with _on(dev):
-            check(
-                lib.pcm_distill_loss(
-                    x2.data_ptr(), _lib.DTYPES[logits.dtype], ld,
-                    values.data_ptr(), _lib.DTYPES[values.dtype],
-                    indices.data_ptr(), ptr(rest), indices.shape[-1],
-                    ptr(targets), ptr(lengths), ptr(step_weight), steps, batch,
-                    vocab, temperature, hard_weight, loss.data_ptr(),
-                    ptr(dlogits), scratch.data_ptr(), ptr(status),
-                    stream_ptr(dev)
-                ), 'pcm_distill_loss'
-            )
+    def forward(ctx, logits, args):
+        loss, dlogits = _distill(logits, True, args)
         ctx.dlogits = dlogits
+        ctx.scale = (dlogits.data_ptr(), args[0], dlogits.numel())
         return loss
 
     @staticmethod
@@ -851,16 +875,14 @@ class DistillLossFn(torch.autograd.Function):
                 'out by the first call (retain_graph is not supported)'
             )
         ctx.dlogits = None
-        dev = dlogits.device
-        dloss = _f32(dloss, 'dloss').reshape(1).contiguous()
-        with _on(dev):
-            check(
-                load().pcm_scale(
-                    dlogits.data_ptr(), _lib.DTYPES[dlogits.dtype],
-                    dlogits.numel(), dloss.data_ptr(), stream_ptr(dev)
-                ), 'pcm_scale'
-            )
-        return (dlogits, ) + (None, ) * 9
+        # (an fp32 scalar; autograd's thread has the device and the stream of
+        # the forward)
+        check(
+            load().pcm_scale(
+                *ctx.scale, dloss.data_ptr(), _stream(dloss.device)
+            ), 'pcm_scale'
+        )
+        return dlogits, None
 
 
 def distill_loss(logits, teacher, targets=None, lengths=None, hard_weight=0.0,
@@ -877,14 +899,14 @@ def distill_loss(logits, teacher, targets=None, lengths=None, hard_weight=0.0,
     ``DecoderHeadFn`` reduces its cross entropy.  Returns an fp32 scalar that
     carries the gradient of the logits.  Indices outside the vocabulary raise
     STATUS_BAD_TOKEN in ``status`` (see ``check_status``)."""
-    load()
     require_device(logits, 'distill logits')
-    _dtype_code(logits, 'distill logits')
-    if logits.dim() != 3 or 0 in logits.shape:
+    code = _dtype_code(logits, 'distill logits')
+    size = logits.shape
+    if len(size) != 3 or 0 in size:
         raise ValueError(
-            f'logits have shape {tuple(logits.shape)}, expected [T, B, V]'
+            f'logits have shape {tuple(size)}, expected [T, B, V]'
         )
-    steps, batch, vocab = logits.shape
+    steps, batch, vocab = size
     _check_vocab(vocab)
     values, indices, rest, temperature = teacher
     temperature = _check_temperature(temperature)
@@ -894,34 +916,33 @@ def distill_loss(logits, teacher, targets=None, lengths=None, hard_weight=0.0,
             f'teacher indices have shape {tuple(indices.shape)}, expected '
             f'[T, B, k] with k in 1..{_lib.TOP_MAX}'
         )
-    shape = logits.shape[:2]
+    shape = size[:2]
     listed = shape + indices.shape[-1:]
-    values = _operand(values.detach(), 'teacher values', dev, listed,
-                      tuple(_lib.DTYPES))
-    indices = _operand(indices, 'teacher indices', dev, listed, (torch.int32, ))
+    values = _operand(values, 'teacher values', dev, listed, *_lib.DTYPES)
+    indices = _operand(indices, 'teacher indices', dev, listed, torch.int32)
     if rest is not None:
-        rest = _operand(rest.detach(), 'teacher rest', dev, shape,
-                        (torch.float32, ))
+        rest = _operand(rest, 'teacher rest', dev, shape, torch.float32)
     hard_weight = float(hard_weight)
     if not 0.0 <= hard_weight <= 1.0:
         raise ValueError(f'hard_weight {hard_weight}: expected 0..1')
     if targets is not None:
-        targets = _operand(targets, 'targets', dev, shape, (torch.int64, ))
+        targets = _operand(targets, 'targets', dev, shape, torch.int64)
     elif hard_weight > 0:
         raise ValueError('hard_weight needs targets')
     if lengths is not None:
         if lengths.dtype != torch.int32 or lengths.device != dev:
             lengths = lengths.to(device=dev, dtype=torch.int32)
-        lengths = _operand(lengths, 'lengths', dev, (batch, ), (torch.int32, ))
+        lengths = _operand(lengths, 'lengths', dev, (batch, ), torch.int32)
     if step_weight is not None:
         step_weight = _operand(
             step_weight.to(device=dev, dtype=torch.float32), 'step_weight',
-            dev, (steps, ), (torch.float32, )
+            dev, (steps, ), torch.float32
         )
-    return DistillLossFn.apply(
-        logits, values, indices, rest, temperature, targets, lengths,
-        hard_weight, step_weight, status
-    )
+    args = (code, vocab, values, indices, rest, temperature, targets, lengths,
+            hard_weight, step_weight, status)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return DistillLossFn.apply(logits, args)
+    return _distill(logits, False, args)[0]
 
 
 class BeamStep(NamedTuple):
@@ -963,14 +984,13 @@ def beam_select(logits, scores, width=None, temperature=1.0, finished=None,
             f'the width within the {beams * vocab} candidates'
         )
     dev = logits.device
-    scores = _operand(scores, 'scores', dev, (beams, batch),
-                      (torch.float64, ))
+    scores = _operand(scores, 'scores', dev, (beams, batch), torch.float64)
     if (finished is None) != (end_token is None):
         raise ValueError('finished and end_token go together')
     finished_out = None
     if finished is not None:
         finished = _operand(finished, 'finished', dev, (beams, batch),
-                            (torch.bool, ))
+                            torch.bool)
         end_token = int(end_token)
         if not 0 <= end_token < vocab:
             raise ValueError(
@@ -978,7 +998,7 @@ def beam_select(logits, scores, width=None, temperature=1.0, finished=None,
             )
         finished_out = torch.empty((width, batch), dtype=torch.bool,
                                    device=dev)
-    x2, _, ld = _rows2d(logits.detach(), 'beam logits')
+    x2, _, ld = _rows_of(logits.detach(), 'beam logits')
     tokens = torch.empty((width, batch), dtype=torch.int64, device=dev)
     parents = torch.empty((width, batch), dtype=torch.int32, device=dev)
     scores_out = torch.empty((width, batch), dtype=torch.float64, device=dev)
@@ -991,23 +1011,29 @@ def beam_select(logits, scores, width=None, temperature=1.0, finished=None,
                 beams, batch, vocab, width, temperature,
                 -1 if end_token is None else end_token, tokens.data_ptr(),
                 parents.data_ptr(), scores_out.data_ptr(), ptr(finished_out),
-                ptr(work), need, stream_ptr(dev)
+                ptr(work), need, _stream(dev)
             ), 'pcm_beam_select'
         )
     return BeamStep(tokens, parents, scores_out, finished_out)
 
 
 def _state_view(t, row_dim, rows, what):
-    """PcmState of a tensor whose dimension ``row_dim`` is the beams' rows."""
+    """The fields of the pcm_state of a tensor whose dimension ``row_dim`` is
+    the beams' rows."""
     dim = t.dim()
     if not -dim <= row_dim < dim:
         raise ValueError(f'{what}: row dimension {row_dim} of {dim}')
     row_dim %= dim
-    shape, stride, size = t.shape, t.stride(), t.element_size()
+    shape, size = t.shape, t.element_size()
     if shape[row_dim] != rows:
         raise ValueError(
             f'{what} has {shape[row_dim]} rows, expected {rows}'
         )
+    if t.is_contiguous():
+        piece = size * math.prod(shape[row_dim + 1:])
+        return (t.data_ptr(), math.prod(shape[:row_dim]), rows * piece, piece,
+                piece)
+    stride = t.stride()
     inner = 1   # elements of a row's piece, in one stretch
     for d in range(dim - 1, row_dim, -1):
         if shape[d] != 1 and stride[d] != inner:
@@ -1026,8 +1052,8 @@ def _state_view(t, row_dim, rows, what):
         if outer == 1:
             outer_stride = stride[d]
         outer *= shape[d]
-    return _lib.PcmState(t.data_ptr(), outer, outer_stride * size,
-                         stride[row_dim] * size, inner * size)
+    return (t.data_ptr(), outer, outer_stride * size, stride[row_dim] * size,
+            inner * size)
 
 
 def reorder_states(parents, states, row_dims=0, status=None):
@@ -1055,21 +1081,25 @@ def reorder_states(parents, states, row_dims=0, status=None):
     if len(row_dims) != len(states):
         raise ValueError('row_dims: one for each state')
     dev = parents.device
-    table = (_lib.PcmState * len(states))()
-    for i, (state, row_dim) in enumerate(zip(states, row_dims)):
+    table = []
+    for state, row_dim in zip(states, row_dims):
         if state.device != dev:
             raise ValueError(
-                f'state {i} is on {state.device}, the parents on {dev}'
+                f'state {len(table) // 5} is on {state.device}, the parents '
+                f'on {dev}'
             )
         if state.requires_grad:
-            raise ValueError(f'state {i} requires a gradient')
-        table[i] = _state_view(state, row_dim, beams * batch, f'state {i}')
-    parents = parents.contiguous()
+            raise ValueError(f'state {len(table) // 5} requires a gradient')
+        table += _state_view(state, row_dim, beams * batch,
+                             f'state {len(table) // 5}')
+    if not parents.is_contiguous():
+        parents = parents.contiguous()
     with _on(dev):
         check(
             lib.pcm_reorder_states(
-                parents.data_ptr(), beams, batch, table, len(states),
-                ptr(status), stream_ptr(dev)
+                parents.data_ptr(), beams, batch,
+                (ctypes.c_int64 * len(table))(*table), len(states),
+                ptr(status), _stream(dev)
             ), 'pcm_reorder_states'
         )
 

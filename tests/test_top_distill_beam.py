@@ -264,7 +264,8 @@ def test_beam_refusals():
     _refused(lib, call(end=20), 'end_token')
     _refused(lib, call(end=-1), 'end_token')
     _refused(lib, call(done=None), 'finished_out')
-    _refused(lib, call(nbytes=0), 'workspace')
+    _refused(lib, call(vocab=1000, ld=1000, nbytes=0), 'workspace')
+    _refused(lib, call(vocab=1000, ld=1000, work=None), 'workspace')
     assert lib.pcm_beam_select_workspace_bytes(0, 1, 5, 1) == 0
 
 
@@ -470,6 +471,7 @@ def _distill_case(T, B, V, k, dtype, kind, rest, g, absent=True):
 
 def _check_distill(got_loss, got, ref_loss, ref, logits, weights, tau, hard,
                    vocab, dtype):
+    got_loss = got_loss.detach()
     live = torch.where(torch.isfinite(logits.double()), logits.double(), 0.0)
     size = 4 + 2 * live.abs().amax(-1) / tau + 2 * math.log(vocab + 1) + 30
     chain = EPS * (vocab / 64 + 64)
