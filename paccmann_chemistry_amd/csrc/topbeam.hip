@@ -30,6 +30,14 @@ template <int NT> struct TopLds {
     int holders, count;
 };
 
+// What a wave has read of its holders again: those number wave, wave + NT / 64,
+// ... of at most 64, sixteen groups each (two per lane), all loads in flight at
+// once.  Stretches that are longer are read where they are needed.
+template <int NT> struct Held {
+    static constexpr int N = NT >= 4096 ? 1 : 4096 / NT;   // 64 / (NT / 64)
+    float v[N][2];
+    static __device__ __forceinline__ bool fits(int n) { return n <= NT * 128; }
+};
 // element of thread `holder` that `lane` looks at when a wave reads eight of its
 // groups from g0 on
 template <int NT>
@@ -94,7 +102,8 @@ __device__ __forceinline__ double bound_of(double key, int k, TopLds<NT> &lds,
 template <int DT, int NT, bool ONE>
 __device__ __forceinline__ double top_of_threads(
     const typename RowType<DT>::T *p, const Row8<DT> &q, int n, int first, int k,
-    float bv, int bg, TopLds<NT> &lds, int tid, int &found, int &slot) {
+    float bv, int bg, TopLds<NT> &lds, Held<NT> &held, int tid, int &found,
+    int &slot) {
     typedef RowType<DT> R;
     const int lane = tid & 63, wave = tid >> 6;
     if (tid == 0) lds.count = lds.holders = 0;
@@ -122,17 +131,45 @@ __device__ __forceinline__ double top_of_threads(
     }
     __syncthreads();
     const int holders = lds.holders;   // (ONE: 0)
-    for (int i = wave; i < holders; i += NT / 64) {
-        const int holder = lds.held[i];
-        for (int g0 = 0; g0 * NT * 8 < n; g0 += 8) {
-            const int e = held_at<NT>(g0, holder, lane);
-            const float v = e < n ? R::up(p[e]) : -INFINITY;
-            if (v > -INFINITY) {
-                const double ek = key_of(v, first + e);
-                if (ek >= bound) {
-                    const int at = atomicAdd(&lds.count, 1);
-                    if (at < top_room(NT)) lds.buf[at] = ek;
+    auto append = [&](float v, int e) {
+        if (v > -INFINITY) {
+            const double ek = key_of(v, first + e);
+            if (ek >= bound) {
+                const int at = atomicAdd(&lds.count, 1);
+                if (at < top_room(NT)) lds.buf[at] = ek;
+            }
+        }
+    };
+    if (ONE) {
+    } else if (Held<NT>::fits(n)) {
+#pragma unroll
+        for (int i = 0; i < Held<NT>::N; ++i) {
+            const int h = wave + i * (NT / 64);
+            if (h < holders) {
+                const int holder = lds.held[h];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int e = held_at<NT>(t * 8, holder, lane);
+                    held.v[i][t] = e < n ? R::up(p[e]) : -INFINITY;
                 }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < Held<NT>::N; ++i) {
+            const int h = wave + i * (NT / 64);
+            if (h < holders) {
+                const int holder = lds.held[h];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    append(held.v[i][t], held_at<NT>(t * 8, holder, lane));
+            }
+        }
+    } else {
+        for (int i = wave; i < holders; i += NT / 64) {
+            const int holder = lds.held[i];
+            for (int g0 = 0; g0 * NT * 8 < n; g0 += 8) {
+                const int e = held_at<NT>(g0, holder, lane);
+                append(e < n ? R::up(p[e]) : -INFINITY, e);
             }
         }
     }
@@ -369,8 +406,9 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
         each_group<DT, NT>(p, n, tid, pass);
     }
     int found, slot;
-    const double key = top_of_threads<DT, NT, ONE>(p, own, n, first, a.k, m, bg,
-                                                   lds, tid, found, slot);
+    Held<NT> held;
+    const double key = top_of_threads<DT, NT, ONE>(
+        p, own, n, first, a.k, m, bg, lds, held, tid, found, slot);
     if (tid < 64) {
         if (a.parts > 1) {
             a.keys[(row * a.parts + part) * 64 + lane] =
@@ -389,30 +427,63 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
     __syncthreads();
     // the holders' others: below the list's last (none if it is not full)
     const double last = s_last;
-    const int holders = lds.holders;
-    for (int i = wave; i < holders; i += NT / 64) {
-        const int holder = lds.held[i];
-        float om = -INFINITY, os = 0.f;
-        bool nan = false;
-        for (int g0 = 0; g0 * NT * 8 < n; g0 += 8) {
-            const int e = held_at<NT>(g0, holder, lane);
-            const float v = e < n ? R::up(p[e]) : -INFINITY;
-            nan |= v != v;
-            if (v > -INFINITY && key_of(v, first + e) < last) om = fmaxf(om, v);
+    const int holders = lds.holders;   // (ONE: 0)
+    auto is_other = [&](float v, int e) {
+        return v > -INFINITY && key_of(v, first + e) < last;
+    };
+    if (ONE) {
+    } else if (Held<NT>::fits(n)) {
+#pragma unroll
+        for (int i = 0; i < Held<NT>::N; ++i) {
+            const int h = wave + i * (NT / 64);
+            if (h < holders) {
+                const int holder = lds.held[h];
+                float ov[2];
+                bool nan = false;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const float v = held.v[i][t];
+                    nan |= v != v;
+                    ov[t] = is_other(v, held_at<NT>(t * 8, holder, lane))
+                                ? v : -INFINITY;
+                }
+                const float om = wave_max(fmaxf(ov[0], ov[1]));
+                const float mm = isinf(om) ? 0.f : om;
+                const float os = wave_sum(
+                    __builtin_amdgcn_exp2f((ov[0] - mm) * a.scale) +
+                    __builtin_amdgcn_exp2f((ov[1] - mm) * a.scale));
+                nan = __any(nan);
+                if (lane == 0) {
+                    s_m[h] = om;
+                    s_s[h] = nan ? NAN : os;
+                }
+            }
         }
-        om = wave_max(om);
-        const float mm = isinf(om) ? 0.f : om;
-        for (int g0 = 0; g0 * NT * 8 < n; g0 += 8) {
-            const int e = held_at<NT>(g0, holder, lane);
-            const float v = e < n ? R::up(p[e]) : -INFINITY;
-            if (v > -INFINITY && key_of(v, first + e) < last)
-                os += __builtin_amdgcn_exp2f((v - mm) * a.scale);
-        }
-        os = wave_sum(os);
-        nan = __any(nan);
-        if (lane == 0) {
-            s_m[i] = om;
-            s_s[i] = nan ? NAN : os;
+    } else {
+        for (int i = wave; i < holders; i += NT / 64) {
+            const int holder = lds.held[i];
+            float om = -INFINITY, os = 0.f;
+            bool nan = false;
+            for (int g0 = 0; g0 * NT * 8 < n; g0 += 8) {
+                const int e = held_at<NT>(g0, holder, lane);
+                const float v = e < n ? R::up(p[e]) : -INFINITY;
+                nan |= v != v;
+                if (is_other(v, e)) om = fmaxf(om, v);
+            }
+            om = wave_max(om);
+            const float mm = isinf(om) ? 0.f : om;
+            for (int g0 = 0; g0 * NT * 8 < n; g0 += 8) {
+                const int e = held_at<NT>(g0, holder, lane);
+                const float v = e < n ? R::up(p[e]) : -INFINITY;
+                if (is_other(v, e))
+                    os += __builtin_amdgcn_exp2f((v - mm) * a.scale);
+            }
+            os = wave_sum(os);
+            nan = __any(nan);
+            if (lane == 0) {
+                s_m[i] = om;
+                s_s[i] = nan ? NAN : os;
+            }
         }
     }
     if (ONE) {
@@ -605,8 +676,9 @@ __global__ __launch_bounds__(NT, 8) void beam_rows_kernel(BeamArgs a) {
         each_group<DT, NT>(p, n, tid, pass);
     }
     int found, slot;
-    const double key = top_of_threads<DT, NT, ONE>(p, own, n, first, a.width, m,
-                                                   bg, lds, tid, found, slot);
+    Held<NT> held;
+    const double key = top_of_threads<DT, NT, ONE>(
+        p, own, n, first, a.width, m, bg, lds, held, tid, found, slot);
     if (tid < a.width) a.keys[(row * a.parts + part) * a.width + lane] = key;
     const float mx = all_max<NT>(nan ? INFINITY : m, redf, tid);
     if (!isinf(mx))
