@@ -12,31 +12,37 @@ namespace {
 // fills up.
 //   1. in the pass every thread keeps its maximum and the group of eight where
 //      it first appeared: the key (maximum, last index of that group) is not above
-//      the thread's largest one.  The waves sort theirs (64, in registers) and
-//      merge them pairwise, keeping 64: the k-th largest is a bound that k
-//      elements reach, all of them in the (at most) k threads whose own key does;
-//   2. a wave reads such a thread's elements again, one per lane, and appends
-//      those at or above the bound to a list in LDS: k and a few as a rule (ONE: a
-//      thread has a single group, still in its registers, and does so itself);
+//      the thread's largest one.  The threads form 64 (k > 32: 128) teams, one
+//      lane of every (other) wave each; the k-th largest of the teams' largest
+//      keys is a bound that k elements reach at least, and not many more: with
+//      random data an element in 64 ln 2 / k teams' shares does, 44 for k = 32.
+//      It costs one sort of 64 keys (two), in registers;
+//   2. the threads whose own key reaches it hold all of those elements (groups
+//      are disjoint stretches).  A wave reads such a thread's elements again, one
+//      per lane, and appends those at or above the bound to a list in LDS (ONE:
+//      a thread has a single group, still in its registers, and does so itself);
 //   3. the list is sorted, 64 at a time.
 // Keys are distinct, so the order in 2 does not matter, and ties take no special
-// path.  A list that overflows (k - 1 threads full of large elements) is made
-// by k passes instead.
+// path.  A list that overflows (few teams hold most of the large elements) is
+// made by k passes instead.
 constexpr int top_room(int nt) { return nt == 64 ? 256 : 1024; }
 template <int NT> struct TopLds {
     double list[NT / 64][64];
     double buf[top_room(NT)];
-    int held[64];    // threads that reach the bound
+    double bound;
+    int held[NT];    // threads that reach the bound
     int holders, count;
 };
 
 // What a wave has read of its holders again: those number wave, wave + NT / 64,
 // ... of at most 64, sixteen groups each (two per lane), all loads in flight at
-// once.  Stretches that are longer are read where they are needed.
+// once.  More holders or longer stretches are read where they are needed.
 template <int NT> struct Held {
-    static constexpr int N = NT >= 4096 ? 1 : 4096 / NT;   // 64 / (NT / 64)
+    static constexpr int N = 4096 / NT;   // 64 / (NT / 64)
     float v[N][2];
-    static __device__ __forceinline__ bool fits(int n) { return n <= NT * 128; }
+    static __device__ __forceinline__ bool fits(int n, int holders) {
+        return n <= NT * 128 && holders <= 64;
+    }
 };
 // element of thread `holder` that `lane` looks at when a wave reads eight of its
 // groups from g0 on
@@ -78,21 +84,39 @@ __device__ __forceinline__ double top_of_list(const double *keys, int n,
     return v;
 }
 
-// the k-th largest of one key per thread, known to all
+// the k-th largest of the teams' largest keys, known to all
 template <int NT>
 __device__ __forceinline__ double bound_of(double key, int k, TopLds<NT> &lds,
                                            int lane, int wave) {
-    key = key_sort(key, lane);
-    key = merge_waves<NT>(key, lds.list, lane, wave);
-    if constexpr (NT > 64) {
-        if (wave == 0 && lane == k - 1) lds.list[0][0] = key;
-        __syncthreads();
-        key = lds.list[0][0];
+    if constexpr (NT == 64) {
+        key = key_lane(key_sort(key, lane), k - 1);
+        __syncthreads();   // (lds.count)
+        return key;
     } else {
-        key = key_lane(key, k - 1);
+        lds.list[wave][lane] = key;
+        __syncthreads();
+        const bool two = k > 32;
+        if (wave < (two ? 2 : 1)) {
+            // 64 teams: lane l of all waves; 128: of the even, of the odd waves
+            key = lds.list[wave][lane];
+#pragma unroll
+            for (int w = 1; w < NT / 64; ++w)
+                if (!two || (w & 1) == wave)
+                    key = fmax(key, lds.list[w][lane]);
+            if (two && wave == 1) key = fmax(key, lds.list[1][lane]);
+            key = key_sort(key, lane);
+        }
+        if (two) {
+            __syncthreads();
+            if (wave == 1) lds.list[1][lane] = key;
+            __syncthreads();
+            if (wave == 0)
+                key = key_merge(fmax(key, lds.list[1][63 - lane]), lane);
+        }
+        if (wave == 0 && lane == k - 1) lds.bound = key;
+        __syncthreads();   // (and lds.count; the lists are free again)
+        return lds.bound;
     }
-    __syncthreads();   // (lds.count, and the lists are free again)
-    return key;
 }
 
 // Steps 1 (from the threads' maxima on) to 3.  bv, bg: the thread's maximum and
@@ -111,6 +135,7 @@ __device__ __forceinline__ double top_of_threads(
                            ? key_of(bv, first + (bg * NT + tid) * 8 + 7)
                            : KEY_NONE;
     const double bound = bound_of<NT>(key, k, lds, lane, wave);
+    const float bound_v = bound == KEY_NONE ? -INFINITY : key_value(bound);
     slot = -1;
     if (key > KEY_NONE && key >= bound) {
         if (ONE) {
@@ -118,10 +143,12 @@ __device__ __forceinline__ double top_of_threads(
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float v = q.get(j);
-                const double ek = key_of(v, first + tid * 8 + j);
-                if (v > -INFINITY && ek >= bound) {
-                    const int at = atomicAdd(&lds.count, 1);
-                    if (at < top_room(NT)) lds.buf[at] = ek;
+                if (v >= bound_v && v > -INFINITY) {
+                    const double ek = key_of(v, first + tid * 8 + j);
+                    if (ek >= bound) {
+                        const int at = atomicAdd(&lds.count, 1);
+                        if (at < top_room(NT)) lds.buf[at] = ek;
+                    }
                 }
             }
         } else {
@@ -132,7 +159,7 @@ __device__ __forceinline__ double top_of_threads(
     __syncthreads();
     const int holders = lds.holders;   // (ONE: 0)
     auto append = [&](float v, int e) {
-        if (v > -INFINITY) {
+        if (v >= bound_v && v > -INFINITY) {
             const double ek = key_of(v, first + e);
             if (ek >= bound) {
                 const int at = atomicAdd(&lds.count, 1);
@@ -141,7 +168,7 @@ __device__ __forceinline__ double top_of_threads(
         }
     };
     if (ONE) {
-    } else if (Held<NT>::fits(n)) {
+    } else if (Held<NT>::fits(n, holders)) {
 #pragma unroll
         for (int i = 0; i < Held<NT>::N; ++i) {
             const int h = wave + i * (NT / 64);
@@ -372,13 +399,19 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
     typedef RowType<DT> R;
     typedef typename R::T T;
     __shared__ TopLds<NT> lds;
-    __shared__ float red[NT / 64], red2[NT / 64], s_m[64], s_s[64];
+    __shared__ float red[NT / 64], red2[NT / 64];
+    __shared__ float s_m[ONE ? 1 : NT], s_s[ONE ? 1 : NT];   // by holder
     __shared__ double s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const long long row = blockIdx.x / a.parts;
     const int part = (int)(blockIdx.x - row * a.parts), first = part * a.len;
     const int n = min(a.len, a.V - first);
     const T *x = (const T *)a.logits + row * a.ld, *p = x + first;
+    auto exp_from = [&](float v, float shift) {
+        return __builtin_amdgcn_exp2f((v - shift) * a.scale);
+    };
+    // (v - m first: a mask of the type's lowest value times scale need not be
+    // finite, nor its rounding small)
     float m = -INFINITY, s = 0.f;
     int bg = 0;
     Row8<DT> own;
@@ -390,14 +423,13 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
             gm = fmaxf(gm, v[j]);
         }
         if (gm > m) {
-            if (m > -INFINITY) s *= __builtin_amdgcn_exp2f((m - gm) * a.scale);
+            if (m > -INFINITY) s *= exp_from(m, gm);
             m = gm;
             bg = g;
         }
         const float mm = isinf(m) ? 0.f : m;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            s += __builtin_amdgcn_exp2f((v[j] - mm) * a.scale);
+        for (int j = 0; j < 8; ++j) s += exp_from(v[j], mm);
     };
     if (ONE) {
         load_group(own, p, n, tid * 8);
@@ -427,12 +459,14 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
     __syncthreads();
     // the holders' others: below the list's last (none if it is not full)
     const double last = s_last;
+    const float last_v = last == KEY_NONE ? -INFINITY : key_value(last);
+    const int last_i = last == KEY_NONE ? 0x7fffffff : key_index(last) - first;
     const int holders = lds.holders;   // (ONE: 0)
     auto is_other = [&](float v, int e) {
-        return v > -INFINITY && key_of(v, first + e) < last;
+        return v < last_v || (v == last_v && e > last_i);
     };
     if (ONE) {
-    } else if (Held<NT>::fits(n)) {
+    } else if (Held<NT>::fits(n, holders)) {
 #pragma unroll
         for (int i = 0; i < Held<NT>::N; ++i) {
             const int h = wave + i * (NT / 64);
@@ -449,9 +483,8 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
                 }
                 const float om = wave_max(fmaxf(ov[0], ov[1]));
                 const float mm = isinf(om) ? 0.f : om;
-                const float os = wave_sum(
-                    __builtin_amdgcn_exp2f((ov[0] - mm) * a.scale) +
-                    __builtin_amdgcn_exp2f((ov[1] - mm) * a.scale));
+                const float os =
+                    wave_sum(exp_from(ov[0], mm) + exp_from(ov[1], mm));
                 nan = __any(nan);
                 if (lane == 0) {
                     s_m[h] = om;
@@ -475,8 +508,7 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
             for (int g0 = 0; g0 * NT * 8 < n; g0 += 8) {
                 const int e = held_at<NT>(g0, holder, lane);
                 const float v = e < n ? R::up(p[e]) : -INFINITY;
-                if (is_other(v, e))
-                    os += __builtin_amdgcn_exp2f((v - mm) * a.scale);
+                if (is_other(v, e)) os += exp_from(v, mm);
             }
             os = wave_sum(os);
             nan = __any(nan);
@@ -493,16 +525,14 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float v = own.get(j);
-                take[j] = v != v || (v > -INFINITY &&
-                                     key_of(v, first + tid * 8 + j) < last);
+                take[j] = v != v || is_other(v, tid * 8 + j);
                 if (take[j]) m = fmaxf(m, v);
             }
             const float mm = isinf(m) ? 0.f : m;
             s = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (take[j])
-                    s += __builtin_amdgcn_exp2f((own.get(j) - mm) * a.scale);
+                if (take[j]) s += exp_from(own.get(j), mm);
         }
     } else {
         __syncthreads();
@@ -512,10 +542,10 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
         }
     }
     const float mx = all_max<NT>(m, red, tid);
-    const float mm = isinf(mx) ? 0.f : mx;
     // (a thread without others has the sum 0, or NaN)
-    const float mt = isinf(m) ? 0.f : m;
-    s = all_sum<NT>(s == 0.f ? 0.f : s * __builtin_amdgcn_exp2f((mt - mm) * a.scale),
+    s = all_sum<NT>(s == 0.f ? 0.f
+                             : s * exp_from(isinf(m) ? 0.f : m,
+                                            isinf(mx) ? 0.f : mx),
                     red2, tid);
     if (tid == 0) {
         if (a.parts > 1) {
@@ -594,26 +624,24 @@ struct BeamArgs {
     double inv_t, scale;   // 1 / temperature; log2(e) / temperature
 };
 
-// 2^t for -1020 <= t <= 0 in 64 bits, to 7e-12 of itself: beams compete by the
+// 2^t for -1020 <= t <= 0 in 64 bits, to 8e-13 of itself: beams compete by the
 // difference of two log-sum-exps, for which 32 bits are too few.  Rounded to
 // the nearest integer n (by adding 1.5 * 2^52: n is then the low word too) the
-// rest f is at most 1/2, where the Taylor series of exp(f ln 2) is off by
-// (ln 2 / 2)^10 / 10! after its ninth power; n goes into the exponent's bits.
-// Additions and fused multiplications only.
+// rest is at most 1/2, where the polynomial of degree 8 with the least
+// largest relative error (found by a Remez exchange) is off by 7.8e-13; n
+// goes into the exponent's bits.  Additions and fused multiplications only.
 __device__ __forceinline__ double exp2_64(double t) {
     const double big = 6755399441055744.0;
     const double r = t + big, f = t - (r - big);
-    constexpr double L = 0.69314718055994530942;
-    double p = L * L * L * L * L * L * L * L * L / 362880.;
-    p = fma(p, f, L * L * L * L * L * L * L * L / 40320.);
-    p = fma(p, f, L * L * L * L * L * L * L / 5040.);
-    p = fma(p, f, L * L * L * L * L * L / 720.);
-    p = fma(p, f, L * L * L * L * L / 120.);
-    p = fma(p, f, L * L * L * L / 24.);
-    p = fma(p, f, L * L * L / 6.);
-    p = fma(p, f, L * L / 2.);
-    p = fma(p, f, L);
-    p = fma(p, f, 1.);
+    double p = 1.3175858821424589139e-6;
+    p = fma(p, f, 0.000015309737294734560971);
+    p = fma(p, f, 0.00015403851744514194029);
+    p = fma(p, f, 0.0013333452062791777427);
+    p = fma(p, f, 0.009618128542870409837);
+    p = fma(p, f, 0.05550410939341089077);
+    p = fma(p, f, 0.24022650698880322565);
+    p = fma(p, f, 0.69314718054651433602);
+    p = fma(p, f, 0.9999999999997623493);
     return __hiloint2double(__double2hiint(p) + (__double2loint(r) << 20),
                             __double2loint(p));
 }
