@@ -659,8 +659,10 @@ struct Exp64 {
 // Per beam row (or part of one): the `width` largest logits -- the row's
 // normaliser does not change their order -- and its maximum and sum, in one
 // pass.
+// (Long rows: 4 waves per SIMD, not 8, so that the eight exponentials in flight
+// stay in registers; it is bound by 64-bit arithmetic, not by latency.)
 template <int DT, int NT, bool ONE>
-__global__ __launch_bounds__(NT, 8) void beam_rows_kernel(BeamArgs a) {
+__global__ __launch_bounds__(NT, ONE ? 8 : 4) void beam_rows_kernel(BeamArgs a) {
     typedef typename RowType<DT>::T T;
     __shared__ TopLds<NT> lds;
     __shared__ float redf[NT / 64];
