@@ -16,7 +16,8 @@ namespace {
 //      lane of every (other) wave each; the k-th largest of the teams' largest
 //      keys is a bound that k elements reach at least, and not many more: with
 //      random data an element in 64 ln 2 / k teams' shares does, 44 for k = 32.
-//      It costs one sort of 64 keys (two), in registers;
+//      It costs one sort of 64 keys (two), in registers.  (A single wave sorts
+//      its lanes' keys, or both halves of their groups');
 //   2. the threads whose own key reaches it hold all of those elements (groups
 //      are disjoint stretches).  A wave reads such a thread's elements again, one
 //      per lane, and appends those at or above the bound to a list in LDS (ONE:
@@ -25,7 +26,8 @@ namespace {
 // Keys are distinct, so the order in 2 does not matter, and ties take no special
 // path.  A list that overflows (few teams hold most of the large elements) is
 // made by k passes instead.
-constexpr int top_room(int nt) { return nt == 64 ? 256 : 1024; }
+// (64 threads, 512 elements: fewer threads than k may hold all of them)
+constexpr int top_room(int nt) { return nt == 64 ? 512 : 1024; }
 template <int NT> struct TopLds {
     double list[NT / 64][64];
     double buf[top_room(NT)];
@@ -88,35 +90,25 @@ __device__ __forceinline__ double top_of_list(const double *keys, int n,
 template <int NT>
 __device__ __forceinline__ double bound_of(double key, int k, TopLds<NT> &lds,
                                            int lane, int wave) {
-    if constexpr (NT == 64) {
-        key = key_lane(key_sort(key, lane), k - 1);
-        __syncthreads();   // (lds.count)
-        return key;
-    } else {
-        lds.list[wave][lane] = key;
-        __syncthreads();
-        const bool two = k > 32;
-        if (wave < (two ? 2 : 1)) {
-            // 64 teams: lane l of all waves; 128: of the even, of the odd waves
-            key = lds.list[wave][lane];
+    lds.list[wave][lane] = key;
+    __syncthreads();
+    const bool two = k > 32;
+    if (wave < (two ? 2 : 1)) {
+        // 64 teams: lane l of all waves; 128: of the even, of the odd waves
 #pragma unroll
-            for (int w = 1; w < NT / 64; ++w)
-                if (!two || (w & 1) == wave)
-                    key = fmax(key, lds.list[w][lane]);
-            if (two && wave == 1) key = fmax(key, lds.list[1][lane]);
-            key = key_sort(key, lane);
-        }
-        if (two) {
-            __syncthreads();
-            if (wave == 1) lds.list[1][lane] = key;
-            __syncthreads();
-            if (wave == 0)
-                key = key_merge(fmax(key, lds.list[1][63 - lane]), lane);
-        }
-        if (wave == 0 && lane == k - 1) lds.bound = key;
-        __syncthreads();   // (and lds.count; the lists are free again)
-        return lds.bound;
+        for (int w = 0; w < NT / 64; ++w)
+            if (!two || (w & 1) == wave) key = fmax(key, lds.list[w][lane]);
+        key = key_sort(key, lane);
     }
+    if (two) {
+        __syncthreads();
+        if (wave == 1) lds.list[1][lane] = key;
+        __syncthreads();
+        if (wave == 0) key = key_merge(fmax(key, lds.list[1][63 - lane]), lane);
+    }
+    if (wave == 0 && lane == k - 1) lds.bound = key;
+    __syncthreads();   // (and lds.count; the lists are free again)
+    return lds.bound;
 }
 
 // Steps 1 (from the threads' maxima on) to 3.  bv, bg: the thread's maximum and
@@ -131,10 +123,35 @@ __device__ __forceinline__ double top_of_threads(
     typedef RowType<DT> R;
     const int lane = tid & 63, wave = tid >> 6;
     if (tid == 0) lds.count = lds.holders = 0;
-    const double key = bv > -INFINITY
-                           ? key_of(bv, first + (bg * NT + tid) * 8 + 7)
-                           : KEY_NONE;
-    const double bound = bound_of<NT>(key, k, lds, lane, wave);
+    double key = bv > -INFINITY ? key_of(bv, first + (bg * NT + tid) * 8 + 7)
+                                : KEY_NONE;
+    double bound;
+    if constexpr (NT == 64) {
+        // a wave has a key per lane, or (k > 32) one for each half of a group;
+        // of 128 elements all are candidates
+        if (n <= 128) {
+            bound = KEY_NONE;
+        } else if (k <= 32) {
+            bound = key_lane(key_sort(key, lane), k - 1);
+        } else {
+            double half[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float v = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v = fmaxf(v, q.get(4 * i + j));
+                half[i] = v > -INFINITY ? key_of(v, first + tid * 8 + 4 * i + 3)
+                                        : KEY_NONE;
+            }
+            key = fmax(half[0], half[1]);
+            half[0] = key_sort(half[0], lane);
+            half[1] = __shfl(key_sort(half[1], lane), 63 - lane, 64);
+            bound = key_lane(key_merge(fmax(half[0], half[1]), lane), k - 1);
+        }
+        __syncthreads();   // lds.count
+    } else {
+        bound = bound_of<NT>(key, k, lds, lane, wave);
+    }
     const float bound_v = bound == KEY_NONE ? -INFINITY : key_value(bound);
     slot = -1;
     if (key > KEY_NONE && key >= bound) {
@@ -277,24 +294,34 @@ template <int KT> struct ShortTop {
     }
 };
 // run the call with the constants LPR (lanes per row), G (groups of eight per
-// lane) and KT (list) for rows of V <= 512 and lists of k <= 16
+// lane) and KT (list) for short rows.  Four lanes
+// share a row of at most 128 where there are enough rows to fill the chip
+// with a wave for 16 of them, else sixteen.
 #define PCM_BY_SHORT_LIST(k, ...)                                     \
     do {                                                              \
         if ((k) <= 4) { constexpr int KT = 4; __VA_ARGS__; }          \
         else if ((k) <= 8) { constexpr int KT = 8; __VA_ARGS__; }     \
         else { constexpr int KT = 16; __VA_ARGS__; }                  \
     } while (0)
-#define PCM_BY_SHORT(V, k, ...)                                               \
+#define PCM_BY_SHORT(rows, V, k, ...)                                         \
     do {                                                                      \
-        if ((V) <= 64) {                                                      \
+        if ((V) <= 128 && (rows) < 8192) {                                    \
+            constexpr int LPR = 16, G = 1; PCM_BY_SHORT_LIST(k, __VA_ARGS__); \
+        } else if ((V) <= 64) {                                               \
             constexpr int LPR = 4, G = 2; PCM_BY_SHORT_LIST(k, __VA_ARGS__);  \
         } else if ((V) <= 128) {                                              \
             constexpr int LPR = 4, G = 4; PCM_BY_SHORT_LIST(k, __VA_ARGS__);  \
-        } else {                                                              \
+        } else if ((V) <= 512) {                                              \
             constexpr int LPR = 16, G = 4; PCM_BY_SHORT_LIST(k, __VA_ARGS__); \
+        } else {                                                              \
+            constexpr int LPR = 16, G = 8; PCM_BY_SHORT_LIST(k, __VA_ARGS__); \
         }                                                                     \
     } while (0)
-constexpr int SHORT_ROW = 512, SHORT_LIST = 16;
+// Rows of more than 128 only where there are many: sixteen lanes that share a row
+// take 14 x 804 logits in 46 us, a block for each (and the join) in 13.
+inline bool short_rows(long long rows, int V, int k) {
+    return k <= 16 && (V <= 128 || (V <= 1024 && rows >= 8192));
+}
 
 // ---- top logits -------------------------------------------------------------------
 struct TopArgs {
@@ -336,7 +363,7 @@ __device__ __forceinline__ float top_rest(float m, float s, float inv_t) {
     return isinf(m) ? m : m * inv_t + logf(s);
 }
 
-// Rows of at most 512, lists of at most 16.
+// Rows of at most 1024, lists of at most 16.
 template <int DT, int LPR, int G, int KT>
 __global__ __launch_bounds__(256) void top_short_kernel(TopArgs a, long long rows) {
     typedef RowType<DT> R;
@@ -720,9 +747,45 @@ __global__ __launch_bounds__(NT, ONE ? 8 : 4) void beam_rows_kernel(BeamArgs a) 
     }
 }
 
+// Places of the candidates of `rows` batch rows from b0 on, [row][beam][width],
+// every beam's own sorted: a candidate's place is the number of better ones,
+// counted list by list from the top until one is not better (or `width` of them
+// are): width + beams steps at most.  Lanes next to each other are of one batch
+// row and mostly read the same entry.
+__device__ __forceinline__ void beam_rank(const double *all_c, const int *all_f,
+                                          const BeamArgs &a, int rows, int b0) {
+    const int W = a.width, n = a.beams * W;
+    for (int at = threadIdx.x; at < rows * n; at += blockDim.x) {
+        const int r = at / n, i = at - r * n, own = i / W;
+        const double *c = all_c + r * n;
+        const int *f = all_f + r * n;
+        const double mine = c[i];
+        const int flat = f[i];
+        int place = i - own * W;
+        for (int k = 0; k < a.beams && place < W; ++k) {
+            if (k == own) continue;
+            for (int j = k * W; j < (k + 1) * W && place < W; ++j) {
+                if (!(c[j] > mine || (c[j] == mine && f[j] < flat))) break;
+                ++place;
+            }
+        }
+        if (place < W) {
+            const int from = flat / a.V, t = flat - from * a.V, b = b0 + r;
+            const long long o = (long long)place * a.batch + b;
+            a.tokens[o] = t;
+            a.parents[o] = from;
+            a.scores_out[o] = mine;
+            if (a.finished_out)
+                a.finished_out[o] =
+                    (a.finished && a.finished[(long long)from * a.batch + b]) ||
+                    t == a.end;
+        }
+    }
+}
+
 // One block per batch row, one wave per beam: the beam's parts become `width`
-// candidates with their scores; wave 0 ranks those of all beams (256 at most,
-// four per lane) by score, then beam and token.
+// candidates with their scores, all of which are ranked by score, then beam and
+// token.
 __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
     __shared__ double s_c[PCM_BEAM_MAX * PCM_BEAM_MAX];
     __shared__ int s_f[PCM_BEAM_MAX * PCM_BEAM_MAX];
@@ -783,51 +846,11 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
         s_f[k * W + lane] = tok < a.V ? k * a.V + tok : 0x7fffffff;
     }
     __syncthreads();
-    if (k != 0) return;
-    const int all = a.beams * W;
-    double cc[4];
-    int f[4];   // beam * V + token, 0x7fffffff where there is no candidate
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int at = lane + 64 * i;
-        f[i] = at < all ? s_f[at] : 0x7fffffff;
-        cc[i] = f[i] != 0x7fffffff ? s_c[at] : -INFINITY;
-    }
-    for (int j = 0; j < W; ++j) {
-        double bc = cc[0];
-        int bf = f[0];
-#pragma unroll
-        for (int i = 1; i < 4; ++i)
-            if (cc[i] > bc || (cc[i] == bc && f[i] < bf)) { bc = cc[i]; bf = f[i]; }
-        const double best = wave_max(bc);
-        // the lowest of those with this score
-        unsigned cand = bc == best ? (unsigned)bf : 0x7fffffffu;
-        cand = min(cand, lane_xor<1>(cand));
-        cand = min(cand, lane_xor<2>(cand));
-        cand = min(cand, lane_xor<4>(cand));
-        cand = min(cand, lane_xor<8>(cand));
-        cand = min(cand, lane_xor<16>(cand));
-        cand = min(cand, lane_xor<32>(cand));
-        bf = (int)cand;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (f[i] == bf) { cc[i] = -INFINITY; f[i] = 0x7fffffff; }
-        if (lane == 0) {
-            const int from = bf / a.V, t = bf - from * a.V;
-            const long long o = (long long)j * a.batch + b;
-            a.tokens[o] = t;
-            a.parents[o] = from;
-            a.scores_out[o] = best;
-            if (a.finished_out)
-                a.finished_out[o] =
-                    (a.finished && a.finished[(long long)from * a.batch + b]) ||
-                    t == a.end;
-        }
-    }
+    beam_rank(s_c, s_f, a, 1, b);
 }
 
 // Short rows, everything in one launch: a block takes 64 / LPR batch rows, one
-// wave per beam; a candidate's place is the number of better ones.
+// wave per beam.
 template <int DT, int LPR, int G, int KT>
 __global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
     typedef typename RowType<DT>::T T;
@@ -889,27 +912,8 @@ __global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
             }
     }
     __syncthreads();
-    const int rows = min(RB, a.batch - (int)blockIdx.x * RB);
-    for (int i = threadIdx.x; i < rows * per; i += blockDim.x) {
-        const int r = i / per;
-        const double c = beam_c[i];
-        const int f = beam_f[i];
-        int place = 0;
-        for (int j = r * per; j < (r + 1) * per; ++j)
-            place += beam_c[j] > c || (beam_c[j] == c && beam_f[j] < f);
-        if (place < a.width) {
-            const int from = f / a.V, t = f - from * a.V;
-            const int bb = blockIdx.x * RB + r;
-            const long long o = (long long)place * a.batch + bb;
-            a.tokens[o] = t;
-            a.parents[o] = from;
-            a.scores_out[o] = c;
-            if (a.finished_out)
-                a.finished_out[o] =
-                    (a.finished && a.finished[(long long)from * a.batch + bb]) ||
-                    t == a.end;
-        }
-    }
+    beam_rank(beam_c, beam_f, a, min(RB, a.batch - (int)blockIdx.x * RB),
+              blockIdx.x * RB);
 }
 
 // How a row of V logits is dealt out: `parts` blocks of `len` elements each.
@@ -1127,8 +1131,8 @@ int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
     a.inv_t = (float)(1.0 / temperature);
     PCM_REQUIRE(rows * plan.parts < (1ll << 31), PCM_EINVAL,
                 "top_logits: too many rows");
-    if (vocab <= SHORT_ROW && k <= SHORT_LIST) {
-        PCM_BY_DTYPE(dtype, PCM_BY_SHORT(vocab, k, {
+    if (short_rows(rows, vocab, k)) {
+        PCM_BY_DTYPE(dtype, PCM_BY_SHORT(rows, vocab, k, {
             constexpr int per_block = 256 / LPR;
             hipLaunchKernelGGL((top_short_kernel<DT, LPR, G, KT>),
                                dim3((unsigned)((rows + per_block - 1) / per_block)),
@@ -1154,8 +1158,8 @@ size_t pcm_beam_select_workspace_bytes(int32_t beams, int32_t batch,
     if (beams < 1 || batch < 1 || width < 1 || vocab < 1 ||
         vocab > PCM_MAX_VOCAB)
         return 0;
-    if (vocab <= SHORT_ROW) return 0;
     const size_t rows = (size_t)beams * batch;
+    if (short_rows(rows, vocab, width)) return 0;
     return rows * row_plan(rows, vocab).parts * (width + 2) * sizeof(double);
 }
 
@@ -1211,8 +1215,8 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
     a.parts = plan.parts; a.len = plan.len; a.end = end_token;
     a.inv_t = 1.0 / temperature;
     a.scale = 1.4426950408889634 / temperature;
-    if (vocab <= SHORT_ROW) {
-        PCM_BY_DTYPE(dtype, PCM_BY_SHORT(vocab, width, {
+    if (short_rows(rows, vocab, width)) {
+        PCM_BY_DTYPE(dtype, PCM_BY_SHORT(rows, vocab, width, {
             constexpr int per_block = 64 / LPR;
             const size_t lds = (size_t)per_block * beams * width *
                                (sizeof(double) + sizeof(int));
