@@ -685,6 +685,16 @@ int pcm_distill_loss(const void *logits, int32_t dtype, int64_t ld,
                 "distill_loss: hard_weight=%f outside 0..1", hard_weight);
     PCM_REQUIRE(hard_weight == 0. || targets, PCM_EINVAL,
                 "distill_loss: hard_weight needs targets");
+    // (a launch has less than 2^32 threads)
+    PCM_REQUIRE(vocab <= 2048 || (long long)steps * batch < (1ll << 22),
+                PCM_EINVAL, "distill_loss: %lld rows of %d logits are too many "
+                "for a launch", (long long)steps * batch, vocab);
+    PCM_REQUIRE(vocab <= 512 || (long long)steps * batch < (1ll << 24),
+                PCM_EINVAL, "distill_loss: %lld rows of %d logits are too many "
+                "for a launch", (long long)steps * batch, vocab);
+    PCM_REQUIRE((long long)steps * batch < (1ll << 28), PCM_EINVAL,
+                "distill_loss: %lld rows are too many for a launch",
+                (long long)steps * batch);
     hipStream_t st = (hipStream_t)stream;
     DistillArgs a;
     a.logits = logits; a.values = values; a.indices = indices; a.rest = rest;

@@ -53,12 +53,13 @@ __device__ __forceinline__ int held_at(int g0, int holder, int lane) {
     return ((g0 + (lane >> 3)) * NT + holder) * 8 + (lane & 7);
 }
 
-// the 64 largest of the waves' sorted lists; in wave 0 afterwards
+// the 64 largest of the first `lists` waves' sorted lists; in wave 0 afterwards
 template <int NT>
 __device__ __forceinline__ double merge_waves(double v, double (*list)[64],
-                                              int lane, int wave) {
+                                              int lists, int lane, int wave) {
     if constexpr (NT > 64) {
         for (int s = NT / 128; s > 0; s >>= 1) {
+            if (s >= lists) continue;
             if (wave >= s && wave < 2 * s) list[wave][lane] = v;
             __syncthreads();
             if (wave < s)
@@ -82,7 +83,7 @@ __device__ __forceinline__ double top_of_list(const double *keys, int n,
         const double turned = __shfl(x, 63 - lane, 64);
         v = c == wave * 64 ? x : key_merge(fmax(v, turned), lane);
     }
-    if (n > 64) v = merge_waves<NT>(v, list, lane, wave);
+    if (n > 64) v = merge_waves<NT>(v, list, (n + 63) / 64, lane, wave);
     return v;
 }
 
@@ -937,6 +938,12 @@ RowPlan row_plan(long long rows, int V) {
     p.parts = (V + p.len - 1) / p.len;
     return p;
 }
+// A launch has less than 2^32 threads: may these rows be one?
+bool rows_fit(long long rows, int V, int k, const RowPlan &p) {
+    if (short_rows(rows, V, k)) return rows < (1ll << 28);
+    const int threads = p.len <= 512 ? 64 : p.len <= 2048 ? 256 : 1024;
+    return rows * p.parts * threads < (1ll << 32);
+}
 // run the call with the constants NT (threads) and ONE (a group of eight per
 // thread) for a stretch of `len` elements
 #define PCM_BY_LENGTH(len, ...)                                                \
@@ -1129,8 +1136,9 @@ int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
     a.ld = ld; a.V = vocab; a.k = k; a.parts = plan.parts; a.len = plan.len;
     a.scale = (float)(1.4426950408889634 / temperature);
     a.inv_t = (float)(1.0 / temperature);
-    PCM_REQUIRE(rows * plan.parts < (1ll << 31), PCM_EINVAL,
-                "top_logits: too many rows");
+    PCM_REQUIRE(rows_fit(rows, vocab, k, plan), PCM_EINVAL,
+                "top_logits: %lld rows of %d logits are too many for a launch",
+                (long long)rows, vocab);
     if (short_rows(rows, vocab, k)) {
         PCM_BY_DTYPE(dtype, PCM_BY_SHORT(rows, vocab, k, {
             constexpr int per_block = 256 / LPR;
@@ -1203,8 +1211,9 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
     hipStream_t st = (hipStream_t)stream;
     const long long rows = (long long)beams * batch;
     const RowPlan plan = row_plan(rows, vocab);
-    PCM_REQUIRE(rows * plan.parts < (1ll << 31), PCM_EINVAL,
-                "beam_select: too many rows");
+    PCM_REQUIRE(rows_fit(rows, vocab, width, plan), PCM_EINVAL,
+                "beam_select: %lld rows of %d logits are too many for a launch",
+                rows, vocab);
     BeamArgs a;
     a.logits = logits; a.scores = scores; a.finished = finished;
     a.keys = (double *)workspace;

@@ -207,6 +207,8 @@ def test_top_logits_refusals():
     _refused(lib, call(vocab=100, ld=100, k=65), 'k=65')
     _refused(lib, call(tau=0.0), 'temperature')
     _refused(lib, call(tau=float('nan')), 'temperature')
+    _refused(lib, call(rows=1 << 28), 'too many')
+    _refused(lib, call(rows=1 << 22, vocab=9000, ld=9000), 'too many')
 
 
 def test_distill_refusals():
@@ -226,6 +228,11 @@ def test_distill_refusals():
     _refused(lib, call(steps=0), 'shape')
     _refused(lib, call(vocab=(1 << 18) + 1, ld=1 << 20), 'shape')
     _refused(lib, call(steps=1 << 16, batch=1 << 16), 'rows')
+    _refused(lib, call(steps=1 << 14, batch=1 << 14), 'too many')
+    _refused(lib, call(steps=1 << 12, batch=1 << 12, vocab=600, ld=600),
+             'too many')
+    _refused(lib, call(steps=1 << 11, batch=1 << 11, vocab=9000, ld=9000),
+             'too many')
     _refused(lib, call(ld=3), 'row stride')
     _refused(lib, call(k=0), 'k=0')
     _refused(lib, call(k=65), 'k=65')
@@ -261,6 +268,7 @@ def test_beam_refusals():
     _refused(lib, call(vocab=0, ld=0), 'vocab=0')
     _refused(lib, call(ld=19), 'row stride')
     _refused(lib, call(tau=0.0), 'temperature')
+    _refused(lib, call(batch=1 << 22, vocab=9000, ld=9000), 'too many')
     _refused(lib, call(end=20), 'end_token')
     _refused(lib, call(end=-1), 'end_token')
     _refused(lib, call(done=None), 'finished_out')
