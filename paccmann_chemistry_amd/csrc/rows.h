@@ -173,10 +173,12 @@ static __device__ __forceinline__ T all_sum(T v, T *red, int tid) {
 }
 
 // ---- sorting 64 keys across a wave ------------------------------------------------------
+// (one comparison and a choice: a maximum of values that a lane swap brought would
+// be preceded by two that quiet NaNs, which keys never are)
 template <int STRIDE>
 static __device__ __forceinline__ double key_exchange(double v, bool keep_max) {
     const double o = lane_xor<STRIDE>(v);
-    return keep_max ? fmax(v, o) : fmin(v, o);
+    return (v > o) == keep_max ? v : o;
 }
 template <int SIZE, int STRIDE>
 static __device__ __forceinline__ double key_sort_steps(double v, int lane) {

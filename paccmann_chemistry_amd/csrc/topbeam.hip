@@ -36,22 +36,36 @@ template <int NT> struct TopLds {
     int holders, count;
 };
 
-// What a wave has read of its holders again: those number wave, wave + NT / 64,
-// ... of at most 64, sixteen groups each (two per lane), all loads in flight at
-// once.  More holders or longer stretches are read where they are needed.
-template <int NT> struct Held {
-    static constexpr int N = 4096 / NT;   // 64 / (NT / 64)
-    float v[N][2];
-    static __device__ __forceinline__ bool fits(int n, int holders) {
-        return n <= NT * 128 && holders <= 64;
-    }
-};
 // element of thread `holder` that `lane` looks at when a wave reads eight of its
 // groups from g0 on
 template <int NT>
 __device__ __forceinline__ int held_at(int g0, int holder, int lane) {
     return ((g0 + (lane >> 3)) * NT + holder) * 8 + (lane & 7);
 }
+// Holders that a wave reads again: of the SPAN from h0 on, those at h0 + wave,
+// h0 + wave + NT / 64, ...; sixteen groups each (two elements per lane), all
+// loads in flight at once.  Longer stretches are read where they are needed.
+template <int DT, int NT> struct Held {
+    static constexpr int N = 4096 / NT, SPAN = 64;
+    float v[N][2];
+    static __device__ __forceinline__ bool fits(int n) { return n <= NT * 128; }
+    __device__ __forceinline__ void load(const typename RowType<DT>::T *p, int n,
+                                         const TopLds<NT> &lds, int h0,
+                                         int holders, int lane, int wave) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int h = h0 + wave + i * (NT / 64);
+            if (h < holders) {
+                const int holder = lds.held[h];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int e = held_at<NT>(t * 8, holder, lane);
+                    v[i][t] = e < n ? RowType<DT>::up(p[e]) : -INFINITY;
+                }
+            }
+        }
+    }
+};
 
 // the 64 largest of the first `lists` waves' sorted lists; in wave 0 afterwards
 template <int NT>
@@ -119,7 +133,7 @@ __device__ __forceinline__ double bound_of(double key, int k, TopLds<NT> &lds,
 template <int DT, int NT, bool ONE>
 __device__ __forceinline__ double top_of_threads(
     const typename RowType<DT>::T *p, const Row8<DT> &q, int n, int first, int k,
-    float bv, int bg, TopLds<NT> &lds, Held<NT> &held, int tid, int &found,
+    float bv, int bg, TopLds<NT> &lds, Held<DT, NT> &held, int tid, int &found,
     int &slot) {
     typedef RowType<DT> R;
     const int lane = tid & 63, wave = tid >> 6;
@@ -185,28 +199,20 @@ __device__ __forceinline__ double top_of_threads(
             }
         }
     };
+    typedef Held<DT, NT> H;
     if (ONE) {
-    } else if (Held<NT>::fits(n, holders)) {
+    } else if (H::fits(n)) {
+        for (int h0 = 0; h0 < holders; h0 += H::SPAN) {
+            held.load(p, n, lds, h0, holders, lane, wave);
 #pragma unroll
-        for (int i = 0; i < Held<NT>::N; ++i) {
-            const int h = wave + i * (NT / 64);
-            if (h < holders) {
-                const int holder = lds.held[h];
+            for (int i = 0; i < H::N; ++i) {
+                const int h = h0 + wave + i * (NT / 64);
+                if (h < holders) {
+                    const int holder = lds.held[h];
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int e = held_at<NT>(t * 8, holder, lane);
-                    held.v[i][t] = e < n ? R::up(p[e]) : -INFINITY;
+                    for (int t = 0; t < 2; ++t)
+                        append(held.v[i][t], held_at<NT>(t * 8, holder, lane));
                 }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < Held<NT>::N; ++i) {
-            const int h = wave + i * (NT / 64);
-            if (h < holders) {
-                const int holder = lds.held[h];
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    append(held.v[i][t], held_at<NT>(t * 8, holder, lane));
             }
         }
     } else {
@@ -242,20 +248,41 @@ __device__ __forceinline__ double top_of_threads(
 }
 
 // ---- the largest of a short row ---------------------------------------------------
-// LPR lanes share a row, each sorts what it holds into a list of KT by insertion
-// (two instructions per place: v_max_f64, v_min_f64), then the lanes' lists are
-// merged pairwise; every lane ends with the row's list.  A row of 60 costs about
-// 30 instructions of a wave this way (16 rows in it) against 800 for a wave per
-// row.  All elements are ranked, -inf and NaN too.
+// LPR lanes share a row; each sorts its groups of eight (19 comparators of two
+// instructions, v_max_f64 and v_min_f64), merges them into a list of KT, then the
+// lanes' lists are merged pairwise; every lane ends with the row's list.  A row
+// of 60 costs about 40 instructions of a wave this way (16 rows in it) against
+// 800 for a wave per row.  All elements are ranked, -inf and NaN too.
 template <int KT> struct ShortTop {
     double l[KT];
-    __device__ __forceinline__ void add(double key) {
+    static __device__ __forceinline__ void order(double &a, double &b) {
+        const double hi = fmax(a, b);
+        b = fmin(a, b);
+        a = hi;
+    }
+    static __device__ __forceinline__ void sort8(double (&g)[8]) {
+        constexpr int net[19][2] = {
+            {0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6},
+            {5, 7}, {1, 2}, {5, 6}, {0, 4}, {3, 7}, {1, 5}, {2, 6},
+            {1, 4}, {3, 6}, {2, 4}, {3, 5}, {3, 4}};
 #pragma unroll
-        for (int j = 0; j < KT; ++j) {
-            const double hi = fmax(l[j], key);
-            key = fmin(l[j], key);
-            l[j] = hi;
-        }
+        for (int i = 0; i < 19; ++i) order(g[net[i][0]], g[net[i][1]]);
+    }
+    // l is bitonic: sort it
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int s = KT / 2; s > 0; s >>= 1)
+#pragma unroll
+            for (int j = 0; j < KT; ++j)
+                if ((j & s) == 0) order(l[j], l[j + s]);
+    }
+    // the list and a sorted group: its largest meet the list's smallest
+    __device__ __forceinline__ void take(const double (&g)[8]) {
+        constexpr int N = KT < 8 ? KT : 8;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            l[KT - 1 - j] = fmax(l[KT - 1 - j], g[j]);
+        settle();
     }
     template <int M> __device__ __forceinline__ void merge() {
         double o[KT];
@@ -263,15 +290,7 @@ template <int KT> struct ShortTop {
         for (int j = 0; j < KT; ++j) o[j] = lane_xor<M>(l[j]);
 #pragma unroll
         for (int j = 0; j < KT; ++j) l[j] = fmax(l[j], o[KT - 1 - j]);
-#pragma unroll
-        for (int s = KT / 2; s > 0; s >>= 1)
-#pragma unroll
-            for (int j = 0; j < KT; ++j)
-                if ((j & s) == 0) {
-                    const double hi = fmax(l[j], l[j + s]);
-                    l[j + s] = fmin(l[j], l[j + s]);
-                    l[j] = hi;
-                }
+        settle();
     }
     template <int DT, int LPR, int G>
     __device__ __forceinline__ void of(const RowRegs<DT, LPR, G> &x, int V,
@@ -279,13 +298,22 @@ template <int KT> struct ShortTop {
 #pragma unroll
         for (int j = 0; j < KT; ++j) l[j] = KEY_NONE;
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g) {
+            double e[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int at = x.at(g, sub) + j;
                 const double key = key_of(x.r[g].get(j), at);
-                add(at < V ? key : KEY_NONE);
+                e[j] = at < V ? key : KEY_NONE;
             }
+            sort8(e);
+            if (g == 0) {
+#pragma unroll
+                for (int j = 0; j < (KT < 8 ? KT : 8); ++j) l[j] = e[j];
+            } else {
+                take(e);
+            }
+        }
         merge<1>();
         merge<2>();
         if constexpr (LPR == 16) {
@@ -466,7 +494,7 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
         each_group<DT, NT>(p, n, tid, pass);
     }
     int found, slot;
-    Held<NT> held;
+    Held<DT, NT> held;   // (afterwards: the last SPAN of them)
     const double key = top_of_threads<DT, NT, ONE>(
         p, own, n, first, a.k, m, bg, lds, held, tid, found, slot);
     if (tid < 64) {
@@ -493,30 +521,34 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
     auto is_other = [&](float v, int e) {
         return v < last_v || (v == last_v && e > last_i);
     };
+    typedef Held<DT, NT> H;
     if (ONE) {
-    } else if (Held<NT>::fits(n, holders)) {
+    } else if (H::fits(n)) {
+        for (int h0 = 0; h0 < holders; h0 += H::SPAN) {
+            if (holders > H::SPAN) held.load(p, n, lds, h0, holders, lane, wave);
 #pragma unroll
-        for (int i = 0; i < Held<NT>::N; ++i) {
-            const int h = wave + i * (NT / 64);
-            if (h < holders) {
-                const int holder = lds.held[h];
-                float ov[2];
-                bool nan = false;
+            for (int i = 0; i < H::N; ++i) {
+                const int h = h0 + wave + i * (NT / 64);
+                if (h < holders) {
+                    const int holder = lds.held[h];
+                    float ov[2];
+                    bool nan = false;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const float v = held.v[i][t];
-                    nan |= v != v;
-                    ov[t] = is_other(v, held_at<NT>(t * 8, holder, lane))
-                                ? v : -INFINITY;
-                }
-                const float om = wave_max(fmaxf(ov[0], ov[1]));
-                const float mm = isinf(om) ? 0.f : om;
-                const float os =
-                    wave_sum(exp_from(ov[0], mm) + exp_from(ov[1], mm));
-                nan = __any(nan);
-                if (lane == 0) {
-                    s_m[h] = om;
-                    s_s[h] = nan ? NAN : os;
+                    for (int t = 0; t < 2; ++t) {
+                        const float v = held.v[i][t];
+                        nan |= v != v;
+                        ov[t] = is_other(v, held_at<NT>(t * 8, holder, lane))
+                                    ? v : -INFINITY;
+                    }
+                    const float om = wave_max(fmaxf(ov[0], ov[1]));
+                    const float mm = isinf(om) ? 0.f : om;
+                    const float os =
+                        wave_sum(exp_from(ov[0], mm) + exp_from(ov[1], mm));
+                    nan = __any(nan);
+                    if (lane == 0) {
+                        s_m[h] = om;
+                        s_s[h] = nan ? NAN : os;
+                    }
                 }
             }
         }
@@ -734,7 +766,7 @@ __global__ __launch_bounds__(NT, ONE ? 8 : 4) void beam_rows_kernel(BeamArgs a) 
         each_group<DT, NT>(p, n, tid, pass);
     }
     int found, slot;
-    Held<NT> held;
+    Held<DT, NT> held;   // (afterwards: the last SPAN of them)
     const double key = top_of_threads<DT, NT, ONE>(
         p, own, n, first, a.width, m, bg, lds, held, tid, found, slot);
     if (tid < a.width) a.keys[(row * a.parts + part) * a.width + lane] = key;
@@ -918,16 +950,21 @@ __global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
 }
 
 // How a row of V logits is dealt out: `parts` blocks of `len` elements each.
-// Few rows leave most of the 256 CUs idle, so long ones are split until there
-// are about 512 blocks or a part is down to 4096 elements; the join costs one more
-// launch.
+// Few rows leave most of the 256 CUs idle, so rows of at least `least` are split
+// until there are about 512 blocks or a part is down to 4096 elements.  Joining
+// top logits is a launch more: it pays beyond 131072 (top 12 of one row of 131071:
+// 18 us in two launches, 14.6 in one; of 262144: 18 and 22), for long lists beyond
+// 65536 (top 64 of one of 65536: 18 and 15; of 131071: 18 and 21).  Beams are joined
+// anyway.
+constexpr int top_split(int k) { return k > 32 ? 65537 : 131073; }
+constexpr int BEAM_SPLIT = 8193;
 struct RowPlan {
     int parts, len;
 };
-RowPlan row_plan(long long rows, int V) {
+RowPlan row_plan(long long rows, int V, int least) {
     RowPlan p;
     long long parts = 1;
-    if (rows < 256) {
+    if (rows < 256 && V >= least) {
         long long want = 512 / rows, most = V / 4096;
         if (want > most) want = most;
         if (want > 64) want = 64;
@@ -945,8 +982,11 @@ bool rows_fit(long long rows, int V, int k, const RowPlan &p) {
     return rows * p.parts * threads < (1ll << 32);
 }
 // run the call with the constants NT (threads) and ONE (a group of eight per
-// thread) for a stretch of `len` elements
-#define PCM_BY_LENGTH(len, ...)                                                \
+// thread) for `blocks` stretches of `len` elements.  Long ones: 1024 threads while
+// that fills the chip (top 64 of one row of 32767: 13.5 us against 18 with 512),
+// 512 when there are enough blocks that one computes while another loads (top 32
+// of 1024 x 50021: 34 us against 43 with 1024 and 63 with 256).
+#define PCM_BY_LENGTH(blocks, len, ...)                                        \
     do {                                                                       \
         if ((len) <= 512) {                                                    \
             constexpr int NT = 64; constexpr bool ONE = true; __VA_ARGS__;     \
@@ -956,10 +996,13 @@ bool rows_fit(long long rows, int V, int k, const RowPlan &p) {
             constexpr int NT = 512; constexpr bool ONE = true; __VA_ARGS__;    \
         } else if ((len) <= 8192) {                                            \
             constexpr int NT = 1024; constexpr bool ONE = true; __VA_ARGS__;   \
+        } else if ((blocks) < 256) {                                           \
+            constexpr int NT = 1024; constexpr bool ONE = false; __VA_ARGS__;  \
         } else {                                                               \
             constexpr int NT = 512; constexpr bool ONE = false; __VA_ARGS__;   \
         }                                                                      \
     } while (0)
+
 // ---- states follow their beams ------------------------------------------------------
 struct ReorderState {
     char *data;
@@ -1096,7 +1139,7 @@ extern "C" {
 
 size_t pcm_top_logits_workspace_bytes(int64_t rows, int32_t vocab, int32_t k) {
     if (rows < 1 || vocab < 1 || vocab > PCM_MAX_VOCAB || k < 1) return 0;
-    const RowPlan p = row_plan(rows, vocab);
+    const RowPlan p = row_plan(rows, vocab, top_split(k));
     if (p.parts == 1) return 0;
     return (size_t)rows * p.parts * (64 * sizeof(double) + 2 * sizeof(float));
 }
@@ -1127,7 +1170,7 @@ int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
     PCM_REQUIRE(((uintptr_t)workspace & 7) == 0, PCM_EINVAL,
                 "top_logits: workspace must be 8-byte aligned");
     hipStream_t st = (hipStream_t)stream;
-    const RowPlan plan = row_plan(rows, vocab);
+    const RowPlan plan = row_plan(rows, vocab, top_split(k));
     TopArgs a;
     a.logits = logits; a.values = values; a.indices = indices; a.rest = rest;
     a.keys = (double *)workspace;
@@ -1148,7 +1191,7 @@ int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
         }));
         return pcm_check_launch("top_logits");
     }
-    PCM_BY_DTYPE(dtype, PCM_BY_LENGTH(plan.len, {
+    PCM_BY_DTYPE(dtype, PCM_BY_LENGTH(rows * plan.parts, plan.len, {
         hipLaunchKernelGGL((top_kernel<DT, NT, ONE>),
                            dim3((unsigned)(rows * plan.parts)), dim3(NT), 0, st,
                            a);
@@ -1168,7 +1211,7 @@ size_t pcm_beam_select_workspace_bytes(int32_t beams, int32_t batch,
         return 0;
     const size_t rows = (size_t)beams * batch;
     if (short_rows(rows, vocab, width)) return 0;
-    return rows * row_plan(rows, vocab).parts * (width + 2) * sizeof(double);
+    return rows * row_plan(rows, vocab, BEAM_SPLIT).parts * (width + 2) * sizeof(double);
 }
 
 int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
@@ -1210,7 +1253,7 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
                 "beam_select: workspace must be 8-byte aligned");
     hipStream_t st = (hipStream_t)stream;
     const long long rows = (long long)beams * batch;
-    const RowPlan plan = row_plan(rows, vocab);
+    const RowPlan plan = row_plan(rows, vocab, BEAM_SPLIT);
     PCM_REQUIRE(rows_fit(rows, vocab, width, plan), PCM_EINVAL,
                 "beam_select: %lld rows of %d logits are too many for a launch",
                 rows, vocab);
@@ -1235,7 +1278,7 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
         }));
         return pcm_check_launch("beam_select");
     }
-    PCM_BY_DTYPE(dtype, PCM_BY_LENGTH(plan.len, {
+    PCM_BY_DTYPE(dtype, PCM_BY_LENGTH(rows * plan.parts, plan.len, {
         hipLaunchKernelGGL((beam_rows_kernel<DT, NT, ONE>),
                            dim3((unsigned)(rows * plan.parts)), dim3(NT), 0, st,
                            a);
