@@ -459,7 +459,7 @@ int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
  *            other tokens no probability.  A row without any teacher
  *            probability has no distillation term
  *   targets  int64[T*B], needed when hard_weight > 0 (clamped like
- *            pcm_softmax_ce's)
+ *            pcm_softmax_ce's); with hard_weight 1 the teacher is not looked at
  *   loss     fp32[1]; dlogits (nullable) [T*B][vocab] of `dtype`, dense: zero in
  *            rows that take no part, whatever their logits hold
  *   scratch  fp32[pcm_distill_scratch_floats(T, B)]

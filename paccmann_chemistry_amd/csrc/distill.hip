@@ -203,7 +203,7 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
                 }
     __syncthreads();
     // teacher, and the listed tokens' part of the student
-    const bool taught = um > -INFINITY || (flags & 1);
+    const bool taught = a.soft > 0.f && (um > -INFINITY || (flags & 1));
     const float uo = finite_or_0(um);
     float us = 0.f, xm = -INFINITY;
     if (live)
@@ -445,7 +445,7 @@ distill_row_kernel(DistillArgs a) {
         }
         const float um = wave_max(fmaxf(u, rest));
         const bool bad = __any(u != u || rest != rest);
-        const bool taught = um > -INFINITY || bad;
+        const bool taught = a.soft > 0.f && (um > -INFINITY || bad);
         const float uo = finite_or_0(um);
         const float e = __builtin_amdgcn_exp2f((u - uo) * LOG2E);
         const float ro = __builtin_amdgcn_exp2f((rest - uo) * LOG2E);
@@ -593,6 +593,8 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float *x,
     }
 }
 
+// (16-bit gradients of a loss that is scaled are rounded twice, half a step each;
+// the usual factor is 1, for which they stay as they are)
 template <int DT>
 __global__ __launch_bounds__(256) void scale_kernel(typename RowType<DT>::T *x,
                                                     long long n,

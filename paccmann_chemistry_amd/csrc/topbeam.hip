@@ -323,9 +323,8 @@ template <int KT> struct ShortTop {
     }
 };
 // run the call with the constants LPR (lanes per row), G (groups of eight per
-// lane) and KT (list) for short rows.  Four lanes
-// share a row of at most 128 where there are enough rows to fill the chip
-// with a wave for 16 of them, else sixteen.
+// lane) and KT (list) for short rows.  Four lanes share a row of at most 128 where
+// there are enough rows to fill the chip with a wave for 16 of them, else sixteen.
 #define PCM_BY_SHORT_LIST(k, ...)                                     \
     do {                                                              \
         if ((k) <= 4) { constexpr int KT = 4; __VA_ARGS__; }          \
@@ -706,13 +705,14 @@ __device__ __forceinline__ double exp2_64(double t) {
                             __double2loint(p));
 }
 // exp of logits relative to a maximum m (finite): (v - m) / temperature, in powers
-// of two; what is below 2^-1000 counts as 2^-1000
+// of two; what is below 2^-1000 counts as 2^-1000.  The difference first: of a
+// product less a rounded product 3e38 times temperature leaves 1e22, of either sign.
 struct Exp64 {
-    double scale, shift;
-    __device__ __forceinline__ Exp64(double scale_, float m)
-        : scale(scale_), shift(-(double)m * scale_) {}
+    double scale, m;
+    __device__ __forceinline__ Exp64(double scale_, float m_)
+        : scale(scale_), m((double)m_) {}
     __device__ __forceinline__ double operator()(float v) const {
-        return exp2_64(fmax(fma((double)v, scale, shift), -1000.));
+        return exp2_64(fmax(((double)v - m) * scale, -1000.));
     }
 };
 

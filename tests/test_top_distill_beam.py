@@ -383,6 +383,10 @@ def test_distill_definition_by_differences():
     (2, 8192, 64, 'sorted'), (2, 33001, 17, 'masked'), (1, 70001, 64, 'ties'),
     (2, 65536, 64, 'same'), (1, 131071, 7, 'normal'),
     (1, 262144, 64, 'normal'), (300, 700, 4, 'normal'),
+    (2, 416, 53, 'normal'), (2, 321, 61, 'ties'), (9000, 129, 9, 'lowest'),
+    (8192, 700, 16, 'ties'), (300, 9000, 64, 'lowest'),
+    (2, 131071, 64, 'lowest'), (1, 140000, 33, 'sorted'),
+    (3, 262144, 40, 'same'), (2, 100, 20, 'masked'), (5, 17, 17, 'far'),
 ])
 def test_top_logits(dtype, rows, vocab, k, kind):
     import paccmann_chemistry_amd as P
@@ -636,7 +640,7 @@ def test_distill_values_that_are_not_numbers():
             loss = P.distill_loss(
                 xd, P.TopLogits(values.to(dev), indices.to(dev), rest.to(dev),
                                 tau), lengths=one.to(dev))
-            value = float(loss)
+            value = float(loss.detach())
             grad, = torch.autograd.grad(loss, xd)
             others = [r for r in range(6) if r != b]
             assert bool((grad[0, others] == 0).all())
@@ -647,6 +651,32 @@ def test_distill_values_that_are_not_numbers():
                 assert math.isnan(value)
             else:
                 assert math.isfinite(value)
+
+
+@gpu
+@pytest.mark.parametrize('V', [60, 300, 900, 5000])
+def test_distill_on_targets_alone(V):
+    """hard_weight 1: the cross entropy, whatever the teacher says."""
+    import paccmann_chemistry_amd as P
+    g = _gen(V, 13)
+    dev = _dev()
+    logits, values, indices, rest, tau = _distill_case(
+        2, 3, V, 5, torch.float32, 'normal', True, g, absent=False)
+    targets = torch.randint(0, V, (2, 3), generator=g)
+    values[0, 0, 1] = math.nan
+    rest[0, 1] = math.inf
+    logits[0, 2, indices[0, 2, 0].long()] = -math.inf
+    targets[0, 2] = indices[0, 2, 1]
+    ref_loss, ref = ref_distill(
+        logits, torch.zeros_like(values), torch.full_like(indices, -1), None,
+        tau, targets, None, 1.0)
+    xd = logits.to(dev).requires_grad_(True)
+    loss = P.distill_loss(
+        xd, P.TopLogits(values.to(dev), indices.to(dev), rest.to(dev), tau),
+        targets=targets.to(dev), hard_weight=1.0)
+    grad, = torch.autograd.grad(loss, xd)
+    _check_distill(loss, grad.cpu(), ref_loss, ref, logits,
+                   _weights(2, 3, None, None), tau, 1.0, V, torch.float32)
 
 
 @gpu
@@ -757,7 +787,10 @@ def _check_beam(step, want, logits):
     (3, 2, 1000, 16, 'lowest', False), (8, 3, 5003, 8, 'normal', True),
     (2, 2, 8192, 3, 'sorted', False), (4, 1, 131071, 4, 'normal', False),
     (2, 1, 262144, 16, 'normal', True), (5, 130, 33, 5, 'far', False),
-    (1, 2, 70001, 16, 'normal', False),
+    (1, 2, 70001, 16, 'normal', False), (3, 30, 60, 3, 'lowest', False),
+    (2, 40, 300, 4, 'lowest', True), (3, 70, 5003, 8, 'lowest', False),
+    (4, 2, 131071, 4, 'lowest', False), (2, 300, 8300, 3, 'lowest', False),
+    (3, 2731, 700, 5, 'lowest', True),
 ])
 def test_beam_select(dtype, K, B, V, W, kind, ends):
     import paccmann_chemistry_amd as P
