@@ -129,6 +129,8 @@ __device__ __forceinline__ RowStats row_stats(const DistillArgs &a, float w,
 // with a wave per row.  The row is in registers; a copy in LDS is where the
 // listed tokens are looked up, and where the gradients meet: of the others from the
 // registers, of the listed ones and the target from their entries.
+// 61440 ragged x 60 fp32, k = 8, with targets: 15.5 us for 24.6 MB (1.6 TB/s), bound
+// by the instructions and LDS accesses of the lists; a wave per row took 201 us.
 template <int DT, int LPR, int G, bool HARD>
 __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
     typedef RowType<DT> R;
@@ -330,16 +332,22 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
 
 // ---- longer rows ----------------------------------------------------------------
 // One block per row.  KEEP: the row stays in registers, read once and written
-// once; else it is read twice.  Wave 0 holds
-// the list, one entry per lane; the listed tokens are marked in a bitmap in LDS
-// -- a group of eight elements is one byte of it -- and become -inf in the
-// registers, so the passes see the others only.
-template <int DT, int NT, int G, bool HARD, bool KEEP>
+// once; else it is read twice.  Wave 0 holds the list, one entry per lane; the
+// listed tokens are marked in a bitmap in LDS -- a group of eight elements is one
+// byte of it -- and become -inf in the registers, so the passes see the others
+// only.  What bounds it is memory, as long as two blocks fit a CU and one loads
+// while the other computes: 2048 x 32000 bf16 in 56 us (4.7 TB/s, what a large
+// copy reaches), 1024 ragged x 50021 fp32 with targets in 87 us (3.6 TB/s: at most
+// four rows per CU, so two turns of loads with little to hide behind); 7 x 601 fp16 in 4.6 us (latency).
+// LG: up to so many more groups of a thread are kept in LDS, in the threads' order
+// (each thread reads what it wrote: no barrier).
+template <int DT, int NT, int G, bool HARD, bool KEEP, int LG = 0>
 __global__ __launch_bounds__(NT, KEEP ? row_waves(DT, NT, G) : 8) void
 distill_row_kernel(DistillArgs a) {
+    static_assert(LG == 0 || (KEEP && DT == PCM_DTYPE_F32), "fp32 halves in LDS");
     typedef RowType<DT> R;
     typedef typename R::T T;
-    extern __shared__ unsigned marks[];   // a bit per element
+    extern __shared__ __align__(16) unsigned marks[];   // a bit per element
     __shared__ float red[NT / 64], red2[NT / 64];
     __shared__ float s_list[6];
     // what wave 0 needs of its list after the passes (registers are the row's)
@@ -350,7 +358,7 @@ distill_row_kernel(DistillArgs a) {
     const int V = a.V, k = a.k;
     const float w = uniform(row_weight(a, row));
     T *dl = a.dlogits ? (T *)a.dlogits + row * V : nullptr;
-    const int groups = KEEP ? G : (V + NT * 8 - 1) / (NT * 8);
+    const int groups = KEEP ? G + LG : (V + NT * 8 - 1) / (NT * 8);
     if (w == 0.f) {
         if (tid == 0) a.rowloss[row] = 0.f;
         if (dl)
@@ -366,6 +374,27 @@ distill_row_kernel(DistillArgs a) {
     const T *x = (const T *)a.logits + row * a.ld;
     RowRegs<DT, NT, G> regs;
     if (KEEP) regs.load(x, V, tid);
+    const int words = groups * NT / 4;   // groups * NT bytes
+    // a group in LDS: the first halves of all its threads, then the second ones
+    // (neighbours 16 bytes apart: no bank is asked twice)
+    auto each_kept = [&](auto f) {
+#pragma unroll 1
+        for (int l = 0; l < LG; ++l) {
+            const int e = ((G + l) * NT + tid) * 8;
+            if (e >= V) break;
+            const int last = (V - (G + l) * NT * 8 + 7) / 8;
+            float *lo = (float *)(marks + words) + l * NT * 8 + tid * 4;
+            f(e, G + l, (row_u32x4 *)lo,
+              (row_u32x4 *)(lo + 4 * (last < NT ? last : NT)));
+        }
+    };
+    if constexpr (LG > 0)
+        each_kept([&](int e, int, row_u32x4 *lo, row_u32x4 *hi) {
+            Row8<DT> q;
+            load_group(q, x, V, e);
+            *lo = q.a;
+            *hi = q.b;
+        });
     // the list: lane j of wave 0 holds entry j
     int idx = -1, tg = -1;
     float u = -INFINITY, lx = -INFINITY, xt = 0.f, rest = -INFINITY;
@@ -383,7 +412,6 @@ distill_row_kernel(DistillArgs a) {
             }
         }
     }
-    const int words = groups * NT / 4;   // groups * NT bytes
     for (int i = tid; i < words; i += NT) marks[i] = 0;
     __syncthreads();
     bool first = false;
@@ -408,6 +436,20 @@ distill_row_kernel(DistillArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) m = fmaxf(m, regs.r[g].get(j));
         }
+        if constexpr (LG > 0)
+            each_kept([&](int, int g, row_u32x4 *lo, row_u32x4 *hi) {
+                Row8<DT> q;
+                q.a = *lo;
+                q.b = *hi;
+                const unsigned bits = mark8[g * NT + tid];
+                if (bits) {
+                    q.drop(bits);
+                    *lo = q.a;
+                    *hi = q.b;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = fmaxf(m, q.get(j));
+            });
     } else {
         // maximum and sums in one pass, relative to the thread's running maximum
         each_group<DT, NT>(x, V, tid, [&](Row8<DT> &q, int g) {
@@ -484,17 +526,27 @@ distill_row_kernel(DistillArgs a) {
     m = uniform(all_max<NT>(m, red, tid));
     const float mo = finite_or_0(m);
     if (KEEP) {
+        auto add = [&](const Row8<DT> &q) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float d = q.get(j) - mo;
+                s += __builtin_amdgcn_exp2f(d * a.scale);
+                if (HARD) h += __builtin_amdgcn_exp2f(d * LOG2E);
+            }
+        };
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             regs.r[g].touch(s);
             if (HARD) regs.r[g].touch(h);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float d = regs.r[g].get(j) - mo;
-                s += __builtin_amdgcn_exp2f(d * a.scale);
-                if (HARD) h += __builtin_amdgcn_exp2f(d * LOG2E);
-            }
+            add(regs.r[g]);
         }
+        if constexpr (LG > 0)
+            each_kept([&](int, int, row_u32x4 *lo, row_u32x4 *hi) {
+                Row8<DT> q;
+                q.a = *lo;
+                q.b = *hi;
+                add(q);
+            });
     } else {
         // (a thread without others has the sums 0, or NaN)
         if (!(s == 0.f)) s *= __builtin_amdgcn_exp2f((mt - mo) * a.scale);
@@ -546,6 +598,13 @@ distill_row_kernel(DistillArgs a) {
             regs.r[g].touch();
             write(g, regs.r[g]);
         }
+        if constexpr (LG > 0)
+            each_kept([&](int, int g, row_u32x4 *lo, row_u32x4 *hi) {
+                Row8<DT> q;
+                q.a = *lo;
+                q.b = *hi;
+                write(g, q);
+            });
     } else {
         each_group<DT, NT>(x, V, tid, [&](Row8<DT> &q, int g) {
             unlist(q, g);
@@ -611,6 +670,11 @@ __global__ __launch_bounds__(256) void scale_kernel(typename RowType<DT>::T *x,
 // Up to 65536 a row stays in the registers of its block (read once): 1552 rows of
 // 32768 in 96 us (fp32) and 51 us (bf16) against 111 and 60 when it is read
 // twice, 776 of 65536 in 110 and 55 against 121 and 63.
+// With 32-bit logits past 32768 the registers of a row leave one block per CU, which
+// loads and computes in turn; two fit where what is past 32768 lies in LDS: 1024
+// rows of 50944 in 106 us (111 with targets) against 115 (126) of 50945 in
+// registers alone.
+constexpr int KEPT_MAX = 50944;   // (two blocks of at most 80 KB of LDS)
 template <int DT, bool HARD>
 long long launch_rows(const DistillArgs &a, hipStream_t st) {
     const int V = a.V;
@@ -638,7 +702,12 @@ long long launch_rows(const DistillArgs &a, hipStream_t st) {
     else if (V <= 8192) PCM_DISTILL_ROWS(256, 4);
     else if (V <= 16384) PCM_DISTILL_ROWS(512, 4);
     else if (V <= 32768) PCM_DISTILL_ROWS(1024, 4);
-    else if (V <= 65536) PCM_DISTILL_ROWS(1024, 8);
+    else if (DT == PCM_DTYPE_F32 && V <= KEPT_MAX) {
+        // past 32768 in LDS, beside the bitmap
+        const size_t lds = 7 * 1024 + (size_t)(V - 32768 + 7) / 8 * 32;
+        hipLaunchKernelGGL((distill_row_kernel<PCM_DTYPE_F32, 1024, 4, HARD, true, 3>),
+                           dim3((unsigned)a.rows), dim3(1024), lds, st, a);
+    } else if (V <= 65536) PCM_DISTILL_ROWS(1024, 8);
 #undef PCM_DISTILL_ROWS
     else {
         const size_t lds = (size_t)(V + 8191) / 8192 * 1024;
@@ -681,8 +750,9 @@ int pcm_distill_loss(const void *logits, int32_t dtype, int64_t ld,
                 (long long)ld, vocab);
     PCM_REQUIRE(k >= 1 && k <= PCM_TOP_MAX, PCM_EINVAL,
                 "distill_loss: k=%d outside 1..%d", k, PCM_TOP_MAX);
-    PCM_REQUIRE(temperature > 1e-30 && temperature < 1e30, PCM_EINVAL,
-                "distill_loss: temperature must be positive");
+    // (the loss carries its square, in 32 bits)
+    PCM_REQUIRE(temperature >= 1e-3 && temperature <= 1e3, PCM_EINVAL,
+                "distill_loss: temperature outside 1e-3..1e3");
     PCM_REQUIRE(hard_weight >= 0. && hard_weight <= 1., PCM_EINVAL,
                 "distill_loss: hard_weight=%f outside 0..1", hard_weight);
     PCM_REQUIRE(hard_weight == 0. || targets, PCM_EINVAL,

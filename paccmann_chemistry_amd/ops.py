@@ -893,8 +893,8 @@ def distill_loss(logits, teacher, targets=None, lengths=None, hard_weight=0.0,
         (1 - hard_weight) temperature^2 KL(teacher || student)
             + hard_weight * cross entropy(logits, targets)
 
-    with both distributions at the teacher's temperature over its listed tokens
-    and "any other token", summed over steps after weighting step t by
+    with both distributions at the teacher's temperature (1e-3..1e3) over its
+    listed tokens and "any other token", summed over steps after weighting step t by
     ``step_weight[t]`` (default: one over the rows with ``lengths > t``), as
     ``DecoderHeadFn`` reduces its cross entropy.  Returns an fp32 scalar that
     carries the gradient of the logits.  Indices outside the vocabulary raise
@@ -910,6 +910,8 @@ def distill_loss(logits, teacher, targets=None, lengths=None, hard_weight=0.0,
     _check_vocab(vocab)
     values, indices, rest, temperature = teacher
     temperature = _check_temperature(temperature)
+    if not 1e-3 <= temperature <= 1e3:   # (the loss carries its square)
+        raise ValueError(f'temperature {temperature}: expected 1e-3..1e3')
     dev = logits.device
     if indices.dim() != 3 or not 1 <= indices.shape[-1] <= _lib.TOP_MAX:
         raise ValueError(

@@ -237,6 +237,9 @@ def test_distill_refusals():
     _refused(lib, call(k=0), 'k=0')
     _refused(lib, call(k=65), 'k=65')
     _refused(lib, call(tau=-1.0), 'temperature')
+    _refused(lib, call(tau=1e-20), 'temperature')   # its square is 0 in 32 bits
+    _refused(lib, call(tau=1e20), 'temperature')    # its square is infinite
+    _refused(lib, call(tau=float('nan')), 'temperature')
     _refused(lib, call(hard=1.5), 'hard_weight')
     _refused(lib, call(hard=float('nan')), 'hard_weight')
     _refused(lib, call(targets=None), 'targets')
@@ -518,6 +521,11 @@ def _check_distill(got_loss, got, ref_loss, ref, logits, weights, tau, hard,
     (1, 3, 2050, 17, 'normal', True, 0.0, False),
     (2, 2, 5003, 33, 'normal', True, 0.25, True),
     (1, 2, 33001, 64, 'normal', True, 0.25, False),
+    (1, 2, 32769, 3, 'far', True, 0.5, False),
+    (2, 2, 40960, 33, 'lowest', False, 0.0, True),
+    (1, 3, 50021, 64, 'normal', True, 0.25, False),
+    (1, 1, 50944, 64, 'ties', True, 1.0, False),
+    (1, 1, 50945, 64, 'ties', True, 0.0, False),
     (1, 2, 65537, 9, 'normal', True, 0.5, False),
     (1, 1, 140001, 9, 'normal', True, 0.5, False),
 ])
@@ -562,7 +570,7 @@ def test_distill(dtype, T, B, V, k, kind, rest, hard, ragged):
 
 
 @gpu
-@pytest.mark.parametrize('V', [60, 700, 5000])
+@pytest.mark.parametrize('V', [60, 700, 5000, 45001])
 def test_distill_odd_teachers(V):
     """A list with the same index twice, an empty one, one whose values are all
     -inf, indices outside the vocabulary, no probability for the others, a
