@@ -482,8 +482,9 @@ int pcm_scale(void *x, int32_t dtype, int64_t n, const float *scale,
  * One selection of a beam search over beams AND vocabulary: the `width` best of
  * the beams * vocab candidates
  *   c[k][v] = scores[k][b] + logits[k][b][v] / temperature - lse[k][b]
- * of every batch row b, best first, equal ones by lowest k * vocab + v.  Scores
- * are carried, summed and compared in 64 bits.  (BeamSearch.step of the
+ * of every batch row b, best first, equal ones by lowest k * vocab + v (of one
+ * beam the larger logit first, also where the sums round to one).  Scores are
+ * carried, summed and compared in 64 bits.  (BeamSearch.step of the
  * reference, utils/search.py:247-275, ranks top_tokens candidates per beam.)
  *
  *   logits   rows k * batch + b of `vocab` elements, row stride ld

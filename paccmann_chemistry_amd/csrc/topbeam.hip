@@ -680,41 +680,45 @@ struct BeamArgs {
     uint8_t *finished_out;
     long long ld;
     int beams, batch, V, width, parts, len, end;
-    double inv_t, scale;   // 1 / temperature; log2(e) / temperature
+    double inv_t;         // 1 / temperature
+    double scale, least;  // log2(e) / temperature; the difference 2^-1000 is of
 };
 
-// 2^t for -1020 <= t <= 0 in 64 bits, to 8e-13 of itself: beams compete by the
-// difference of two log-sum-exps, for which 32 bits are too few.  Rounded to
-// the nearest integer n (by adding 1.5 * 2^52: n is then the low word too) the
-// rest is at most 1/2, where the polynomial of degree 8 with the least
-// largest relative error (found by a Remez exchange) is off by 7.8e-13; n
+// exp of logits relative to a maximum m (finite) in 64 bits, to 8e-13 of itself:
+// beams compete by the difference of two log-sum-exps, for which 32 bits are too
+// few.  d = v - m first (of a product less a rounded product 3e38 times
+// temperature leaves 1e22, of either sign); what is below 2^-1000 counts as that.
+// d scale, rounded to the nearest integer n (by adding 1.5 * 2^52: n is then the
+// low word too), leaves at most 1/2, where the polynomial of degree 8 with the
+// least largest relative error (found by a Remez exchange) is off by 7.8e-13; n
 // goes into the exponent's bits.  Additions and fused multiplications only.
-__device__ __forceinline__ double exp2_64(double t) {
-    const double big = 6755399441055744.0;
-    const double r = t + big, f = t - (r - big);
-    double p = 1.3175858821424589139e-6;
-    p = fma(p, f, 0.000015309737294734560971);
-    p = fma(p, f, 0.00015403851744514194029);
-    p = fma(p, f, 0.0013333452062791777427);
-    p = fma(p, f, 0.009618128542870409837);
-    p = fma(p, f, 0.05550410939341089077);
-    p = fma(p, f, 0.24022650698880322565);
-    p = fma(p, f, 0.69314718054651433602);
-    p = fma(p, f, 0.9999999999997623493);
-    return __hiloint2double(__double2hiint(p) + (__double2loint(r) << 20),
-                            __double2loint(p));
-}
-// exp of logits relative to a maximum m (finite): (v - m) / temperature, in powers
-// of two; what is below 2^-1000 counts as 2^-1000.  The difference first: of a
-// product less a rounded product 3e38 times temperature leaves 1e22, of either sign.
 struct Exp64 {
-    double scale, m;
-    __device__ __forceinline__ Exp64(double scale_, float m_)
-        : scale(scale_), m((double)m_) {}
+    double scale, least, m;
+    __device__ __forceinline__ Exp64(const BeamArgs &a, float m_)
+        : scale(a.scale), least(a.least), m((double)m_) {}
     __device__ __forceinline__ double operator()(float v) const {
-        return exp2_64(fmax(((double)v - m) * scale, -1000.));
+        const double big = 6755399441055744.0;
+        const double d = fmax((double)v - m, least);
+        const double r = fma(d, scale, big), f = fma(d, scale, -(r - big));
+        double p = 1.3175858821424589139e-6;
+        p = fma(p, f, 0.000015309737294734560971);
+        p = fma(p, f, 0.00015403851744514194029);
+        p = fma(p, f, 0.0013333452062791777427);
+        p = fma(p, f, 0.009618128542870409837);
+        p = fma(p, f, 0.05550410939341089077);
+        p = fma(p, f, 0.24022650698880322565);
+        p = fma(p, f, 0.69314718054651433602);
+        p = fma(p, f, 0.9999999999997623493);
+        return __hiloint2double(__double2hiint(p) + (__double2loint(r) << 20),
+                                __double2loint(p));
     }
 };
+// score of a candidate: the differences first here too (a row whose tokens all
+// hold the type's lowest value is uniform)
+__device__ __forceinline__ double beam_score(const BeamArgs &a, double score,
+                                             float v, double m, double log_s) {
+    return score + (((double)v - m) * a.inv_t - log_s);
+}
 
 // Per beam row (or part of one): the `width` largest logits -- the row's
 // normaliser does not change their order -- and its maximum and sum, in one
@@ -748,12 +752,12 @@ __global__ __launch_bounds__(NT, ONE ? 8 : 4) void beam_rows_kernel(BeamArgs a) 
             nan |= v[j] != v[j];
         }
         if (gm > m) {
-            if (m > -INFINITY) s *= Exp64(a.scale, gm)(m);
+            if (m > -INFINITY) s *= Exp64(a, gm)(m);
             m = gm;
             bg = g;
         }
         // (without any element above -inf yet, or with a +inf: not used)
-        const Exp64 e(a.scale, isinf(m) ? 0.f : m);
+        const Exp64 e(a, isinf(m) ? 0.f : m);
         double sum = 0.;
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += e(v[j]);
@@ -772,7 +776,7 @@ __global__ __launch_bounds__(NT, ONE ? 8 : 4) void beam_rows_kernel(BeamArgs a) 
     if (tid < a.width) a.keys[(row * a.parts + part) * a.width + lane] = key;
     const float mx = all_max<NT>(nan ? INFINITY : m, redf, tid);
     if (!isinf(mx))
-        s = all_sum<NT>(m == -INFINITY ? 0. : s * Exp64(a.scale, mx)(m), red, tid);
+        s = all_sum<NT>(m == -INFINITY ? 0. : s * Exp64(a, mx)(m), red, tid);
     if (tid == 0) {
         double *q = a.part + (row * a.parts + part) * 2;
         q[0] = mx;   // +inf: a NaN or +inf in this part, no distribution
@@ -784,7 +788,8 @@ __global__ __launch_bounds__(NT, ONE ? 8 : 4) void beam_rows_kernel(BeamArgs a) 
 // every beam's own sorted: a candidate's place is the number of better ones,
 // counted list by list from the top until one is not better (or `width` of them
 // are): width + beams steps at most.  Lanes next to each other are of one batch
-// row and mostly read the same entry.
+// row and mostly read the same entry.  An entry's flat place is 2 (beam V + token),
+// plus 1 if the beam had ended (a load of `finished` here would be 0.3 us more).
 __device__ __forceinline__ void beam_rank(const double *all_c, const int *all_f,
                                           const BeamArgs &a, int rows, int b0) {
     const int W = a.width, n = a.beams * W;
@@ -803,15 +808,14 @@ __device__ __forceinline__ void beam_rank(const double *all_c, const int *all_f,
             }
         }
         if (place < W) {
-            const int from = flat / a.V, t = flat - from * a.V, b = b0 + r;
+            const int id = flat >> 1, from = id / a.V, t = id - from * a.V;
+            const int b = b0 + r;
             const long long o = (long long)place * a.batch + b;
             a.tokens[o] = t;
             a.parents[o] = from;
             a.scores_out[o] = mine;
             if (a.finished_out)
-                a.finished_out[o] =
-                    (a.finished && a.finished[(long long)from * a.batch + b]) ||
-                    t == a.end;
+                a.finished_out[o] = (flat & 1) || t == a.end;
         }
     }
 }
@@ -847,8 +851,8 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
         tok = lane;   // a row without a distribution: the tokens in order
         if (!isinf(m)) {
             const double s = wave_sum(
-                ps > 0. ? ps * Exp64(a.scale, (float)m)((float)pm) : 0.);
-            const double lse = m * a.inv_t + log(s);
+                ps > 0. ? ps * Exp64(a, (float)m)((float)pm) : 0.);
+            const double log_s = log(s);
             if (a.parts > 1) key = key_sort(key, lane);
             for (int at = 64; at < n; at += 64) {
                 const double x =
@@ -859,7 +863,7 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
             const int found = __popcll(__ballot(real));
             if (real) {
                 tok = key_index(key);
-                c = score + ((double)key_value(key) * a.inv_t - lse);
+                c = beam_score(a, score, key_value(key), m, log_s);
             } else if (lane < W) {
                 // fewer tokens above -inf: the lowest ones that are not listed
                 int want = lane - found, t = 0;
@@ -876,7 +880,8 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
     }
     if (lane < W) {
         s_c[k * W + lane] = c;
-        s_f[k * W + lane] = tok < a.V ? k * a.V + tok : 0x7fffffff;
+        s_f[k * W + lane] =
+            tok < a.V ? 2 * (k * a.V + tok) + (done ? 1 : 0) : 0x7fffffff;
     }
     __syncthreads();
     beam_rank(s_c, s_f, a, 1, b);
@@ -898,7 +903,8 @@ __global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
         const long long row = (long long)k * a.batch + b;
         const double score = a.scores[row];
         const bool done = a.finished && a.finished[row];
-        double lse = 0.;
+        double log_s = 0.;
+        float m = 0.f;
         bool live = !done && score > -INFINITY;
         ShortTop<KT> top;
         if (live) {
@@ -914,17 +920,17 @@ __global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
                     nan |= v != v;
                 }
             // (the list's first is the maximum; a NaN anywhere ends the row)
-            const float m = row_max<LPR>(nan ? INFINITY : key_value(top.l[0]));
+            m = row_max<LPR>(nan ? INFINITY : key_value(top.l[0]));
             live = !isinf(m);
             if (live) {
-                const Exp64 e(a.scale, m);
+                const Exp64 e(a, m);
                 double s = 0.;
 #pragma unroll
                 for (int g = 0; g < G; ++g)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) s += e(x.r[g].get(j));
                 s = row_sum<LPR>(s);
-                lse = (double)m * a.inv_t + log(s);
+                log_s = log(s);
             }
         }
 #pragma unroll
@@ -937,11 +943,12 @@ __global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
                     if (j == 0 && score == score) c = score;
                 } else if (live) {
                     tok = top.l[j] > KEY_NONE ? key_index(top.l[j]) : a.V;
-                    c = score + ((double)key_value(top.l[j]) * a.inv_t - lse);
+                    c = beam_score(a, score, key_value(top.l[j]), m, log_s);
                 }
                 const int at = rb * per + k * a.width + j;
                 beam_c[at] = tok < a.V ? c : -INFINITY;
-                beam_f[at] = tok < a.V ? k * a.V + tok : 0x7fffffff;
+                beam_f[at] = tok < a.V ? 2 * (k * a.V + tok) + (done ? 1 : 0)
+                                       : 0x7fffffff;
             }
     }
     __syncthreads();
@@ -1267,6 +1274,7 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
     a.parts = plan.parts; a.len = plan.len; a.end = end_token;
     a.inv_t = 1.0 / temperature;
     a.scale = 1.4426950408889634 / temperature;
+    a.least = -1000. / a.scale;
     if (short_rows(rows, vocab, width)) {
         PCM_BY_DTYPE(dtype, PCM_BY_SHORT(rows, vocab, width, {
             constexpr int per_block = 64 / LPR;

@@ -127,8 +127,7 @@ def ref_beam(logits, scores, width, tau, finished=None, end=None):
             if not s > -math.inf or bool(torch.isnan(x).any()) or \
                     not math.isfinite(float(x.max())):
                 continue
-            x = x / tau
-            c[k, b] = s + (x - torch.logsumexp(x, 0))
+            c[k, b] = s + torch.log_softmax(x / tau, 0)
     flat = c.permute(1, 0, 2).reshape(batch, -1)
     best, at = torch.sort(flat, dim=-1, descending=True, stable=True)
     best, at = best[:, :width].t(), at[:, :width].t()
@@ -850,6 +849,23 @@ def test_beam_select_of_rows_without_a_distribution(V):
     _check_beam(step, want, logits)
     want = ref_beam(logits, scores, 2, 1.0)
     step = P.beam_select(logits.to(dev), scores.to(dev), width=2)
+    _check_beam(step, want, logits)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('V', [20, 60, 700, 9000])
+def test_beam_select_where_all_tokens_are_masked(dtype, V):
+    """Masks of the type's lowest value over a whole row: it is uniform."""
+    import paccmann_chemistry_amd as P
+    logits = torch.full((2, 3, V), torch.finfo(dtype).min, dtype=dtype)
+    logits[1, 1] = 0.5
+    scores = torch.tensor([[-1.0, -1.0, -2.0], [-1.5, -0.5, -1.0]],
+                          dtype=torch.float64)
+    want = ref_beam(logits, scores, 2, 0.8)
+    assert float(want[2][0, 0]) == pytest.approx(-1.0 - math.log(V))
+    dev = _dev()
+    step = P.beam_select(logits.to(dev), scores.to(dev), temperature=0.8)
     _check_beam(step, want, logits)
 
 
