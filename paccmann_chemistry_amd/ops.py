@@ -751,6 +751,14 @@ def _operand(t, what, device, shape, *dtypes):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _status_word(status, device):
+    if status is not None and (status.dtype != torch.int32
+                               or status.device != device
+                               or status.numel() != 1):
+        raise ValueError(f'status: expected one int32 on {device}')
+    return status
+
+
 def _rows_of(x, what):
     """(tensor kept alive, rows, row stride) of ``x[..., V]``."""
     if x.is_contiguous():
@@ -874,6 +882,8 @@ class DistillLossFn(torch.autograd.Function):
                 'distill_loss backward called twice: the gradient is handed '
                 'out by the first call (retain_graph is not supported)'
             )
+        if dloss.requires_grad:
+            raise RuntimeError('distill_loss has no second derivative')
         ctx.dlogits = None
         # (an fp32 scalar; autograd's thread has the device and the stream of
         # the forward)
@@ -898,7 +908,9 @@ def distill_loss(logits, teacher, targets=None, lengths=None, hard_weight=0.0,
     ``step_weight[t]`` (default: one over the rows with ``lengths > t``), as
     ``DecoderHeadFn`` reduces its cross entropy.  Returns an fp32 scalar that
     carries the gradient of the logits.  Indices outside the vocabulary raise
-    STATUS_BAD_TOKEN in ``status`` (see ``check_status``)."""
+    STATUS_BAD_TOKEN in ``status`` (see ``check_status``).  Into a graph,
+    forward and backward are captured together, while no eager autograd graph
+    of the same leaves is alive."""
     require_device(logits, 'distill logits')
     code = _dtype_code(logits, 'distill logits')
     size = logits.shape
@@ -941,7 +953,7 @@ def distill_loss(logits, teacher, targets=None, lengths=None, hard_weight=0.0,
             dev, (steps, ), torch.float32
         )
     args = (code, vocab, values, indices, rest, temperature, targets, lengths,
-            hard_weight, step_weight, status)
+            hard_weight, step_weight, _status_word(status, dev))
     if logits.requires_grad and torch.is_grad_enabled():
         return DistillLossFn.apply(logits, args)
     return _distill(logits, False, args)[0]
@@ -1096,6 +1108,7 @@ def reorder_states(parents, states, row_dims=0, status=None):
                              f'state {len(table) // 5}')
     if not parents.is_contiguous():
         parents = parents.contiguous()
+    _status_word(status, dev)
     with _on(dev):
         check(
             lib.pcm_reorder_states(

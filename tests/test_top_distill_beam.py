@@ -762,6 +762,15 @@ def test_distill_refusals_of_tensors():
         P.distill_loss(x, good, step_weight=torch.ones(3, device=dev))
     with pytest.raises(TypeError):
         P.distill_loss(x.double(), good)
+    with pytest.raises(ValueError):
+        P.distill_loss(x, P.TopLogits(v, i, None, 1e20))
+    with pytest.raises(ValueError):
+        P.distill_loss(x, good, status=torch.zeros(1, dtype=torch.int32))
+    leaf = x.clone().requires_grad_(True)
+    grad = torch.ones((), device=dev, requires_grad=True)
+    with pytest.raises(RuntimeError, match='second derivative'):
+        torch.autograd.grad(P.distill_loss(leaf, good), leaf, grad,
+                            create_graph=True)
 
 
 # --------------------------------------------------------------------------
@@ -996,6 +1005,8 @@ def test_reorder_views_bad_parents_and_refusals():
     with pytest.raises(ValueError):
         P.reorder_states(p, [got.requires_grad_(True)])
     y = torch.randn(K * B, 5, device=dev)
+    with pytest.raises(ValueError):
+        P.reorder_states(p, [y], status=torch.zeros(1, device=dev))
     with pytest.raises(P._lib.PaccmannHipError, match='memory'):
         P.reorder_states(p, [y, y])
     with pytest.raises(P._lib.PaccmannHipError, match='memory'):
