@@ -448,8 +448,7 @@ int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
  *          + hard * cross entropy(logits, target)
  *   loss = sum_t weight_t sum_b row(t, b)
  * over the rows with lengths[b] > t; weight_t = step_weight[t], or one over the
- * number of those rows (as pcm_softmax_ce).  temperature 1e-3..1e3; the KL is
- * summed in 32 bits, so the first term is known to about temperature^2 2^-20.
+ * number of those rows (as pcm_softmax_ce).  temperature 1e-3..1e3.
  *
  *   logits   [T*B] rows (t * B + b) of `vocab` elements, row stride ld
  *   values   [T*B][k] of values_dtype, indices int32[T*B][k]: a negative index

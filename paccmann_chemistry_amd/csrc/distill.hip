@@ -10,6 +10,15 @@
 // listed ones, so q_rest keeps its digits when the list holds nearly
 // everything (lse(all) minus the list would not), and the gradient of the others
 // is exp(x - m_R) times ONE factor per row.
+//
+// Where student and teacher are near each other the terms of the first sum cancel:
+// logarithms of 10 known to 1e-6 for a sum of 1e-3.  Probabilities of the outcomes
+// sum to 1 on both sides, so with d = log q - log p
+//   sum p (log p - log q) = sum p (e^d - 1 - d),
+// terms that are not negative, in which an error of a normaliser, common to all d,
+// is multiplied by sum (q - p) = 0.  d and e^d - 1 - d are taken in 64 bits, for the
+// k + 1 outcomes only; the normalisers' logarithm in 32.  (An outcome without p adds its q; an index that appears
+// twice has its q once.)
 #include "rows.h"
 
 namespace {
@@ -27,7 +36,8 @@ struct DistillArgs {
     long long ld, rows;
     int B, V, k, values_dtype;
     float weight_all;
-    float inv_t, scale;    // 1 / tau; log2(e) / tau
+    double inv_t64;        // 1 / tau
+    float inv_t, scale;    // the same; log2(e) / tau
     float soft, hard;      // (1 - hard) tau^2; hard
     float dsoft;           // (1 - hard) tau
 };
@@ -87,12 +97,18 @@ __device__ __forceinline__ float uniform(float v) {
     return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
 }
 
+// p (log p - log q) + q - p of an outcome, d = log q - log p.  (Below 1e-30 p has
+// lost digits, and what it adds to q is nothing unless q is 0.)
+__device__ __forceinline__ float kl_term(float p, double d, float q) {
+    if (!(p <= 1e-30f)) return (float)((double)p * (expm1(d) - d));
+    return p == 0.f ? q : (float)((double)q - (double)p * (1. + d));
+}
+
 // What a row's factors are made of: the others' maximum m and sum(s), the listed
 // tokens' xm and sums, the teacher's.  (Sums relative to exp(max).)
 struct RowStats {
     float ma;        // maximum of the row
     float sa, ha;    // sums over the row relative to it: / tau, plain
-    float other;     // log q_rest
     float cq, ch;    // gradient of an other token: exp((x - mo) / tau) cq +
                      // exp(x - mo) ch
 };
@@ -107,7 +123,6 @@ __device__ __forceinline__ RowStats row_stats(const DistillArgs &a, float w,
     const float fo = s == 0.f ? 0.f : exp_below(mo, r.ma, a.scale);
     const float fx = xs == 0.f ? 0.f : exp_below(xo, r.ma, a.scale);
     r.sa = s * fo + xs * fx;
-    r.other = (mo - r.ma) * a.inv_t + logf(s) - logf(r.sa);
     r.cq = 0.f;
     if (taught)
         r.cq = a.dsoft * w * (fo / r.sa - (pr > 0.f && s > 0.f ? pr / s : 0.f));
@@ -129,8 +144,9 @@ __device__ __forceinline__ RowStats row_stats(const DistillArgs &a, float w,
 // with a wave per row.  The row is in registers; a copy in LDS is where the
 // listed tokens are looked up, and where the gradients meet: of the others from the
 // registers, of the listed ones and the target from their entries.
-// 61440 ragged x 60 fp32, k = 8, with targets: 15.5 us for 24.6 MB (1.6 TB/s), bound
-// by the instructions and LDS accesses of the lists; a wave per row took 201 us.
+// 61440 ragged x 60 fp32, k = 8, with targets: 18.4 us for 24.6 MB (1.3 TB/s), bound
+// by the instructions and LDS accesses of the lists (2.5 us of it are the loss's 64
+// bits); a wave per row took 201 us.
 template <int DT, int LPR, int G, bool HARD>
 __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
     typedef RowType<DT> R;
@@ -140,7 +156,7 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
     const int lane = threadIdx.x, r = lane / LPR, sub = lane % LPR;
     const int V = a.V, k = a.k, LD = V | 1, LK = k | 1;
     float *tile = sm + r * LD;                         // a row: logits, gradients
-    float *u = sm + ROWS * LD + r * LK;                // its list: u, then p
+    float *u = sm + ROWS * LD + r * LK;                // its list: values, then p
     float *lx = sm + ROWS * (LD + LK) + r * LK;        // its logits
     int *li = (int *)(sm + ROWS * (LD + 2 * LK)) + r * LK;   // its indices; -1:
                                 // absent; -2 - index: an earlier entry has it
@@ -160,7 +176,7 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
         for (int j = sub; j < k; j += LPR) {
             const int idx = teacher_index(a, row * k + j);
             li[j] = idx;
-            u[j] = idx < 0 ? -INFINITY : teacher_value(a, row * k + j) * a.inv_t;
+            u[j] = idx < 0 ? -INFINITY : teacher_value(a, row * k + j);
         }
         for (int i = sub; i < MW; i += LPR) marks[i] = 0;
 #pragma unroll
@@ -178,7 +194,7 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
         if (HARD) xt = tile[tg];
         for (int j = sub; j < k; j += LPR) {
             const int idx = li[j];
-            um = fmaxf(um, u[j]);
+            um = fmaxf(um, u[j] * a.inv_t);
             if (u[j] != u[j]) flags |= 1;
             lx[j] = idx < 0 ? -INFINITY : tile[idx];
             if (idx >= 0) {
@@ -210,14 +226,14 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
     float us = 0.f, xm = -INFINITY;
     if (live)
         for (int j = sub; j < k; j += LPR) {
-            us += __builtin_amdgcn_exp2f((u[j] - uo) * LOG2E);
+            us += __builtin_amdgcn_exp2f((u[j] * a.inv_t - uo) * LOG2E);
             if (li[j] >= 0) xm = fmaxf(xm, lx[j]);
         }
     us = row_sum<LPR>(us);
     xm = row_max<LPR>(xm);
     const float ro = __builtin_amdgcn_exp2f((rest - uo) * LOG2E);
     us += ro;
-    const float ius = 1.f / us, pr = taught ? ro * ius : 0.f, lus = logf(us);
+    const float ius = 1.f / us, pr = taught ? ro * ius : 0.f;
     const float xo = finite_or_0(xm);
     float xs = 0.f, xh = 0.f, m = -INFINITY;
     if (live) {
@@ -258,76 +274,85 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
     s = row_sum<LPR>(s);
     if (HARD) h = row_sum<LPR>(h);
     const RowStats st = row_stats(a, w, m, s, h, xm, xs, xh, taught, pr);
-    const float lsa = logf(st.sa);
-    // the row's loss
+    auto teacher_p = [&](int j) {
+        return __builtin_amdgcn_exp2f((u[j] * a.inv_t - uo) * LOG2E) * ius;
+    };
+    // gradients: the others', the listed ones', the target's
+    if (a.dlogits) {
+        if (live) {
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int at = regs.at(g, sub) + j;
+                    float q = e[g * 8 + j] * st.cq;
+                    if (HARD) q += eh[g * 8 + j] * st.ch;
+                    if (at < V) tile[at] = q;
+                }
+        }
+        __syncthreads();
+        if (live) {
+            const float cs = taught ? a.dsoft * w : 0.f;
+            const float ca = cs / st.sa, ch = HARD ? a.hard * w / st.ha : 0.f;
+            for (int j = sub; j < k; j += LPR)
+                if (li[j] >= 0) {
+                    float q = ca * exp_below(lx[j], st.ma, a.scale);
+                    if (HARD) q += ch * exp_below(lx[j], st.ma, LOG2E);
+                    if (!twice && taught) q -= cs * teacher_p(j);
+                    tile[li[j]] = q;
+                }
+        }
+        __syncthreads();
+        if (live && sub == 0) {
+            if (twice && taught)
+                for (int j = 0; j < k; ++j) {
+                    const int idx = li[j] >= -1 ? li[j] : -2 - li[j];
+                    if (idx >= 0) tile[idx] -= a.dsoft * w * teacher_p(j);
+                }
+            if (HARD) tile[tg] -= a.hard * w;
+        }
+        __syncthreads();
+        if (inside) {
+            T *dl = (T *)a.dlogits + row * V;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int at = regs.at(g, sub);
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    v[j] = live && at + j < V ? tile[at + j] : 0.f;
+                if (at + 8 <= V) Row8<DT>::store(dl + at, v);
+                else {
+#pragma unroll
+                    for (int j = 0; j < 7; ++j)
+                        if (at + j < V) dl[at + j] = R::down(v[j]);
+                }
+            }
+        }
+    }
+    // the row's loss, when the registers are free again
     float loss = 0.f;
     if (live && taught) {
-        for (int j = sub; j < k; j += LPR) {
-            const float p = __builtin_amdgcn_exp2f((u[j] - uo) * LOG2E) * ius;
-            if (!(p == 0.f))
-                loss += p * ((u[j] - uo - lus) -
-                             ((lx[j] - st.ma) * a.inv_t - lsa));
-            u[j] = p;
+        const double c = (double)uo + logf(us / st.sa);
+        // (entry k: any other token)
+        for (int j = sub; j <= k; j += LPR) {
+            const bool other = j == k;
+            const int idx = other ? 0 : li[j];
+            const float p = other ? pr : teacher_p(j), at = other ? mo : lx[j];
+            const double d = ((double)at - st.ma) * a.inv_t64 + c -
+                             (other ? rest - log((double)s)
+                                    : (double)u[j] * a.inv_t64);
+            const float q =
+                exp_below(at, st.ma, a.scale) * (other ? s : 1.f) / st.sa;
+            if (idx != -1 || p != p) loss += kl_term(p, d, q);
+            if (idx < -1) loss -= q;
         }
-        if (sub == 0 && !(pr == 0.f))
-            loss += pr * ((rest - uo - lus) - st.other);
         loss *= a.soft;
     }
     if (HARD && live && sub == 0)
         loss += a.hard * (logf(st.ha) - (xt - st.ma));
     loss = wave_sum(live ? loss * w : 0.f);
     if (lane == 0) a.rowloss[blockIdx.x] = loss;
-    if (!a.dlogits) return;
-    // gradients: the others', the listed ones', the target's
-    if (live) {
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int at = regs.at(g, sub) + j;
-                float q = e[g * 8 + j] * st.cq;
-                if (HARD) q += eh[g * 8 + j] * st.ch;
-                if (at < V) tile[at] = q;
-            }
-    }
-    __syncthreads();
-    if (live) {
-        const float cs = taught ? a.dsoft * w : 0.f;
-        const float ca = cs / st.sa, ch = HARD ? a.hard * w / st.ha : 0.f;
-        for (int j = sub; j < k; j += LPR)
-            if (li[j] >= 0) {
-                float q = ca * exp_below(lx[j], st.ma, a.scale);
-                if (HARD) q += ch * exp_below(lx[j], st.ma, LOG2E);
-                if (!twice && taught) q -= cs * u[j];
-                tile[li[j]] = q;
-            }
-    }
-    __syncthreads();
-    if (live && sub == 0) {
-        if (twice && taught)
-            for (int j = 0; j < k; ++j) {
-                const int idx = li[j] >= -1 ? li[j] : -2 - li[j];
-                if (idx >= 0) tile[idx] -= a.dsoft * w * u[j];
-            }
-        if (HARD) tile[tg] -= a.hard * w;
-    }
-    __syncthreads();
-    if (!inside) return;
-    T *dl = (T *)a.dlogits + row * V;
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-        const int e = regs.at(g, sub);
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[j] = live && e + j < V ? tile[e + j] : 0.f;
-        if (e + 8 <= V) Row8<DT>::store(dl + e, v);
-        else {
-#pragma unroll
-            for (int j = 0; j < 7; ++j)
-                if (e + j < V) dl[e + j] = R::down(v[j]);
-        }
-    }
 }
 
 // ---- longer rows ----------------------------------------------------------------
@@ -336,9 +361,9 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
 // listed tokens are marked in a bitmap in LDS -- a group of eight elements is one
 // byte of it -- and become -inf in the registers, so the passes see the others
 // only.  What bounds it is memory, as long as two blocks fit a CU and one loads
-// while the other computes: 2048 x 32000 bf16 in 56 us (4.7 TB/s, what a large
-// copy reaches), 1024 ragged x 50021 fp32 with targets in 87 us (3.6 TB/s: at most
-// four rows per CU, so two turns of loads with little to hide behind); 7 x 601 fp16 in 4.6 us (latency).
+// while the other computes: 2048 x 32000 bf16 in 59 us (4.5 TB/s; a large copy
+// reaches 4.7), 1024 ragged x 50021 fp32 with targets in 87 us (3.6 TB/s: at most
+// four rows per CU, so two turns of loads with little to hide behind); 7 x 601 fp16 in 5.0 us (latency).
 // LG: up to so many more groups of a thread are kept in LDS, in the threads' order
 // (each thread reads what it wrote: no barrier).
 template <int DT, int NT, int G, bool HARD, bool KEEP, int LG = 0>
@@ -349,10 +374,10 @@ distill_row_kernel(DistillArgs a) {
     typedef typename R::T T;
     extern __shared__ __align__(16) unsigned marks[];   // a bit per element
     __shared__ float red[NT / 64], red2[NT / 64];
-    __shared__ float s_list[6];
+    __shared__ float s_list[9];
     // what wave 0 needs of its list after the passes (registers are the row's)
     __shared__ int w_idx[64];
-    __shared__ float w_x[64], w_p[64], w_logp[64], w_mass[64];
+    __shared__ float w_x[64], w_p[64], w_value[64], w_mass[64];
     const int tid = threadIdx.x, lane = tid & 63;
     const long long row = blockIdx.x;
     const int V = a.V, k = a.k;
@@ -397,7 +422,7 @@ distill_row_kernel(DistillArgs a) {
         });
     // the list: lane j of wave 0 holds entry j
     int idx = -1, tg = -1;
-    float u = -INFINITY, lx = -INFINITY, xt = 0.f, rest = -INFINITY;
+    float value = -INFINITY, lx = -INFINITY, xt = 0.f, rest = -INFINITY;
     if (tid < 64) {
         if (a.rest) rest = a.rest[row];
         if (HARD) {
@@ -407,7 +432,7 @@ distill_row_kernel(DistillArgs a) {
         if (lane < k) {
             idx = teacher_index(a, row * k + lane);
             if (idx >= 0) {
-                u = teacher_value(a, row * k + lane) * a.inv_t;
+                value = teacher_value(a, row * k + lane);
                 lx = R::up(x[idx]);
             }
         }
@@ -485,13 +510,13 @@ distill_row_kernel(DistillArgs a) {
             }
             first = idx >= 0 && !again;
         }
-        const float um = wave_max(fmaxf(u, rest));
+        const float u = value * a.inv_t, um = wave_max(fmaxf(u, rest));
         const bool bad = __any(u != u || rest != rest);
         const bool taught = a.soft > 0.f && (um > -INFINITY || bad);
         const float uo = finite_or_0(um);
         const float e = __builtin_amdgcn_exp2f((u - uo) * LOG2E);
         const float ro = __builtin_amdgcn_exp2f((rest - uo) * LOG2E);
-        const float us = wave_sum(e) + ro, lus = logf(us);
+        const float us = wave_sum(e) + ro;
         if (taught) p = e / us;
         mass = p;
         if (__any(idx >= 0 && !first)) {
@@ -508,13 +533,16 @@ distill_row_kernel(DistillArgs a) {
         const float xs = wave_sum(first ? exp_below(lx, xo, a.scale) : 0.f);
         const float xh =
             HARD ? wave_sum(first ? exp_below(lx, xo, LOG2E) : 0.f) : 0.f;
-        w_idx[lane] = first ? idx : -1;   // (an entry that is not the first of its
-        w_x[lane] = lx;                   // index has a loss, but no gradient)
+        w_idx[lane] = first ? idx : idx >= 0 ? -2 : -1;   // (an entry that is not
+        w_x[lane] = lx;           // the first of its index: a loss, no gradient)
         w_p[lane] = p;
-        w_logp[lane] = u - uo - lus;
+        w_value[lane] = value;
         w_mass[lane] = mass;
         if (lane == 0) {
-            s_list[5] = rest - uo - lus;
+            s_list[5] = us;
+            s_list[6] = uo;
+            s_list[7] = rest;
+            s_list[8] = xt;
             s_list[0] = xm;
             s_list[1] = xs;
             s_list[2] = xh;
@@ -564,17 +592,33 @@ distill_row_kernel(DistillArgs a) {
     st.ha = uniform(st.ha);
     st.cq = uniform(st.cq);
     st.ch = uniform(st.ch);
-    if (tid < 64) {
-        const float lsa = logf(st.sa), p = w_p[lane];
-        float kl = 0.f;
-        if (!(p == 0.f))
-            kl = p * (w_logp[lane] - ((w_x[lane] - st.ma) * a.inv_t - lsa));
-        if (lane == 0 && !(pr == 0.f)) kl += pr * (s_list[5] - st.other);
-        float loss = a.soft * wave_sum(kl);
-        if (HARD) loss += a.hard * (logf(st.ha) - (xt - st.ma));
+    // The last wave does this after its stores (the first has the list to write): it
+    // takes no registers from the row, and less than what the stores take to arrive.
+    auto row_loss = [&] {
+        float loss = 0.f;
+        if (taught) {
+            const float us = s_list[5], uo = s_list[6], rest = s_list[7];
+            const double c = (double)uo + logf(us / st.sa);
+            const float p = w_p[lane], at = w_x[lane];
+            const float q = exp_below(at, st.ma, a.scale) / st.sa;
+            const int li = w_idx[lane];
+            if (li != -1 || p != p)
+                loss = kl_term(p, ((double)at - st.ma) * a.inv_t64 + c -
+                                      (double)w_value[lane] * a.inv_t64, q);
+            if (li < -1) loss -= q;
+            if (lane == 0)
+                loss += kl_term(pr, ((double)mo - st.ma) * a.inv_t64 + c -
+                                        (rest - log((double)s)),
+                                exp_below(mo, st.ma, a.scale) * s / st.sa);
+            loss = a.soft * wave_sum(loss);
+        }
+        if (HARD) loss += a.hard * (logf(st.ha) - (s_list[8] - st.ma));
         if (lane == 0) a.rowloss[row] = loss * w;
+    };
+    if (!dl) {
+        if (tid >= NT - 64) row_loss();
+        return;
     }
-    if (!dl) return;
     auto write = [&](int g, const Row8<DT> &q) {
         const int e = (g * NT + tid) * 8;
         if (e >= V) return;
@@ -611,6 +655,7 @@ distill_row_kernel(DistillArgs a) {
             write(g, q);
         });
     }
+    if (tid >= NT - 64) row_loss();
     __syncthreads();   // the listed tokens and the target over what is there
     if (tid < 64) {
         const int li = w_idx[lane];
@@ -778,7 +823,8 @@ int pcm_distill_loss(const void *logits, int32_t dtype, int64_t ld,
     a.values_dtype = values_dtype;
     a.weight = step_weight;
     a.weight_all = 1.0f / (float)batch;
-    a.inv_t = (float)(1.0 / temperature);
+    a.inv_t64 = 1.0 / temperature;
+    a.inv_t = (float)a.inv_t64;
     a.scale = (float)(1.4426950408889634 / temperature);
     a.soft = (float)((1.0 - hard_weight) * temperature * temperature);
     a.dsoft = (float)((1.0 - hard_weight) * temperature);

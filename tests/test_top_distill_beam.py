@@ -687,6 +687,44 @@ def test_distill_on_targets_alone(V):
 
 
 @gpu
+@pytest.mark.parametrize('tau', [1.0, 3.0])
+@pytest.mark.parametrize('V', [60, 300, 700, 5003, 40000, 70000])
+def test_distill_of_a_student_near_its_teacher(V, tau):
+    """A KL of 1e-7, where log p and log q agree in most of their digits."""
+    import paccmann_chemistry_amd as P
+    g = _gen(V, 5)
+    T, B, k = 2, 3, 9
+    said = torch.randn(T, B, V, generator=g) * 3
+    logits = said + 1e-3 * torch.randn(T, B, V, generator=g)
+    values, places = torch.topk(said, k, -1)
+    others = said.double().scatter(-1, places, -math.inf)
+    rest = torch.logsumexp(others / tau, -1).float()
+    # the definition, in 64 bits
+    u = torch.cat([values.double() / tau, rest.double()[..., None]], -1)
+    logp = torch.log_softmax(u, -1)
+    x = logits.double() / tau
+    z = torch.logsumexp(x, -1, keepdim=True)
+    left = torch.logsumexp(x.scatter(-1, places, -math.inf), -1, keepdim=True)
+    logq = torch.cat([x.gather(-1, places) - z, left - z], -1)
+    p, q = logp.exp(), logq.exp()
+    kl = (p * (logp - logq)).sum(-1)
+    # Sums of exponentials in 32 bits: the exponent's product and the factor in it
+    # are rounded (|x - max| / tau half steps each), the exponential to a step, and
+    # no element passes more than 90 additions.  What that moves d = log q - log p
+    # by is met by q - p, and by itself; p and the sum of the terms are rounded.
+    far = float((x.amax(-1) - x.amin(-1)).max())
+    eps = (2 * far + 92) * EPS / 2
+    room = 4 * eps * ((q - p).abs().sum(-1) + kl) + 4 * eps ** 2 + 1e-14
+    want, tol = (tau * tau * t.sum() / B for t in (kl, room))
+    assert float(tol) < 0.5 * float(want)
+    dev = _dev()
+    loss = P.distill_loss(
+        logits.to(dev),
+        P.TopLogits(values.to(dev), places.int().to(dev), rest.to(dev), tau))
+    assert abs(float(loss) - float(want)) <= float(tol)
+
+
+@gpu
 def test_distill_gradient_by_differences_and_scale():
     """The kernel's gradient against differences of the kernel's own loss, and
     an incoming gradient that is not one."""
