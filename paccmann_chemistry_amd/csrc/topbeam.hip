@@ -451,10 +451,11 @@ __global__ __launch_bounds__(256) void top_short_kernel(TopArgs a, long long row
 // maximum; a wave takes the sums of the threads that hold listed elements again,
 // without those.  (The whole row's sum minus the listed ones' would lose what
 // the others are when the list holds nearly all of it.)
-// Top 32 of 1024 x 50021 bf16: 34 us (102.6 MB, 3.0 TB/s), of which an exponential
-// and a maximum per element take about as long as the loads, which they hide only
-// in part, and the selection 6 us at the end of each block; k passes took 8.4 ms.  Top 64 of three rows of 131071 fp16: 8.6 us in 31 blocks a
-// row, and 5.0 to join them: latency.
+// Top 32 of 1024 x 50021 bf16: 34 us (102.6 MB, 3.0 TB/s): 22 at the rate of a large
+// copy, then the selection, a chain of sorts and reads that all 1024 blocks are in
+// at once, being resident together (a sixth fewer instructions in it changed
+// nothing); k passes took 8.4 ms.  Top 64 of three rows of 131071 fp16: 8.6 us in 31
+// blocks a row, and 5.0 to join them: latency.
 template <int DT, int NT, bool ONE>
 __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
     typedef RowType<DT> R;
