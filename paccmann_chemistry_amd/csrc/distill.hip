@@ -17,8 +17,8 @@
 //   sum p (log p - log q) = sum p (e^d - 1 - d),
 // terms that are not negative, in which an error of a normaliser, common to all d,
 // is multiplied by sum (q - p) = 0.  d and e^d - 1 - d are taken in 64 bits, for the
-// k + 1 outcomes only; the normalisers' logarithm in 32.  (An outcome without p adds its q; an index that appears
-// twice has its q once.)
+// k + 1 outcomes only; the normalisers' logarithm in 32.  (An outcome without p adds
+// its q; an index that appears twice has its q once.)
 #include "rows.h"
 
 namespace {
@@ -363,7 +363,8 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
 // only.  What bounds it is memory, as long as two blocks fit a CU and one loads
 // while the other computes: 2048 x 32000 bf16 in 59 us (4.5 TB/s; a large copy
 // reaches 4.7), 1024 ragged x 50021 fp32 with targets in 87 us (3.6 TB/s: at most
-// four rows per CU, so two turns of loads with little to hide behind); 7 x 601 fp16 in 5.0 us (latency).
+// four rows per CU, so two turns of loads with little to hide behind); 7 x 601 fp16
+// in 5.0 us (latency).
 // LG: up to so many more groups of a thread are kept in LDS, in the threads' order
 // (each thread reads what it wrote: no barrier).
 template <int DT, int NT, int G, bool HARD, bool KEEP, int LG = 0>
