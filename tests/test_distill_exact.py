@@ -1,0 +1,213 @@
+"""The distillation loss and its gradient against the definition in 64 bits, with
+room for what the roundings of one element amount to and no more: a group of
+eight that is missing or doubled fails, whatever the length of the row.
+
+EPS is half a step of fp32 (2^-24).  With D = (maximum - x) / tau, the exponent
+of an element is a difference, a factor and a product (3 EPS D), taken once more
+between the maximum of the others and the row's (EPS D), the exponential is good
+to a step (2 EPS); sums pass an element through ``_additions`` roundings.  All of
+it is relative to the terms that make an element of the gradient, q and p; the
+types' own rounding follows once.
+"""
+import math
+
+import pytest
+import torch
+
+from test_top_distill_beam import DTYPES, EPS, HALF, _dev, _gen, _logits
+from test_top_distill_beam import _weights, gpu, ref_distill
+
+
+def _additions(vocab):
+    """Roundings between an element and the sum over its row: the additions of a
+    thread (the rows that are read twice: and the rescalings, a few per group),
+    of the lanes, of the waves, of the two parts."""
+    groups = max(4, -(-vocab // 8192))
+    return 8 * groups + 5 * groups + 6 + 16 + 2
+
+
+def _share(x, mask=None):
+    """(softmax along the last axis, log of the sum), 0 and -inf where nothing
+    is above -inf."""
+    if mask is not None:
+        x = torch.where(mask, x, -math.inf)
+    lse = torch.logsumexp(x, -1, keepdim=True)
+    gone = lse == -math.inf
+    return torch.where(gone, 0.0, (x - torch.where(gone, 0.0, lse)).exp()), lse
+
+
+class Exact:
+    """loss, grad: the definition (no index twice); loss_tol, grad_tol: see
+    above, before the rounding to the gradient's own type."""
+
+    def __init__(self, logits, values, indices, rest, tau, targets=None,
+                 lengths=None, hard=0.0):
+        steps, batch, vocab = logits.shape
+        w = _weights(steps, batch, lengths, None)
+        x = torch.where((w > 0)[..., None], logits.double(), 0.0)
+        there = (indices >= 0) & (indices < vocab)
+        at = torch.where(there, indices, 0).long()
+        held = torch.zeros(x.shape).scatter_add_(-1, at, there.float()) > 0
+        q, z = _share(x / tau)
+        others, zo = _share(x / tau, ~held)
+        u = torch.where(there, values.double() / tau, -math.inf)
+        last = torch.full(w.shape, -math.inf, dtype=torch.float64) \
+            if rest is None else rest.double()
+        u = torch.cat([u, last[..., None]], -1)
+        p, n = _share(u)
+        logq = torch.cat([(x / tau).gather(-1, at) - z, zo - z], -1)
+        terms = torch.where(p > 0, p * (u - n - logq), 0.0)
+        kl = terms.sum(-1)
+        teacher = torch.zeros_like(x).scatter_add_(
+            -1, at, torch.where(there, p[..., :-1], 0.0))
+        teacher = torch.where(held, teacher, p[..., -1:] * others)
+        soft = (1 - hard) * tau
+        row = soft * tau * kl
+        grad = soft * (q - teacher)
+        # roundings, relative
+        high = x.amax(-1, keepdim=True)
+        far = torch.where(x == -math.inf, 0.0, (high - x) / tau)
+        adds = _additions(vocab)
+        sums = EPS * (adds + 4 + 4 * (q * far).sum(-1, keepdim=True) +
+                      4 * (others * far).sum(-1, keepdim=True))
+        live = torch.where(torch.isfinite(u), u, 0.0).abs().amax(-1)
+        said = EPS * (2 * (live + last.nan_to_num(0, 0, 0).abs()) + 4 * live +
+                      64 + 16)[..., None]
+        own = EPS * (4 * far + 8)
+        self.grad_tol = soft * ((own + sums) * q +
+                                (own + sums + said) * teacher)
+        # What moves every d = log q - log p by the same is met by sum (q - p) = 0
+        # but for the roundings; the rest is relative to the terms, which are not
+        # negative
+        outcomes = torch.cat([q.gather(-1, at) * there,
+                              (zo - z).exp()], -1)
+        eps = (sums + said)[..., 0] + EPS * 8
+        apart = (outcomes - p).abs().sum(-1)
+        kl_tol = 2 * eps * (apart + kl.abs().nan_to_num(0, 0, 0)) + 2 * eps ** 2
+        self.loss_tol = soft * tau * kl_tol
+        if hard:
+            tg = targets.clamp(0, vocab - 1)[..., None]
+            s, zh = _share(x)
+            ce = (zh - x.gather(-1, tg))[..., 0]
+            row = row + hard * ce
+            one = torch.zeros_like(x).scatter_(-1, tg, 1.0)
+            grad = grad + hard * (s - one)
+            sums = EPS * (adds + 4 + 8 * (s * far * tau).sum(-1, keepdim=True))
+            self.grad_tol = self.grad_tol + hard * (
+                (EPS * (4 * far * tau + 8) + sums) * s + 4 * EPS * one)
+            self.loss_tol = self.loss_tol + hard * (
+                sums[..., 0] + 4 * EPS * (1 + ce.abs()))
+        self.loss = (w * torch.where(w > 0, row, 0.0)).sum()
+        self.grad = w[..., None] * grad
+        self.grad_tol = w[..., None] * self.grad_tol
+        self.loss_tol = float((w * self.loss_tol).sum() +
+                              2 * EPS * abs(self.loss))
+
+    def check(self, loss, grad, factor=1.0):
+        if loss is not None:
+            assert abs(float(loss) - float(self.loss)) <= self.loss_tol
+        assert bool(self.fine(grad, factor).all())
+
+    def fine(self, grad, factor=1.0):
+        """Which elements of a gradient, times ``factor``, are right."""
+        dtype = grad.dtype
+        want, tol = self.grad * factor, self.grad_tol * abs(factor)
+        tol = tol + 2 * EPS * want.abs()
+        # (results of an exponential below 2^-126 are 0)
+        tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+        tol = tol + HALF[dtype] * (want.abs() + tol) + tiny + 2.0 ** -125
+        return (grad.double() - want).abs() <= tol
+
+
+def _case(T, B, V, k, dtype, kind, rest, g, tau=2.0, absent=True):
+    logits = _logits((T, B, V), kind, dtype, g)
+    teacher = logits.float().clamp(-1e4, 1e4) * 0.7 \
+        + torch.randn(T, B, V, generator=g)
+    values, indices = torch.topk(teacher, k, dim=-1)
+    others = teacher.scatter(-1, indices, -math.inf)
+    rest_t = torch.logsumexp(others / tau, -1).float() if rest else None
+    indices = indices.int()
+    if absent and k > 1:
+        keep = torch.randint(1, k + 1, (T, B, 1), generator=g)
+        indices = torch.where(torch.arange(k) < keep, indices, -1).int()
+    return logits, values.to(dtype), indices, rest_t
+
+
+def _teacher(values, indices, rest, tau):
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    return P.TopLogits(values.to(dev), indices.to(dev),
+                       None if rest is None else rest.to(dev), tau)
+
+
+SHAPES = [
+    (3, 5, 60, 8, 'normal', True, 0.5), (2, 3, 64, 64, 'ties', False, 0.0),
+    (2, 3, 129, 5, 'normal', True, 0.25), (2, 2, 601, 64, 'far', True, 0.25),
+    (1, 3, 2050, 17, 'normal', True, 0.0), (2, 2, 5003, 33, 'normal', True, .5),
+    (1, 2, 9001, 9, 'masked', True, 0.0), (1, 2, 33001, 64, 'normal', True, .25),
+    (1, 2, 32769, 3, 'far', True, 0.5), (1, 2, 50021, 64, 'normal', True, 0.25),
+    (1, 2, 50945, 8, 'normal', False, 0.0), (1, 2, 65537, 9, 'normal', True, .5),
+    (1, 1, 140001, 9, 'normal', True, 0.5),
+]
+
+
+def _inputs(shape, dtype):
+    T, B, V, k, kind, rest, hard = shape
+    g = _gen(T, B, V, k, 31)
+    case = _case(T, B, V, k, dtype, kind, rest, g)
+    targets = torch.randint(0, V, (T, B), generator=g)
+    return case, targets
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('shape', SHAPES)
+def test_the_check_sees_a_group_of_eight(shape, dtype):
+    """The exact gradient, rounded, passes; with eight neighbours that are no
+    listed tokens 0, doubled or of the next row it does not."""
+    (logits, values, indices, rest), targets = _inputs(shape, dtype)
+    exact = Exact(logits, values, indices, rest, 2.0, targets, None, shape[-1])
+    good = exact.grad.to(dtype)
+    assert bool(exact.fine(good).all())
+    V = shape[2]
+    seen = 0
+    for start in range(0, V - 7, max(8, V // 64 // 8 * 8)):
+        group = slice(start, start + 8)
+        # 16 bits cannot tell what is below their smallest step from 0
+        step = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        if float(good[0, 0, group].abs().max()) < 4 * step:
+            continue
+        seen += 1
+        for factor in (0, 2):
+            bad = good.clone()
+            bad[0, 0, group] *= factor
+            assert not bool(exact.fine(bad).all()), (start, factor)
+    assert seen or shape[4] == 'far'
+
+
+def test_two_ways_to_the_definition():
+    """The closed form above against autograd through the definition."""
+    g = _gen(3, 4)
+    logits, values, indices, rest = _case(2, 3, 40, 6, torch.float32, 'normal',
+                                          True, g)
+    targets = torch.randint(0, 40, (2, 3), generator=g)
+    lengths = torch.tensor([2, 1, 2])
+    exact = Exact(logits, values, indices, rest, 2.0, targets, lengths, 0.3)
+    loss, grad = ref_distill(logits, values, indices, rest, 2.0, targets,
+                             lengths, 0.3)
+    assert abs(loss - exact.loss) < 1e-13
+    assert bool(((grad - exact.grad).abs() < 1e-14).all())
+
+
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('shape', SHAPES)
+def test_distill_element_by_element(shape, dtype):
+    import paccmann_chemistry_amd as P
+    (logits, values, indices, rest), targets = _inputs(shape, dtype)
+    hard = shape[-1]
+    exact = Exact(logits, values, indices, rest, 2.0, targets, None, hard)
+    x = logits.to(_dev()).requires_grad_(True)
+    loss = P.distill_loss(x, _teacher(values, indices, rest, 2.0),
+                          targets=targets.to(_dev()), hard_weight=hard)
+    grad, = torch.autograd.grad(loss, x)
+    exact.check(loss.detach(), grad.cpu())
