@@ -104,6 +104,13 @@ __device__ __forceinline__ float kl_term(float p, double d, float q) {
     return p == 0.f ? q : (float)((double)q - (double)p * (1. + d));
 }
 
+// probability of the outcome "any other token".  (Where none is left mo is not a
+// maximum, and 0 times a power of it need not be 0.)
+__device__ __forceinline__ float other_q(float mo, float s, float ma, float sa,
+                                         float scale) {
+    return s == 0.f ? 0.f : exp_below(mo, ma, scale) * s / sa;
+}
+
 // What a row's factors are made of: the others' maximum m and sum(s), the listed
 // tokens' xm and sums, the teacher's.  (Sums relative to exp(max).)
 struct RowStats {
@@ -342,8 +349,8 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
             const double d = ((double)at - st.ma) * a.inv_t64 + c -
                              (other ? rest - log((double)s)
                                     : (double)u[j] * a.inv_t64);
-            const float q =
-                exp_below(at, st.ma, a.scale) * (other ? s : 1.f) / st.sa;
+            const float q = other ? other_q(mo, s, st.ma, st.sa, a.scale)
+                                  : exp_below(at, st.ma, a.scale) / st.sa;
             if (idx != -1 || p != p) loss += kl_term(p, d, q);
             if (idx < -1) loss -= q;
         }
@@ -610,7 +617,7 @@ distill_row_kernel(DistillArgs a) {
             if (lane == 0)
                 loss += kl_term(pr, ((double)mo - st.ma) * a.inv_t64 + c -
                                         (rest - log((double)s)),
-                                exp_below(mo, st.ma, a.scale) * s / st.sa);
+                                other_q(mo, s, st.ma, st.sa, a.scale));
             loss = a.soft * wave_sum(loss);
         }
         if (HARD) loss += a.hard * (logf(st.ha) - (s_list[8] - st.ma));
