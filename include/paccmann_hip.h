@@ -462,7 +462,8 @@ int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
  *            pcm_softmax_ce's); with hard_weight 1 the teacher is not looked at
  *   loss     fp32[1]; dlogits (nullable) [T*B][vocab] of `dtype`, dense: zero in
  *            rows that take no part, whatever their logits hold
- *   scratch  fp32[pcm_distill_scratch_floats(T, B)]
+ *   scratch  fp32[pcm_distill_scratch_floats(T, B)]; a weight that is made of
+ *            the lengths is left at scratch[T * B + t] for pcm_distill_grad
  */
 size_t pcm_distill_scratch_floats(int32_t steps, int32_t batch);
 int pcm_distill_loss(const void *logits, int32_t dtype, int64_t ld,
@@ -473,6 +474,20 @@ int pcm_distill_loss(const void *logits, int32_t dtype, int64_t ld,
                      int32_t vocab, double temperature, double hard_weight,
                      float *loss, void *dlogits, float *scratch,
                      int32_t *status, void *stream);
+/*
+ * The gradient of pcm_distill_loss times factor[0] (a device scalar: what comes
+ * in from behind the loss), rounded once.  For fp16, where a gradient that is
+ * rounded before a loss scale is applied has lost what the scale is to keep:
+ * leave pcm_distill_loss's dlogits NULL and call this in the backward pass.
+ */
+int pcm_distill_grad(const void *logits, int32_t dtype, int64_t ld,
+                     const void *values, int32_t values_dtype,
+                     const int32_t *indices, const float *rest, int32_t k,
+                     const int64_t *targets, const int32_t *lengths,
+                     const float *step_weight, int32_t steps, int32_t batch,
+                     int32_t vocab, double temperature, double hard_weight,
+                     const float *factor, void *dlogits, float *scratch,
+                     void *stream);
 /* x[i] *= scale[0] (a device scalar); leaves x alone when it is 1. */
 int pcm_scale(void *x, int32_t dtype, int64_t n, const float *scale,
               void *stream);

@@ -171,6 +171,12 @@ PROTOTYPES = {
             _I32, _I32, _F64, _F64, _VP, _VP, _VP, _VP, _VP
         ]
     ),
+    'pcm_distill_grad': (
+        ctypes.c_int, [
+            _VP, _I32, _I64, _VP, _I32, _VP, _VP, _I32, _VP, _VP, _VP, _I32,
+            _I32, _I32, _F64, _F64, _VP, _VP, _VP, _VP
+        ]
+    ),
     'pcm_scale': (ctypes.c_int, [_VP, _I32, _I64, _VP, _VP]),
     'pcm_beam_select_workspace_bytes': (_SZ, [_I32, _I32, _I32, _I32]),
     'pcm_beam_select': (

@@ -30,7 +30,8 @@ struct DistillArgs {
     const int64_t *targets;
     const int32_t *lengths;
     const float *weight;   // [T], or null: weight_all
-    float *rowloss;        // one sum per block
+    const float *factor;   // of the gradient, on the device, or null: 1
+    float *rowloss;        // one sum per block, or null: the gradient only
     void *dlogits;
     int32_t *status;
     long long ld, rows;
@@ -60,6 +61,10 @@ __device__ __forceinline__ float row_weight(const DistillArgs &a, long long row)
     const int len = a.lengths ? a.lengths[row - (long long)t * a.B] : t + 1;
     const float w = a.weight ? a.weight[t] : a.weight_all;
     return t < len ? w : 0.f;
+}
+// weight of the row's gradient
+__device__ __forceinline__ float grad_weight(const DistillArgs &a, float w) {
+    return a.factor ? w * a.factor[0] : w;
 }
 __device__ __forceinline__ float teacher_value(const DistillArgs &a,
                                                long long at) {
@@ -112,7 +117,8 @@ __device__ __forceinline__ float other_q(float mo, float s, float ma, float sa,
 }
 
 // What a row's factors are made of: the others' maximum m and sum(s), the listed
-// tokens' xm and sums, the teacher's.  (Sums relative to exp(max).)
+// tokens' xm and sums, the teacher's; w: the weight of its gradient.  (Sums relative
+// to exp(max).)
 struct RowStats {
     float ma;        // maximum of the row
     float sa, ha;    // sums over the row relative to it: / tau, plain
@@ -172,6 +178,7 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
     const bool inside = row < a.rows;
     const float w = inside ? row_weight(a, row) : 0.f;
     const bool live = w != 0.f;
+    const float wg = grad_weight(a, w);
     const T *x = (const T *)a.logits + row * a.ld;
     RowRegs<DT, LPR, G> regs;
     float rest = -INFINITY;
@@ -280,7 +287,7 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
     }
     s = row_sum<LPR>(s);
     if (HARD) h = row_sum<LPR>(h);
-    const RowStats st = row_stats(a, w, m, s, h, xm, xs, xh, taught, pr);
+    const RowStats st = row_stats(a, wg, m, s, h, xm, xs, xh, taught, pr);
     auto teacher_p = [&](int j) {
         return __builtin_amdgcn_exp2f((u[j] * a.inv_t - uo) * LOG2E) * ius;
     };
@@ -299,8 +306,8 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
         }
         __syncthreads();
         if (live) {
-            const float cs = taught ? a.dsoft * w : 0.f;
-            const float ca = cs / st.sa, ch = HARD ? a.hard * w / st.ha : 0.f;
+            const float cs = taught ? a.dsoft * wg : 0.f;
+            const float ca = cs / st.sa, ch = HARD ? a.hard * wg / st.ha : 0.f;
             for (int j = sub; j < k; j += LPR)
                 if (li[j] >= 0) {
                     float q = ca * exp_below(lx[j], st.ma, a.scale);
@@ -314,9 +321,9 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
             if (twice && taught)
                 for (int j = 0; j < k; ++j) {
                     const int idx = li[j] >= -1 ? li[j] : -2 - li[j];
-                    if (idx >= 0) tile[idx] -= a.dsoft * w * teacher_p(j);
+                    if (idx >= 0) tile[idx] -= a.dsoft * wg * teacher_p(j);
                 }
-            if (HARD) tile[tg] -= a.hard * w;
+            if (HARD) tile[tg] -= a.hard * wg;
         }
         __syncthreads();
         if (inside) {
@@ -338,6 +345,7 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
         }
     }
     // the row's loss, when the registers are free again
+    if (!a.rowloss) return;
     float loss = 0.f;
     if (live && taught) {
         const double c = (double)uo + logf(us / st.sa);
@@ -393,7 +401,7 @@ distill_row_kernel(DistillArgs a) {
     T *dl = a.dlogits ? (T *)a.dlogits + row * V : nullptr;
     const int groups = KEEP ? G + LG : (V + NT * 8 - 1) / (NT * 8);
     if (w == 0.f) {
-        if (tid == 0) a.rowloss[row] = 0.f;
+        if (tid == 0 && a.rowloss) a.rowloss[row] = 0.f;
         if (dl)
             for (int g = 0; g < groups; ++g) {
                 const int e = (g * NT + tid) * 8;
@@ -593,7 +601,8 @@ distill_row_kernel(DistillArgs a) {
     __syncthreads();   // s_list
     const bool taught = s_list[3] != 0.f;
     const float pr = s_list[4];
-    RowStats st = row_stats(a, w, m, s, h, s_list[0], s_list[1], s_list[2], taught,
+    const float wg = uniform(grad_weight(a, w));
+    RowStats st = row_stats(a, wg, m, s, h, s_list[0], s_list[1], s_list[2], taught,
                             pr);
     st.ma = uniform(st.ma);
     st.sa = uniform(st.sa);
@@ -603,6 +612,7 @@ distill_row_kernel(DistillArgs a) {
     // The last wave does this after its stores (the first has the list to write): it
     // takes no registers from the row, and less than what the stores take to arrive.
     auto row_loss = [&] {
+        if (!a.rowloss) return;
         float loss = 0.f;
         if (taught) {
             const float us = s_list[5], uo = s_list[6], rest = s_list[7];
@@ -671,11 +681,11 @@ distill_row_kernel(DistillArgs a) {
             const float lv = w_x[lane];
             float g = 0.f;
             if (s_list[3] != 0.f)
-                g = a.dsoft * w *
+                g = a.dsoft * wg *
                     (exp_below(lv, st.ma, a.scale) / st.sa - w_mass[lane]);
             if (HARD) {
-                g += a.hard * w * exp_below(lv, st.ma, LOG2E) / st.ha;
-                if (li == tg) g -= a.hard * w;
+                g += a.hard * wg * exp_below(lv, st.ma, LOG2E) / st.ha;
+                if (li == tg) g -= a.hard * wg;
             }
             dl[li] = R::down(g);
         }
@@ -683,7 +693,7 @@ distill_row_kernel(DistillArgs a) {
             const float d = xt - mo;
             dl[tg] = R::down(__builtin_amdgcn_exp2f(d * a.scale) * st.cq +
                              __builtin_amdgcn_exp2f(d * LOG2E) * st.ch -
-                             a.hard * w);
+                             a.hard * wg);
         }
     }
 }
@@ -705,8 +715,11 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float *x,
     }
 }
 
-// (16-bit gradients of a loss that is scaled are rounded twice, half a step each;
-// the usual factor is 1, for which they stay as they are)
+// For a gradient that was rounded before its factor was known: fp32, and bf16, which
+// has fp32's exponents, so that what is rounded twice is off by half a step each
+// time, however small.  (fp16 would lose here what is below 6e-8, most of a
+// large vocabulary's gradient, which is what a loss scale is there to keep:
+// pcm_distill_grad.)  The usual factor is 1, for which they stay as they are.
 template <int DT>
 __global__ __launch_bounds__(256) void scale_kernel(typename RowType<DT>::T *x,
                                                     long long n,
@@ -779,16 +792,16 @@ size_t pcm_distill_scratch_floats(int32_t steps, int32_t batch) {
     return (size_t)steps * batch + steps;
 }
 
-int pcm_distill_loss(const void *logits, int32_t dtype, int64_t ld,
-                     const void *values, int32_t values_dtype,
-                     const int32_t *indices, const float *rest, int32_t k,
-                     const int64_t *targets, const int32_t *lengths,
-                     const float *step_weight, int32_t steps, int32_t batch,
-                     int32_t vocab, double temperature, double hard_weight,
-                     float *loss, void *dlogits, float *scratch,
-                     int32_t *status, void *stream) {
-    PCM_API_GUARD;
-    PCM_REQUIRE(logits && values && indices && loss && scratch, PCM_EINVAL,
+// loss, or the gradient times a factor
+static int distill(const void *logits, int32_t dtype, int64_t ld,
+                   const void *values, int32_t values_dtype,
+                   const int32_t *indices, const float *rest, int32_t k,
+                   const int64_t *targets, const int32_t *lengths,
+                   const float *step_weight, int32_t steps, int32_t batch,
+                   int32_t vocab, double temperature, double hard_weight,
+                   const float *factor, float *loss, void *dlogits,
+                   float *scratch, int32_t *status, void *stream) {
+    PCM_REQUIRE(logits && values && indices && scratch, PCM_EINVAL,
                 "distill_loss: null pointer");
     PCM_REQUIRE(pcm_dtype_known(dtype) && pcm_dtype_known(values_dtype),
                 PCM_EINVAL, "distill_loss: unknown dtype %d / %d", dtype,
@@ -826,7 +839,8 @@ int pcm_distill_loss(const void *logits, int32_t dtype, int64_t ld,
     a.targets = targets; a.lengths = lengths; a.dlogits = dlogits;
     a.status = status;
     a.rows = (long long)steps * batch;
-    a.rowloss = scratch;
+    a.factor = factor;
+    a.rowloss = loss ? scratch : nullptr;
     a.ld = ld; a.B = batch; a.V = vocab; a.k = k;
     a.values_dtype = values_dtype;
     a.weight = step_weight;
@@ -848,10 +862,44 @@ int pcm_distill_loss(const void *logits, int32_t dtype, int64_t ld,
         PCM_BY_DTYPE(dtype, sums = launch_rows<DT, true>(a, st));
     else
         PCM_BY_DTYPE(dtype, sums = launch_rows<DT, false>(a, st));
-    hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, st,
-                       a.rowloss, sums, loss);
+    if (loss)
+        hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, st,
+                           a.rowloss, sums, loss);
     return pcm_check_launch("distill_loss");
 }
+
+int pcm_distill_loss(const void *logits, int32_t dtype, int64_t ld,
+                     const void *values, int32_t values_dtype,
+                     const int32_t *indices, const float *rest, int32_t k,
+                     const int64_t *targets, const int32_t *lengths,
+                     const float *step_weight, int32_t steps, int32_t batch,
+                     int32_t vocab, double temperature, double hard_weight,
+                     float *loss, void *dlogits, float *scratch,
+                     int32_t *status, void *stream) {
+    PCM_API_GUARD;
+    PCM_REQUIRE(loss, PCM_EINVAL, "distill_loss: null pointer");
+    return distill(logits, dtype, ld, values, values_dtype, indices, rest, k,
+                   targets, lengths, step_weight, steps, batch, vocab,
+                   temperature, hard_weight, nullptr, loss, dlogits, scratch,
+                   status, stream);
+}
+
+int pcm_distill_grad(const void *logits, int32_t dtype, int64_t ld,
+                     const void *values, int32_t values_dtype,
+                     const int32_t *indices, const float *rest, int32_t k,
+                     const int64_t *targets, const int32_t *lengths,
+                     const float *step_weight, int32_t steps, int32_t batch,
+                     int32_t vocab, double temperature, double hard_weight,
+                     const float *factor, void *dlogits, float *scratch,
+                     void *stream) {
+    PCM_API_GUARD;
+    PCM_REQUIRE(factor && dlogits, PCM_EINVAL, "distill_grad: null pointer");
+    return distill(logits, dtype, ld, values, values_dtype, indices, rest, k,
+                   targets, lengths, step_weight, steps, batch, vocab,
+                   temperature, hard_weight, factor, nullptr, dlogits, scratch,
+                   nullptr, stream);
+}
+
 
 int pcm_scale(void *x, int32_t dtype, int64_t n, const float *scale,
               void *stream) {

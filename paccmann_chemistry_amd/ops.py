@@ -835,7 +835,7 @@ def top_logits(logits, k, temperature=1.0):
 
 
 def _distill(logits, want, args):
-    """pcm_distill_loss on checked operands: (loss, dlogits or None)."""
+    """pcm_distill_loss on checked operands: (loss, dlogits or None, scratch)."""
     (code, vocab, values, indices, rest, temperature, targets, lengths,
      hard_weight, step_weight, status) = args
     lib = load()
@@ -860,7 +860,7 @@ def _distill(logits, want, args):
                 scratch.data_ptr(), ptr(status), _stream(dev)
             ), 'pcm_distill_loss'
         )
-    return loss, dlogits
+    return loss, dlogits, scratch
 
 
 class DistillLossFn(torch.autograd.Function):
@@ -869,7 +869,7 @@ class DistillLossFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, args):
-        loss, dlogits = _distill(logits, True, args)
+        loss, dlogits, _ = _distill(logits, True, args)
         ctx.dlogits = dlogits
         ctx.scale = (dlogits.data_ptr(), args[0], dlogits.numel())
         return loss
@@ -895,6 +895,47 @@ class DistillLossFn(torch.autograd.Function):
         return dlogits, None
 
 
+class DistillHalfLossFn(torch.autograd.Function):
+    """The same for fp16: the gradient is computed in ``backward``, where the
+    incoming one goes in before the rounding (a loss scale keeps what fp16
+    cannot hold without it).  The logits are read once more for it."""
+
+    @staticmethod
+    def forward(ctx, logits, args):
+        (code, vocab, values, indices, rest, temperature, targets, lengths,
+         hard_weight, step_weight, _) = args
+        loss, _, scratch = _distill(logits, False, args)
+        ctx.save_for_backward(logits, values, indices, rest, targets, lengths,
+                              step_weight, scratch)
+        ctx.scalars = code, vocab, temperature, hard_weight
+        return loss
+
+    @staticmethod
+    def backward(ctx, dloss):
+        if dloss.requires_grad:
+            raise RuntimeError('distill_loss has no second derivative')
+        (logits, values, indices, rest, targets, lengths, step_weight,
+         scratch) = ctx.saved_tensors
+        code, vocab, temperature, hard_weight = ctx.scalars
+        steps, batch, _ = logits.shape
+        dev = logits.device
+        x2, _, ld = _rows_of(logits, 'distill logits')
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        weights = ptr(step_weight)
+        if weights is None and lengths is not None:   # the forward's
+            weights = scratch.data_ptr() + 4 * steps * batch
+        check(
+            load().pcm_distill_grad(
+                x2.data_ptr(), code, ld, values.data_ptr(),
+                _lib.DTYPES[values.dtype], indices.data_ptr(), ptr(rest),
+                indices.shape[-1], ptr(targets), ptr(lengths), weights, steps,
+                batch, vocab, temperature, hard_weight, dloss.data_ptr(),
+                dlogits.data_ptr(), scratch.data_ptr(), _stream(dev)
+            ), 'pcm_distill_grad'
+        )
+        return dlogits, None
+
+
 def distill_loss(logits, teacher, targets=None, lengths=None, hard_weight=0.0,
                  step_weight=None, status=None):
     """Distillation of ``logits[T,B,V]`` (fp32, bf16 or fp16) from a teacher's
@@ -907,10 +948,11 @@ def distill_loss(logits, teacher, targets=None, lengths=None, hard_weight=0.0,
     listed tokens and "any other token", summed over steps after weighting step t by
     ``step_weight[t]`` (default: one over the rows with ``lengths > t``), as
     ``DecoderHeadFn`` reduces its cross entropy.  Returns an fp32 scalar that
-    carries the gradient of the logits.  Indices outside the vocabulary raise
-    STATUS_BAD_TOKEN in ``status`` (see ``check_status``).  Into a graph,
-    forward and backward are captured together, while no eager autograd graph
-    of the same leaves is alive."""
+    carries the gradient of the logits (in fp16 rounded after the incoming
+    gradient has gone in, so a loss scale does what it is there for).  Indices
+    outside the vocabulary raise STATUS_BAD_TOKEN in ``status`` (see
+    ``check_status``).  Into a graph, forward and backward are captured
+    together, while no eager autograd graph of the same leaves is alive."""
     require_device(logits, 'distill logits')
     code = _dtype_code(logits, 'distill logits')
     size = logits.shape
@@ -955,6 +997,8 @@ def distill_loss(logits, teacher, targets=None, lengths=None, hard_weight=0.0,
     args = (code, vocab, values, indices, rest, temperature, targets, lengths,
             hard_weight, step_weight, _status_word(status, dev))
     if logits.requires_grad and torch.is_grad_enabled():
+        if logits.dtype == torch.float16:
+            return DistillHalfLossFn.apply(logits, args)
         return DistillLossFn.apply(logits, args)
     return _distill(logits, False, args)[0]
 

@@ -273,3 +273,122 @@ def test_a_full_list_does_not_change_with_a_shift():
         assert math.isfinite(losses[0]) and losses[0] > 0
         # (32-bit logits, shifted: half a step of 300 each)
         assert max(losses) - min(losses) < 6 * 2.0 ** -15
+
+
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('B,V,k,hard', [
+    (64, 60, 8, 0.5), (64, 500, 8, 0.0), (64, 1500, 9, 0.25),
+    (64, 32000, 32, 0.0), (3, 45001, 64, 0.5), (2, 70001, 9, 0.25)])
+def test_distill_gradient_times_a_factor(B, V, k, hard, dtype):
+    """The incoming gradient goes in before the gradient is rounded: what 16 bits
+    cannot hold without a loss scale they hold with it.  (bf16, which has fp32's
+    exponents, is rounded before and after, so twice.)"""
+    import paccmann_chemistry_amd as P
+    g = _gen(B, V, k)
+    logits, values, indices, rest = _case(1, B, V, k, dtype, 'normal', True, g)
+    targets = torch.randint(0, V, (1, B), generator=g)
+    lengths = (torch.arange(B) != 1).int()
+    exact = Exact(logits, values, indices, rest, 2.0, targets, lengths, hard)
+    dev = _dev()
+    x = logits.to(dev)
+    x[0, 1] = math.nan
+    x.requires_grad_(True)
+    teacher = _teacher(values, indices, rest, 2.0)
+    wide = _strided_leaf(x.detach(), dev)
+    for leaf in (x, wide):
+        for factor in (1.0, 1024.0, 65536.0, -0.25):
+            loss = P.distill_loss(leaf, teacher, targets=targets.to(dev),
+                                  lengths=lengths.to(dev), hard_weight=hard)
+            grad, = torch.autograd.grad(loss * factor, leaf)
+            got = grad.cpu()
+            assert got.dtype == dtype
+            fine = exact.fine(got, factor)
+            if dtype == torch.bfloat16:
+                fine |= (got.double() - exact.grad * factor).abs() <= \
+                    exact.grad_tol * abs(factor) + \
+                    2.01 * HALF[dtype] * (exact.grad * factor).abs()
+            assert bool(fine.all())
+            assert bool((got[0, 1] == 0).all())
+
+
+def _strided_leaf(x, dev):
+    """A leaf whose rows are 3 elements further apart."""
+    wide = torch.full(x.shape[:-1] + (x.shape[-1] + 3, ), math.nan,
+                      dtype=x.dtype, device=dev)
+    view = wide[..., 1:-2]
+    view.copy_(x)
+    return view.detach().requires_grad_(True)
+
+
+@gpu
+def test_distill_of_half_precision_more_than_once():
+    """fp16: the gradient is made in the backward call, so a graph that is kept
+    gives it again, and logits that changed meanwhile raise."""
+    import paccmann_chemistry_amd as P
+    g = _gen(41)
+    dev = _dev()
+    for V in (60, 900):
+        logits, values, indices, rest = _case(3, 4, V, 6, torch.float16,
+                                              'normal', True, g)
+        teacher = _teacher(values, indices, rest, 2.0)
+        weight = torch.tensor([0.5, 0.0, 2.0], device=dev)
+        x = logits.to(dev).requires_grad_(True)
+        want, = torch.autograd.grad(
+            P.distill_loss(x, teacher, step_weight=weight) * 512.0, x)
+        # with one over the rows for a weight it is the weighted one divided
+        plain, = torch.autograd.grad(P.distill_loss(x, teacher) * 1024.0, x)
+        assert bool(((want[2].double() - plain[2].double() * 4).abs() <= 2.02 *
+                     HALF[torch.float16] * want[2].double().abs() + 2.0 ** -22)
+                    .all())
+        assert bool((want[1] == 0).all())
+        loss = P.distill_loss(x, teacher, step_weight=weight) * 512.0
+        first, = torch.autograd.grad(loss, x, retain_graph=True)
+        again, = torch.autograd.grad(loss, x)
+        assert torch.equal(first, want) and torch.equal(again, want)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(loss, x)
+        loss = P.distill_loss(x, teacher)
+        with torch.no_grad():
+            x.mul_(1.0)
+        with pytest.raises(RuntimeError, match='inplace operation'):
+            loss.backward()
+
+
+@gpu
+@pytest.mark.parametrize('V', [60, 900])
+def test_distill_of_half_precision_on_a_side_stream_and_captured(V):
+    import paccmann_chemistry_amd as P
+    g = _gen(41, V)
+    dev = _dev()
+    logits, values, indices, rest = _case(3, 4, V, 6, torch.float16, 'normal',
+                                          True, g)
+    teacher = _teacher(values, indices, rest, 2.0)
+    lengths = torch.tensor([3, 1, 2, 3], dtype=torch.int32, device=dev)
+    x = logits.to(dev).requires_grad_(True)
+    scale = torch.tensor(512.0, device=dev)
+
+    def step(leaf):
+        loss = P.distill_loss(leaf, teacher, lengths=lengths)
+        return torch.autograd.grad(loss * scale, leaf)[0]
+    want = step(x.detach().clone().requires_grad_(True))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(x)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grad = step(x)
+    for i, factor in enumerate((512.0, 64.0, 512.0)):
+        new = torch.randn(3, 4, V, generator=_gen(i, V)).half().to(dev)
+        scale.fill_(factor)
+        with torch.no_grad():
+            x.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = step(new.clone().requires_grad_(True))
+        torch.cuda.synchronize()
+        assert torch.equal(grad, eager)
