@@ -1122,7 +1122,9 @@ def reorder_states(parents, states, row_dims=0, status=None):
     StackGRU's hidden [L, K*B, H] has 1, its stack [K*B, D, W] has 0).  Any
     element type; the dimensions after the rows must be contiguous, no two
     tensors may share memory.  A parent outside [0, K) leaves its rows alone
-    and raises STATUS_BAD_PARENT in ``status`` (see ``check_status``)."""
+    and raises STATUS_BAD_PARENT in ``status`` (see ``check_status``).  For
+    autograd it is an operation in place: a backward that needs a state as it
+    was raises."""
     lib = load()
     require_device(parents, 'parents')
     if parents.dtype != torch.int32 or parents.dim() != 2 \
@@ -1161,6 +1163,8 @@ def reorder_states(parents, states, row_dims=0, status=None):
                 ptr(status), _stream(dev)
             ), 'pcm_reorder_states'
         )
+    # what an operation saved of them for its backward is no longer there
+    torch._C._increment_version(states)
 
 
 def adam_step(param, grad, exp_avg, exp_avg_sq, lr, beta1, beta2, eps, step,
