@@ -3,8 +3,40 @@ reordering promise beside their numbers: what they refuse, what autograd is told
 orders among equals, values bit for bit, the paths of the model around them."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from test_top_distill_beam import _dev, _gen, gpu
+
+
+# --------------------------------------------------------------------------
+# distillation
+# --------------------------------------------------------------------------
+def _small(dtype=torch.float32):
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    g = _gen(4, 4)
+    x = torch.randn(2, 3, 40, generator=g).to(dtype).to(dev)
+    values, places = torch.topk(torch.randn(2, 3, 40, generator=g), 5)
+    rest = torch.zeros(2, 3, device=dev)
+    return x, P.TopLogits(values.to(dev), places.int().to(dev), rest, 2.0)
+
+
+@gpu
+def test_distill_refuses_forward_mode():
+    """A tangent that would be lost raises."""
+    import paccmann_chemistry_amd as P
+    x, teacher = _small()
+    with forward_ad.dual_level():
+        plain = float(P.distill_loss(x, teacher))
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match='forward mode'):
+            P.distill_loss(dual, teacher)
+        with pytest.raises(RuntimeError, match='forward mode'):
+            P.distill_loss(dual.clone().requires_grad_(True), teacher)
+        rest = forward_ad.make_dual(teacher.rest, torch.ones_like(teacher.rest))
+        with pytest.raises(RuntimeError, match='forward mode'):
+            P.distill_loss(x, teacher._replace(rest=rest))
+    assert plain == float(P.distill_loss(x, teacher))
 
 
 # --------------------------------------------------------------------------
@@ -29,3 +61,18 @@ def test_reorder_states_tells_autograd():
         state = torch.arange(4.0, device=dev).view(4, 1)
         P.reorder_states(parents, [state, hidden])
         assert state.view(-1).tolist() == [2.0, 1.0, 0.0, 3.0]
+
+
+@gpu
+def test_reorder_states_refuses_forward_mode():
+    """A tangent that would stay where it was raises."""
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    parents = torch.tensor([[1], [1]], dtype=torch.int32, device=dev)
+    state = torch.randn(2, 8, generator=_gen(1)).to(dev)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(state, torch.ones_like(state))
+        with pytest.raises(ValueError, match='tangent'):
+            P.reorder_states(parents, [dual])
+        P.reorder_states(parents, [state])
+    assert torch.equal(state[0], state[1])
