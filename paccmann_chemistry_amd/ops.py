@@ -872,6 +872,16 @@ def _distill(logits, want, args):
     return loss, dlogits, scratch
 
 
+def _refuse_create_graph():
+    """In a ``backward``: the gradient would be a constant of that graph, and a
+    second derivative through it silently lack this loss."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(
+            'distill_loss has no second derivative (backward with '
+            'create_graph)'
+        )
+
+
 class DistillLossFn(torch.autograd.Function):
     """loss = distill(logits[T,B,V], teacher); the gradient is computed with
     the loss and multiplied by the incoming one in ``backward``."""
@@ -891,8 +901,7 @@ class DistillLossFn(torch.autograd.Function):
                 'distill_loss backward called twice: the gradient is handed '
                 'out by the first call (retain_graph is not supported)'
             )
-        if dloss.requires_grad:
-            raise RuntimeError('distill_loss has no second derivative')
+        _refuse_create_graph()
         ctx.dlogits = None
         # (an fp32 scalar; autograd's thread has the device and the stream of
         # the forward)
@@ -921,8 +930,7 @@ class DistillHalfLossFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dloss):
-        if dloss.requires_grad:
-            raise RuntimeError('distill_loss has no second derivative')
+        _refuse_create_graph()
         (logits, values, indices, rest, targets, lengths, step_weight,
          scratch) = ctx.saved_tensors
         code, vocab, temperature, hard_weight = ctx.scalars
@@ -958,8 +966,9 @@ def distill_loss(logits, teacher, targets=None, lengths=None, hard_weight=0.0,
     ``step_weight[t]`` (default: one over the rows with ``lengths > t``), as
     ``DecoderHeadFn`` reduces its cross entropy.  Returns an fp32 scalar that
     carries the gradient of the logits (in fp16 rounded after the incoming
-    gradient has gone in, so a loss scale does what it is there for).  Indices
-    outside the vocabulary raise STATUS_BAD_TOKEN in ``status`` (see
+    gradient has gone in, so a loss scale does what it is there for; a
+    backward with ``create_graph`` raises, for there is no second derivative).
+    Indices outside the vocabulary raise STATUS_BAD_TOKEN in ``status`` (see
     ``check_status``).  Into a graph, forward and backward are captured
     together, while no eager autograd graph of the same leaves is alive."""
     require_device(logits, 'distill logits')

@@ -5,7 +5,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from test_top_distill_beam import _dev, _gen, gpu
+from test_top_distill_beam import DTYPES, _dev, _gen, gpu
 
 
 # --------------------------------------------------------------------------
@@ -37,6 +37,27 @@ def test_distill_refuses_forward_mode():
         with pytest.raises(RuntimeError, match='forward mode'):
             P.distill_loss(x, teacher._replace(rest=rest))
     assert plain == float(P.distill_loss(x, teacher))
+
+
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_distill_second_derivative_is_not_left_out(dtype):
+    """With create_graph the gradient would be a constant: it raises, and the
+    loss can be derived once all the same."""
+    import paccmann_chemistry_amd as P
+    x, teacher = _small(dtype)
+    x.requires_grad_(True)
+    want, = torch.autograd.grad(P.distill_loss(x, teacher), x)
+    loss = P.distill_loss(x, teacher)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match='second derivative'):
+            torch.autograd.grad(loss, x, create_graph=True)
+    loss = P.distill_loss(x, teacher)
+    with pytest.raises(RuntimeError, match='second derivative'):
+        grad, = torch.autograd.grad(loss, x, create_graph=True)
+        (grad.float().pow(2).sum() + x.float().sum()).backward()
+    grad, = torch.autograd.grad(loss, x)
+    assert torch.equal(grad, want)
 
 
 # --------------------------------------------------------------------------
