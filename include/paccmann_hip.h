@@ -427,7 +427,7 @@ int pcm_stackgru_generate_beam(const pcm_dims *dims,
  *
  *   logits   [rows] rows of `vocab` elements of `dtype`, row stride ld elements
  *   k        1 .. min(vocab, PCM_TOP_MAX)
- *   values   [rows][k] of `dtype`, exact;  indices int32[rows][k]
+ *   values   [rows][k] of `dtype`, bit for bit;  indices int32[rows][k]
  *   rest     fp32[rows]
  *   A NaN ranks below every number and makes the row's rest NaN.
  */

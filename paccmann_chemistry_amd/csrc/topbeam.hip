@@ -366,6 +366,15 @@ struct TopArgs {
     float scale, inv_t;     // log2(e) / temperature; 1 / temperature
 };
 
+// A listed element as it is in its row x.  Its key holds a value; the sign of a zero
+// and a NaN's payload are not in it, and these are read again.
+template <int DT>
+__device__ __forceinline__ typename RowType<DT>::T listed_value(
+    const typename RowType<DT>::T *x, double key) {
+    const float v = key_value(key);
+    return fabsf(v) > 0.f ? RowType<DT>::down(v) : x[key_index(key)];
+}
+
 // Entries past the `found` numbers above -inf: the -inf ones by index, then the
 // NaN by index.  One wave; rare.
 template <int DT>
@@ -402,8 +411,9 @@ __global__ __launch_bounds__(256) void top_short_kernel(TopArgs a, long long row
     const long long row =
         (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
     if (row >= rows) return;   // (all lanes of a row)
+    const T *logits = (const T *)a.logits + row * a.ld;
     RowRegs<DT, LPR, G> x;
-    x.load((const T *)a.logits + row * a.ld, a.V, sub);
+    x.load(logits, a.V, sub);
     ShortTop<KT> top;
     top.template of<DT, LPR, G>(x, a.V, sub);
     T *values = (T *)a.values + row * a.k;
@@ -414,7 +424,7 @@ __global__ __launch_bounds__(256) void top_short_kernel(TopArgs a, long long row
         if (j < a.k) {
             last = top.l[j];
             if (j % LPR == sub) {
-                values[j] = R::down(key_value(last));
+                values[j] = listed_value<DT>(logits, last);
                 indices[j] = key_index(last);
             }
         }
@@ -511,7 +521,7 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
             T *values = (T *)a.values + row * a.k;
             int32_t *indices = a.indices + row * a.k;
             if (lane < min(found, a.k)) {
-                values[lane] = R::down(key_value(key));
+                values[lane] = listed_value<DT>(x, key);
                 indices[lane] = key_index(key);
             }
             if (found < a.k) top_fill<DT>(x, a.V, found, a.k, values, indices, lane);
@@ -643,7 +653,7 @@ __global__ __launch_bounds__(1024) void top_join_kernel(TopArgs a) {
         int32_t *indices = a.indices + row * a.k;
         const int found = __popcll(__ballot(key > KEY_NONE && lane < a.k));
         if (lane < found) {
-            values[lane] = R::down(key_value(key));
+            values[lane] = listed_value<DT>((const T *)a.logits + row * a.ld, key);
             indices[lane] = key_index(key);
         }
         if (found < a.k)

@@ -8,6 +8,11 @@ from torch.autograd import forward_ad
 from test_top_distill_beam import DTYPES, _dev, _gen, gpu
 
 
+def _bits(t):
+    """``t`` as whole numbers: -0 is not +0, a NaN is its payload."""
+    return t.view({2: torch.int16, 4: torch.int32}[t.element_size()])
+
+
 # --------------------------------------------------------------------------
 # distillation
 # --------------------------------------------------------------------------
@@ -58,6 +63,36 @@ def test_distill_second_derivative_is_not_left_out(dtype):
         (grad.float().pow(2).sum() + x.float().sum()).backward()
     grad, = torch.autograd.grad(loss, x)
     assert torch.equal(grad, want)
+
+
+# --------------------------------------------------------------------------
+# top logits
+# --------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows,vocab,k', [
+    (3, 16, 16), (9000, 13, 13), (3, 60, 60), (9000, 60, 4), (9000, 700, 16), (3, 300, 20), (2, 5003, 40),
+    (2, 33001, 64), (1, 262144, 50)])
+def test_top_logits_values_keep_their_bits(rows, vocab, k, dtype):
+    """-0 and NaN come back as they are."""
+    import paccmann_chemistry_amd as P
+    g = _gen(rows, vocab, k)
+    x = torch.where(torch.rand(rows, vocab, generator=g) < 0.5, 0.0, -0.0)
+    x[0, 2] = 1.0
+    x = x.to(dtype)
+    # payloads: quiet NaNs of both signs where fewer numbers are left than asked
+    bits = _bits(x)
+    odd = {torch.float32: [0x7FC00123, -0x3FFEDC], torch.bfloat16: [
+        0x7FC3, -0x3B], torch.float16: [0x7E05, -0x1F9]}[dtype]
+    if vocab == k:
+        bits[1, 4:] = torch.tensor(odd, dtype=bits.dtype).repeat(vocab)[
+            :vocab - 4]
+    top = P.top_logits(x.to(_dev()), k)
+    at = top.indices.cpu().long()
+    assert torch.equal(_bits(top.values.cpu()), bits.gather(1, at))
+    if rows > 2:
+        assert torch.equal(at[2], torch.arange(k))
+    assert at[0, :3].tolist() == [2, 0, 1]
 
 
 # --------------------------------------------------------------------------
