@@ -737,6 +737,14 @@ __device__ __forceinline__ double beam_score(const BeamArgs &a, double score,
     return score + (((double)v - m) * a.inv_t - log_s);
 }
 
+// The j-th candidate of a beam that has ended: end_token, then the others, which are
+// -inf, in order; of one that holds no score all are, so all are in order.
+__device__ __forceinline__ int ended_token(const BeamArgs &a, int j,
+                                           double score) {
+    if (!(score > -INFINITY)) return j;
+    return j == 0 ? a.end : j - 1 + (j - 1 >= a.end ? 1 : 0);
+}
+
 // Per beam row (or part of one): the `width` largest logits -- the row's
 // normaliser does not change their order -- and its maximum and sum, in one
 // pass.  8 x 64 rows of 32000 bf16: 23 us (26 MB; 17 operations in 64 bits per
@@ -864,9 +872,8 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
     int tok = -1;
     double c = -INFINITY;
     if (done) {
-        // end_token, then the others in order
-        tok = lane == 0 ? a.end : lane - 1 + (lane - 1 >= a.end ? 1 : 0);
-        if (lane == 0 && score == score) c = score;
+        tok = ended_token(a, lane, score);
+        if (lane == 0 && score > -INFINITY) c = score;
     } else {
         const double m = score > -INFINITY ? wave_max(pm) : -INFINITY;
         tok = lane;   // a row without a distribution: the tokens in order
@@ -960,9 +967,9 @@ __global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
             if (j < a.width && j % LPR == sub) {
                 int tok = j;   // a row without a distribution: tokens in order
                 double c = -INFINITY;
-                if (done) {    // end_token, then the others in order
-                    tok = j == 0 ? a.end : j - 1 + (j - 1 >= a.end ? 1 : 0);
-                    if (j == 0 && score == score) c = score;
+                if (done) {
+                    tok = ended_token(a, j, score);
+                    if (j == 0 && score > -INFINITY) c = score;
                 } else if (live) {
                     tok = top.l[j] > KEY_NONE ? key_index(top.l[j]) : a.V;
                     c = beam_score(a, score, key_value(top.l[j]), m, log_s);

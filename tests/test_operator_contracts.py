@@ -1,11 +1,14 @@
 """What the entry points of top logits, distillation, beam selection and state
 reordering promise beside their numbers: what they refuse, what autograd is told,
 orders among equals, values bit for bit, the paths of the model around them."""
+import math
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from test_top_distill_beam import DTYPES, _dev, _gen, gpu
+from test_top_distill_beam import DTYPES, _check_beam, _dev, _gen, gpu
+from test_top_distill_beam import ref_beam
 
 
 def _bits(t):
@@ -93,6 +96,31 @@ def test_top_logits_values_keep_their_bits(rows, vocab, k, dtype):
     if rows > 2:
         assert torch.equal(at[2], torch.arange(k))
     assert at[0, :3].tolist() == [2, 0, 1]
+
+
+# --------------------------------------------------------------------------
+# beam selection
+# --------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize('V', [20, 60, 700, 9000])
+@pytest.mark.parametrize('lost', [-math.inf, math.nan])
+def test_ended_beams_without_a_score(V, lost):
+    """A beam that ended and holds nothing: all its candidates are -inf, so they
+    are in the order of the tokens, the end token among them."""
+    import paccmann_chemistry_amd as P
+    g = _gen(V)
+    dev = _dev()
+    logits = torch.randn(2, 4, V, generator=g)
+    scores = torch.tensor([[lost, lost, -1.0, lost], [lost, -2.0, lost, lost]],
+                          dtype=torch.float64)
+    finished = torch.tensor([[True, True, False, False],
+                             [True, True, True, True]])
+    for end in (0, 2, 7):
+        want = ref_beam(logits, scores, 5, 1.0, finished, end)
+        step = P.beam_select(logits.to(dev), scores.to(dev), width=5,
+                             finished=finished.to(dev), end_token=end)
+        _check_beam(step, want, logits)
+    assert want[0][:, 0].tolist() == [0, 1, 2, 3, 4]
 
 
 # --------------------------------------------------------------------------
