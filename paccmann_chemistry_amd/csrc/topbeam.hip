@@ -972,7 +972,9 @@ __global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
                     if (j == 0 && score > -INFINITY) c = score;
                 } else if (live) {
                     tok = top.l[j] > KEY_NONE ? key_index(top.l[j]) : a.V;
-                    c = beam_score(a, score, key_value(top.l[j]), m, log_s);
+                    // (a masked token is -inf beside a score of +inf too)
+                    const float v = key_value(top.l[j]);
+                    if (v > -INFINITY) c = beam_score(a, score, v, m, log_s);
                 }
                 const int at = rb * per + k * a.width + j;
                 beam_c[at] = tok < a.V ? c : -INFINITY;

@@ -123,6 +123,36 @@ def test_ended_beams_without_a_score(V, lost):
     assert want[0][:, 0].tolist() == [0, 1, 2, 3, 4]
 
 
+@gpu
+@pytest.mark.parametrize('V,batch', [(60, 5), (60, 3000), (128, 2), (700, 2),
+                                     (5003, 2)])
+def test_beams_of_infinite_score(V, batch):
+    """A score of +inf (a forced beam) wins with its tokens in order; tokens
+    that are masked stay at -inf, and every place is filled."""
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    logits = torch.full((3, batch, V), -math.inf)
+    logits[:, :, 5:8] = torch.tensor([1.0, 3.0, 2.0])
+    scores = torch.full((3, batch), -1.0, dtype=torch.float64)
+    scores[1] = math.inf
+    step = P.beam_select(logits.to(dev), scores.to(dev), width=9)
+    inf, low = math.inf, 0.0
+    tokens, parents = step.tokens.cpu(), step.parents.cpu()
+    # equal sums of one beam: the larger logit first
+    assert bool((parents[:3] == 1).all())
+    assert bool((tokens[:3] == torch.tensor([[6], [7], [5]])).all())
+    assert bool((step.scores.cpu()[:3] == inf).all())
+    assert bool((step.scores.cpu()[3:] < low).all())
+    assert bool((tokens[3:] == torch.tensor(
+        [[6], [6], [7], [7], [5], [5]])).all())
+    assert bool((parents[3:] == torch.tensor(
+        [[0], [2], [0], [2], [0], [2]])).all())
+    step = P.beam_select(logits.to(dev), scores.to(dev), width=12)
+    assert bool((step.scores.cpu()[9:] == -inf).all())
+    assert bool((step.parents.cpu()[9:] == 0).all())
+    assert bool((step.tokens.cpu()[9:] == torch.tensor([[0], [1], [2]])).all())
+
+
 # --------------------------------------------------------------------------
 # states that follow their beams
 # --------------------------------------------------------------------------
