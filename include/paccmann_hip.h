@@ -426,7 +426,7 @@ int pcm_stackgru_generate_beam(const pcm_dims *dims,
  * what a teacher writes for pcm_distill_loss.
  *
  *   logits   [rows] rows of `vocab` elements of `dtype`, row stride ld elements
- *   k        1 .. min(vocab, PCM_TOP_MAX)
+ *   k        1 .. min(vocab, PCM_TOP_MAX);  1e-30 < temperature < 1e30
  *   values   [rows][k] of `dtype`, bit for bit;  indices int32[rows][k]
  *   rest     fp32[rows]
  *   A NaN ranks below every number and makes the row's rest NaN.
@@ -511,7 +511,8 @@ int pcm_scale(void *x, int32_t dtype, int64_t n, const float *scale,
  *   tokens   int64[width][batch], parents int32[width][batch],
  *   scores_out fp64[width][batch], finished_out uint8[width][batch]
  *            (finished[parent], or the token is end_token)
- *   1 <= beams, width <= PCM_BEAM_MAX and width <= beams * vocab.
+ *   1 <= beams, width <= PCM_BEAM_MAX and width <= beams * vocab;
+ *   1e-30 < temperature < 1e30.
  */
 size_t pcm_beam_select_workspace_bytes(int32_t beams, int32_t batch,
                                        int32_t vocab, int32_t width);

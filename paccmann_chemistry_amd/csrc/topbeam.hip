@@ -1203,8 +1203,9 @@ int pcm_top_logits(const void *logits, int32_t dtype, int64_t rows, int64_t ld,
     PCM_REQUIRE(k >= 1 && k <= PCM_TOP_MAX && k <= vocab, PCM_EINVAL,
                 "top_logits: k=%d outside 1..min(%d, vocab %d)", k, PCM_TOP_MAX,
                 vocab);
-    PCM_REQUIRE(temperature > 0. && temperature < 1e30, PCM_EINVAL,
-                "top_logits: temperature must be positive");
+    // (1 / temperature has to be a 32-bit number)
+    PCM_REQUIRE(temperature > 1e-30 && temperature < 1e30, PCM_EINVAL,
+                "top_logits: temperature outside 1e-30..1e30");
     const size_t need = pcm_top_logits_workspace_bytes(rows, vocab, k);
     PCM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), PCM_ENOMEM,
                 "top_logits: workspace %zu < %zu bytes", workspace_bytes, need);

@@ -7,8 +7,8 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from test_top_distill_beam import DTYPES, _check_beam, _dev, _gen, gpu
-from test_top_distill_beam import ref_beam
+from test_top_distill_beam import DTYPES, _check_beam, _dev, _gen, _host
+from test_top_distill_beam import _refused, gpu, ref_beam
 
 
 def _bits(t):
@@ -71,6 +71,16 @@ def test_distill_second_derivative_is_not_left_out(dtype):
 # --------------------------------------------------------------------------
 # top logits
 # --------------------------------------------------------------------------
+def test_top_logits_refuses_temperatures_beyond_its_range():
+    """Below 1e-30 the factor 1 / temperature leaves 32 bits."""
+    from paccmann_chemistry_amd import _lib
+    lib = _lib.load()
+    at, _keep = _host()
+    for tau in (1e-300, 1e-39, 1e-30, 1e30, math.inf, -1.0):
+        _refused(lib, lib.pcm_top_logits(at, 0, 2, 20, 20, 3, tau, at, at, at,
+                                         None, 0, None), 'temperature')
+
+
 @gpu
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('rows,vocab,k', [
