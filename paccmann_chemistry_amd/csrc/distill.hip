@@ -830,9 +830,13 @@ static int distill(const void *logits, int32_t dtype, int64_t ld,
     PCM_REQUIRE(vocab <= 512 || (long long)steps * batch < (1ll << 24),
                 PCM_EINVAL, "distill_loss: %lld rows of %d logits are too many "
                 "for a launch", (long long)steps * batch, vocab);
-    PCM_REQUIRE((long long)steps * batch < (1ll << 28), PCM_EINVAL,
+    // (16 lanes a row, in blocks of four; of up to 128 logits 4 and 16)
+    PCM_REQUIRE((long long)steps * batch <= (1ll << 28) - 4, PCM_EINVAL,
                 "distill_loss: %lld rows are too many for a launch",
                 (long long)steps * batch);
+    PCM_REQUIRE(!lengths || step_weight || steps < (1 << 26) - 4, PCM_EINVAL,
+                "distill_loss: the weights of %d steps are too many for a launch",
+                steps);
     hipStream_t st = (hipStream_t)stream;
     DistillArgs a;
     a.logits = logits; a.values = values; a.indices = indices; a.rest = rest;

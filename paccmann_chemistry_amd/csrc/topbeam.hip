@@ -1015,7 +1015,9 @@ RowPlan row_plan(long long rows, int V, int least) {
 }
 // A launch has less than 2^32 threads: may these rows be one?
 bool rows_fit(long long rows, int V, int k, const RowPlan &p) {
-    if (short_rows(rows, V, k)) return rows < (1ll << 28);
+    // (at most 16 lanes a row, and blocks of at most 64 rows that need not be full;
+    // beams: 4 batch rows of 16)
+    if (short_rows(rows, V, k)) return rows <= (1ll << 28) - 64;
     const int threads = p.len <= 512 ? 64 : p.len <= 2048 ? 256 : 1024;
     return rows * p.parts * threads < (1ll << 32);
 }

@@ -163,6 +163,34 @@ def test_beams_of_infinite_score(V, batch):
     assert bool((step.tokens.cpu()[9:] == torch.tensor([[0], [1], [2]])).all())
 
 
+def test_launches_of_too_many_threads_are_refused():
+    """A launch has less than 2^32 threads, those of its last block included."""
+    from paccmann_chemistry_amd import _lib
+    lib = _lib.load()
+    at, _keep = _host()
+
+    def beam(beams, batch, vocab):
+        return lib.pcm_beam_select(
+            at, 1, vocab, at, None, beams, batch, vocab, 1, 1.0, -1, at, at,
+            at, None, at, 1 << 60, None)
+
+    def top(rows, vocab):
+        return lib.pcm_top_logits(at, 1, rows, vocab, vocab, 3, 1.0, at, at,
+                                  at, at, 1 << 60, None)
+
+    def distill(steps, batch, vocab, lengths):
+        return lib.pcm_distill_loss(
+            at, 1, vocab, at, 0, at, None, 1, None, lengths, None, steps,
+            batch, vocab, 1.0, 0.0, at, None, at, None, None)
+    _refused(lib, beam(16, 1 << 22, 500), 'too many')
+    # the last block of a launch that is just too long, filled up
+    _refused(lib, beam(16, (1 << 24) - 1, 200), 'too many')
+    _refused(lib, top((1 << 28) - 1, 200), 'too many')
+    _refused(lib, distill((1 << 28) - 1, 1, 200, None), 'too many')
+    # the weights of the steps
+    _refused(lib, distill(1 << 26, 1, 20, at), 'too many')
+
+
 # --------------------------------------------------------------------------
 # states that follow their beams
 # --------------------------------------------------------------------------
