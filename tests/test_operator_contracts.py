@@ -182,7 +182,7 @@ def test_launches_of_too_many_threads_are_refused():
         return lib.pcm_distill_loss(
             at, 1, vocab, at, 0, at, None, 1, None, lengths, None, steps,
             batch, vocab, 1.0, 0.0, at, None, at, None, None)
-    _refused(lib, beam(16, 1 << 22, 500), 'too many')
+    _refused(lib, beam(16, 1 << 22, 1025), 'too many')
     # the last block of a launch that is just too long, filled up
     _refused(lib, beam(16, (1 << 24) - 1, 200), 'too many')
     _refused(lib, top((1 << 28) - 1, 200), 'too many')
