@@ -538,7 +538,9 @@ typedef struct pcm_state {
 /*
  * Lets the states follow their beams, in place: in every state, row
  * k * batch + b becomes what row parents[k][b] * batch + b was.  No two rows
- * and no two states may share memory.
+ * and no two states may share memory, nor a state and the parents; states that lie
+ * between each other (columns of one buffer) are told apart by what divides all
+ * their strides.
  *   parents  int32[beams][batch]; one outside [0, beams) leaves its rows as
  *            they were and or-s PCM_STATUS_BAD_PARENT into *status (nullable)
  */

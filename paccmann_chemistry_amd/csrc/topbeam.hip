@@ -1059,6 +1059,52 @@ struct ReorderArgs {
     ReorderState s[PCM_MAX_STATES];
 };
 
+// The bytes of a state: pieces of `piece` bytes from lo on, at multiples of `step`
+// from each other (0: one piece), all before hi.
+struct StateBytes {
+    uintptr_t lo, hi;
+    unsigned long long piece, step;
+    // rows (or outer indices) that lie end to end are one piece
+    StateBytes(const pcm_state &s, long long rows) {
+        lo = (uintptr_t)s.data;
+        hi = lo + (s.outer - 1) * s.outer_stride + (rows - 1) * s.row_stride +
+             s.row_bytes;
+        long long at[2] = {s.row_stride, s.outer_stride}, n[2] = {rows, s.outer};
+        if (n[1] > 1 && (n[0] == 1 || at[1] < at[0])) {   // the inner ones first
+            const long long t = at[0], m = n[0];
+            at[0] = at[1]; n[0] = n[1];
+            at[1] = t; n[1] = m;
+        }
+        piece = s.row_bytes;
+        step = 0;
+        for (int i = 0; i < 2; ++i) {
+            if (n[i] == 1) continue;
+            if (step == 0 && (unsigned long long)at[i] == piece) piece *= n[i];
+            else step = common(step, at[i]);
+        }
+    }
+    StateBytes(const void *data, long long bytes)
+        : lo((uintptr_t)data), hi(lo + bytes), piece(bytes), step(0) {}
+    static unsigned long long common(unsigned long long a, unsigned long long b) {
+        while (b) {
+            const unsigned long long c = a % b;
+            a = b;
+            b = c;
+        }
+        return a;
+    }
+    // Whether they share no byte: one lies before the other, or between the
+    // other's pieces, as seen modulo a number that divides all steps.
+    bool apart(const StateBytes &o) const {
+        if (hi <= o.lo || o.hi <= lo) return true;
+        const unsigned long long m = common(step, o.step);
+        if (m == 0) return false;
+        const unsigned long long d = o.lo >= lo ? (o.lo - lo) % m
+                                                : (m - (lo - o.lo) % m) % m;
+        return d >= piece && d + o.piece <= m;
+    }
+};
+
 // A thread owns the same units of one batch row in ALL beams: it loads what
 // every beam will hold before it stores any of it, so the move is in place
 // whatever the parents are.  K bounds the beams (the arrays stay in registers),
@@ -1348,7 +1394,7 @@ int pcm_reorder_states(const int32_t *parents, int32_t beams, int32_t batch,
     a.parents = parents; a.status = status;
     a.beams = beams; a.batch = batch; a.count = 0;
     const long long rows = (long long)beams * batch;
-    uintptr_t lo[PCM_MAX_STATES], hi[PCM_MAX_STATES];
+    int known[PCM_MAX_STATES];   // states that are not empty
     long long most = 0;
     for (int i = 0; i < count; ++i) {
         pcm_state s = states[i];
@@ -1369,16 +1415,16 @@ int pcm_reorder_states(const int32_t *parents, int32_t beams, int32_t batch,
                     PCM_EINVAL,
                     "reorder_states: rows of state %d share memory", i);
         const int n = a.count;
-        lo[n] = (uintptr_t)s.data;
-        hi[n] = lo[n] + (s.outer - 1) * s.outer_stride +
-                (rows - 1) * s.row_stride + s.row_bytes;
+        const StateBytes bytes(s, rows);
+        known[n] = i;
         for (int j = 0; j < n; ++j)
-            PCM_REQUIRE(hi[n] <= lo[j] || hi[j] <= lo[n], PCM_EINVAL,
+            PCM_REQUIRE(bytes.apart(StateBytes(states[known[j]], rows)),
+                        PCM_EINVAL,
                         "reorder_states: state %d shares memory with another",
                         i);
         int unit = 16;
         const unsigned long long bits =
-            (unsigned long long)lo[n] | (unsigned long long)s.row_bytes |
+            (unsigned long long)bytes.lo | (unsigned long long)s.row_bytes |
             (unsigned long long)s.row_stride |
             (s.outer > 1 ? (unsigned long long)s.outer_stride : 0ull);
         while (bits & (unit - 1)) unit >>= 1;
@@ -1405,6 +1451,11 @@ int pcm_reorder_states(const int32_t *parents, int32_t beams, int32_t batch,
         most = units > most ? units : most;
         a.count = n + 1;
     }
+    const StateBytes from(parents, 4 * rows);
+    for (int n = 0; n < a.count; ++n)
+        PCM_REQUIRE(StateBytes(states[known[n]], rows).apart(from), PCM_EINVAL,
+                    "reorder_states: state %d shares memory with the parents",
+                    known[n]);
     // enough blocks per batch row to spread a small batch over the chip
     long long split = (most + 255) / 256;
     const long long want = (2048 + batch - 1) / batch;

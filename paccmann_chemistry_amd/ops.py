@@ -1099,17 +1099,17 @@ def beam_select(logits, scores, width=None, temperature=1.0, finished=None,
     return BeamStep(tokens, parents, scores_out, finished_out)
 
 
-def _state_view(t, row_dim, rows, what):
-    """The fields of the pcm_state of a tensor whose dimension ``row_dim`` is
-    the beams' rows."""
+def _state_view(t, row_dim, rows, n):
+    """The fields of the pcm_state of state ``n``, a tensor whose dimension
+    ``row_dim`` is the beams' rows."""
     dim = t.dim()
     if not -dim <= row_dim < dim:
-        raise ValueError(f'{what}: row dimension {row_dim} of {dim}')
+        raise ValueError(f'state {n}: row dimension {row_dim} of {dim}')
     row_dim %= dim
     shape, size = t.shape, t.element_size()
     if shape[row_dim] != rows:
         raise ValueError(
-            f'{what} has {shape[row_dim]} rows, expected {rows}'
+            f'state {n} has {shape[row_dim]} rows, expected {rows}'
         )
     if t.is_contiguous():
         piece = size * math.prod(shape[row_dim + 1:])
@@ -1120,7 +1120,7 @@ def _state_view(t, row_dim, rows, what):
     for d in range(dim - 1, row_dim, -1):
         if shape[d] != 1 and stride[d] != inner:
             raise ValueError(
-                f'{what}: the dimensions after its rows must be contiguous'
+                f'state {n}: the dimensions after its rows must be contiguous'
             )
         inner *= shape[d]
     outer, outer_stride = 1, 0   # the dimensions before them, as one
@@ -1129,7 +1129,8 @@ def _state_view(t, row_dim, rows, what):
             continue
         if outer > 1 and stride[d] != outer * outer_stride:
             raise ValueError(
-                f'{what}: the dimensions before its rows must be evenly spaced'
+                f'state {n}: the dimensions before its rows must be evenly '
+                'spaced'
             )
         if outer == 1:
             outer_stride = stride[d]
@@ -1157,6 +1158,8 @@ def reorder_states(parents, states, row_dims=0, status=None):
     beams, batch = parents.shape
     if beams > _lib.BEAM_MAX:
         raise ValueError(f'{beams} beams: expected 1..{_lib.BEAM_MAX}')
+    if isinstance(states, torch.Tensor):
+        raise TypeError('states: expected a list of tensors')
     if not 1 <= len(states) <= _lib.MAX_STATES:
         raise ValueError(f'{len(states)} states: expected 1..'
                          f'{_lib.MAX_STATES}')
@@ -1166,18 +1169,16 @@ def reorder_states(parents, states, row_dims=0, status=None):
         raise ValueError('row_dims: one for each state')
     dev = parents.device
     table = []
-    for state, row_dim in zip(states, row_dims):
+    for n, (state, row_dim) in enumerate(zip(states, row_dims)):
         if state.device != dev:
             raise ValueError(
-                f'state {len(table) // 5} is on {state.device}, the parents '
-                f'on {dev}'
+                f'state {n} is on {state.device}, the parents on {dev}'
             )
         if state.requires_grad:
-            raise ValueError(f'state {len(table) // 5} requires a gradient')
+            raise ValueError(f'state {n} requires a gradient')
         if _has_tangent(state):
-            raise ValueError(f'state {len(table) // 5} carries a tangent')
-        table += _state_view(state, row_dim, beams * batch,
-                             f'state {len(table) // 5}')
+            raise ValueError(f'state {n} carries a tangent')
+        table += _state_view(state, row_dim, beams * batch, n)
     if not parents.is_contiguous():
         parents = parents.contiguous()
     _status_word(status, dev)

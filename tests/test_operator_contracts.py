@@ -8,7 +8,7 @@ import torch
 from torch.autograd import forward_ad
 
 from test_top_distill_beam import DTYPES, _check_beam, _dev, _gen, _host
-from test_top_distill_beam import _refused, gpu, ref_beam
+from test_top_distill_beam import _refused, _rows_of, gpu, ref_beam
 
 
 def _bits(t):
@@ -228,3 +228,56 @@ def test_reorder_states_refuses_forward_mode():
             P.reorder_states(parents, [dual])
         P.reorder_states(parents, [state])
     assert torch.equal(state[0], state[1])
+
+
+def test_reorder_states_of_interleaved_tensors():
+    """Whether tensors share memory is asked of their elements, not of the
+    stretch they lie in; the parents count too."""
+    from paccmann_chemistry_amd import _lib
+    lib = _lib.load()
+    at, _keep = _host()
+    base = at.value
+
+    def call(states, beams=2, batch=2):
+        table = (_lib.PcmState * len(states))(
+            *[_lib.PcmState(*s) for s in states])
+        return lib.pcm_reorder_states(base + 4096, beams, batch, table,
+                                      len(states), None, None)
+    # rows of 64 bytes, three columns: overlapping by one byte
+    _refused(lib, call([(base, 1, 0, 64, 16), (base + 15, 1, 0, 64, 8)]),
+             'another')
+    _refused(lib, call([(base + 8, 1, 0, 64, 16), (base, 1, 0, 64, 9)]),
+             'another')
+    # the second's end meets the next row's beginning
+    _refused(lib, call([(base, 1, 0, 64, 16), (base + 48, 1, 0, 64, 17)]),
+             'another')
+    _refused(lib, call([(base, 1, 0, 64, 16), (base + 32, 2, 128, 32, 16)]),
+             'another')
+    _refused(lib, call([(base + 4092, 1, 0, 64, 16)]), 'parents')
+    _refused(lib, call([(base, 1, 0, 2048, 16)]), 'parents')
+
+
+@gpu
+def test_reorder_states_that_lie_between_each_other():
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    g = _gen(6)
+    K, B = 3, 4
+    parents = torch.randint(0, K, (K, B), generator=g, dtype=torch.int32)
+    rows = _rows_of(parents)
+    pairs = torch.randn(2, K * B, 3, 5, generator=g)
+    got = pairs.to(dev)
+    P.reorder_states(parents.to(dev), [got[:, :, 0], got[:, :, 2]], 1)
+    want = pairs.clone()
+    want[:, :, 0] = pairs[:, rows, 0]
+    want[:, :, 2] = pairs[:, rows, 2]
+    assert torch.equal(got.cpu(), want)
+    halves = torch.randn(K * B, 10, generator=g)
+    got = halves.to(dev)
+    P.reorder_states(parents.to(dev), [got[:, 6:], got[:, :6]])
+    assert torch.equal(got.cpu(), halves[rows])
+    with pytest.raises(P._lib.PaccmannHipError, match='memory'):
+        P.reorder_states(parents.to(dev), [got[:, 5:], got[:, :6]])
+    square = torch.randn(K * B, K * B, device=dev)
+    with pytest.raises(TypeError, match='list'):
+        P.reorder_states(parents.to(dev), square)
