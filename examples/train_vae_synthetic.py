@@ -31,7 +31,9 @@ from paccmann_chemistry.models.vae import (  # noqa: E402
 from paccmann_chemistry.utils import (  # noqa: E402
     collate_fn, disable_rdkit_logging, get_device
 )
-from paccmann_chemistry.utils.hyperparams import SEARCH_FACTORY  # noqa: E402
+from paccmann_chemistry.utils.hyperparams import (  # noqa: E402
+    search_from_params
+)
 from pytoda.datasets import SMILESDataset  # noqa: E402
 from pytoda.smiles.smiles_language import SMILESLanguage  # noqa: E402
 
@@ -166,11 +168,7 @@ def main(argv=None):
     ).to(device)
     logger.info('Total # params: %d',
                 sum(p.numel() for p in gru_vae.parameters()))
-    search = SEARCH_FACTORY[params.get('decoder_search', 'sampling')](
-        temperature=params.get('temperature', 1.),
-        beam_width=params.get('beam_width', 3),
-        top_tokens=params.get('top_tokens', 5)
-    )
+    search = search_from_params(params)
     loss_tracker = {
         'test_loss_a': 10e4, 'test_rec_a': 10e4, 'test_kld_a': 10e4,
         'ep_loss': 0, 'ep_rec': 0, 'ep_kld': 0

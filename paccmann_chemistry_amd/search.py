@@ -166,8 +166,9 @@ class JointBeamSearch(Search):
     ends).  ``generate_from_latent`` runs it on the device
     (pcm_stackgru_generate_joint_beam); ``step`` is one selection."""
 
-    def __init__(self, beam_width: int = 3, temperature: float = 1.0):
-        super().__init__()
+    def __init__(self, beam_width: int = 3, temperature: float = 1.0, *args,
+                 **kwargs):
+        super().__init__(*args, **kwargs)
         self.beam_width = beam_width
         self.temperature = temperature
 
