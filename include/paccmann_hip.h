@@ -568,6 +568,17 @@ int pcm_stackgru_generate_joint_beam(
     int32_t end_token, int64_t *tokens_out, int64_t *beam_tokens_out,
     double *beam_scores_out, void *workspace, size_t workspace_bytes,
     int32_t *status, void *stream);
+/* The same with the end token in device memory, read there: one that is negative
+ * ends nothing, one that the vocabulary does not hold ends nothing and or-s
+ * PCM_STATUS_BAD_TOKEN into *status (nullable). */
+int pcm_stackgru_generate_joint_beam_until(
+    const pcm_dims *dims, const pcm_stackgru_params *weights,
+    const float *out_w, const float *out_b, const float *h0,
+    int64_t h0_layer_stride, const int64_t *prime, int32_t prime_len,
+    int32_t generate_len, int32_t beam_width, double temperature,
+    const int64_t *end_token, int64_t *tokens_out, int64_t *beam_tokens_out,
+    double *beam_scores_out, void *workspace, size_t workspace_bytes,
+    int32_t *status, void *stream);
 
 /* Optimiser ------------------------------------------------------------------*/
 

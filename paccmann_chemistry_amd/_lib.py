@@ -197,6 +197,12 @@ PROTOTYPES = {
             _F64, _I32, _VP, _VP, _VP, _VP, _SZ, _VP, _VP
         ]
     ),
+    'pcm_stackgru_generate_joint_beam_until': (
+        ctypes.c_int, [
+            _DIMS_P, _PARAMS_P, _VP, _VP, _VP, _I64, _VP, _I32, _I32, _I32,
+            _F64, _VP, _VP, _VP, _VP, _VP, _SZ, _VP, _VP
+        ]
+    ),
     'pcm_adam_step': (
         ctypes.c_int,
         [_VP, _VP, _VP, _VP, _I64, _F32, _F32, _F32, _F32, _I64, _F32, _VP]

@@ -1736,6 +1736,7 @@ struct BeamLayout {
     size_t off_jtok;       // int64[G][width][B]
     size_t off_jpar;       // int32[G][width][B]
     size_t off_jfin;       // uint8[2][width][B]
+    size_t off_jend;       // int32: the end token, if it is given on the device
     size_t off_jwork;      // pcm_beam_select's workspace
     size_t jwork_bytes;
     size_t total;          // floats
@@ -1761,6 +1762,7 @@ static int beam_layout(const pcm_dims *dims, int width, int generate_len,
         o->off_jtok = take(off, 2 * bw * g);
         o->off_jpar = take(off, bw * g);
         o->off_jfin = take(off, (2 * bw + 3) / 4);
+        o->off_jend = take(off, 1);
         o->jwork_bytes = pcm_beam_select_workspace_bytes(width, dims->batch,
                                                          dims->vocab, width);
         o->off_jwork = take(off, (o->jwork_bytes + 3) / 4);
@@ -1789,7 +1791,8 @@ size_t pcm_generate_beam_workspace_bytes(const pcm_dims *dims,
 // What the joint search does differently; null for the reference's search.
 struct JointSearch {
     double temperature;
-    int32_t end_token;   // < 0: beams do not end
+    int32_t end_token;       // < 0: beams do not end
+    const int64_t *end_in;   // the same on the device, or null
 };
 
 static int generate_beam(const pcm_dims *dims,
@@ -1870,7 +1873,8 @@ static int generate_beam(const pcm_dims *dims,
     if (joint) {
         jscores = (double *)(ws + bl.off_jscores);
         jfin = (uint8_t *)(ws + bl.off_jfin);
-        pcm_launch_beam_start(jscores, jfin, W, B, st);
+        pcm_launch_beam_start(jscores, jfin, W, B, joint->end_in, V,
+                              (int32_t *)(ws + bl.off_jend), status, st);
     } else {
         scores = (double *)(ws + bl.off_scores);
         hist_tok = (int32_t *)(ws + bl.off_hist_tok);
@@ -1916,12 +1920,14 @@ static int generate_beam(const pcm_dims *dims,
             const size_t in = (size_t)(gi & 1) * BW, out = (size_t)BW - in;
             int64_t *jtok = (int64_t *)(ws + bl.off_jtok) + (size_t)gi * BW;
             int32_t *jpar = (int32_t *)(ws + bl.off_jpar) + (size_t)gi * BW;
-            const bool ends = joint->end_token >= 0;
-            rc = pcm_beam_select(logits, PCM_DTYPE_F32, V, jscores + in,
-                                 ends ? jfin + in : nullptr, W, B, V, W,
-                                 joint->temperature, joint->end_token, jtok,
-                                 jpar, jscores + out, ends ? jfin + out : nullptr,
-                                 ws + bl.off_jwork, bl.jwork_bytes, st);
+            const bool ends = joint->end_in || joint->end_token >= 0;
+            rc = pcm_launch_beam_select(
+                logits, PCM_DTYPE_F32, V, jscores + in,
+                ends ? jfin + in : nullptr, W, B, V, W, joint->temperature,
+                joint->end_token,
+                joint->end_in ? (const int32_t *)(ws + bl.off_jend) : nullptr,
+                jtok, jpar, jscores + out, ends ? jfin + out : nullptr,
+                ws + bl.off_jwork, bl.jwork_bytes, st);
             if (rc) return rc;
             cur_tok = jtok;
             if (s + 1 == total_steps) continue;
@@ -1993,6 +1999,32 @@ size_t pcm_generate_joint_beam_workspace_bytes(const pcm_dims *dims,
     return bl.total * sizeof(float);
 }
 
+}  // extern "C"
+
+static int generate_joint_beam(
+    const pcm_dims *dims, const pcm_stackgru_params *weights,
+    const float *out_w, const float *out_b, const float *h0,
+    int64_t h0_layer_stride, const int64_t *prime, int32_t prime_len,
+    int32_t generate_len, int32_t beam_width, const JointSearch &joint,
+    int64_t *tokens_out, int64_t *beam_tokens_out, double *beam_scores_out,
+    void *workspace, size_t workspace_bytes, int32_t *status, void *stream) {
+    const double temperature = joint.temperature;
+    PCM_REQUIRE(dims && joint.end_token < dims->vocab, PCM_EINVAL,
+                "stackgru_generate_joint_beam: end_token %d outside the "
+                "vocabulary", joint.end_token);
+    PCM_REQUIRE(dims->vocab <= PCM_MAX_VOCAB, PCM_EINVAL,
+                "stackgru_generate_joint_beam: vocabulary %d > %d", dims->vocab,
+                PCM_MAX_VOCAB);
+    PCM_REQUIRE(temperature > 1e-30 && temperature < 1e30, PCM_EINVAL,
+                "stackgru_generate_joint_beam: temperature must be positive");
+    return generate_beam(dims, weights, out_w, out_b, h0, h0_layer_stride, prime,
+                         prime_len, generate_len, beam_width, 1, 1.0f,
+                         tokens_out, beam_tokens_out, beam_scores_out, workspace,
+                         workspace_bytes, status, stream, &joint);
+}
+
+extern "C" {
+
 int pcm_stackgru_generate_joint_beam(
     const pcm_dims *dims, const pcm_stackgru_params *weights,
     const float *out_w, const float *out_b, const float *h0,
@@ -2002,19 +2034,29 @@ int pcm_stackgru_generate_joint_beam(
     double *beam_scores_out, void *workspace, size_t workspace_bytes,
     int32_t *status, void *stream) {
     PCM_API_GUARD;
-    PCM_REQUIRE(dims && end_token < dims->vocab, PCM_EINVAL,
-                "stackgru_generate_joint_beam: end_token %d outside the "
-                "vocabulary", end_token);
-    PCM_REQUIRE(dims->vocab <= PCM_MAX_VOCAB, PCM_EINVAL,
-                "stackgru_generate_joint_beam: vocabulary %d > %d", dims->vocab,
-                PCM_MAX_VOCAB);
-    PCM_REQUIRE(temperature > 1e-30 && temperature < 1e30, PCM_EINVAL,
-                "stackgru_generate_joint_beam: temperature must be positive");
-    const JointSearch joint = {temperature, end_token};
-    return generate_beam(dims, weights, out_w, out_b, h0, h0_layer_stride, prime,
-                         prime_len, generate_len, beam_width, 1, 1.0f,
-                         tokens_out, beam_tokens_out, beam_scores_out, workspace,
-                         workspace_bytes, status, stream, &joint);
+    return generate_joint_beam(
+        dims, weights, out_w, out_b, h0, h0_layer_stride, prime, prime_len,
+        generate_len, beam_width, {temperature, end_token, nullptr}, tokens_out,
+        beam_tokens_out, beam_scores_out, workspace, workspace_bytes, status,
+        stream);
+}
+
+int pcm_stackgru_generate_joint_beam_until(
+    const pcm_dims *dims, const pcm_stackgru_params *weights,
+    const float *out_w, const float *out_b, const float *h0,
+    int64_t h0_layer_stride, const int64_t *prime, int32_t prime_len,
+    int32_t generate_len, int32_t beam_width, double temperature,
+    const int64_t *end_token, int64_t *tokens_out, int64_t *beam_tokens_out,
+    double *beam_scores_out, void *workspace, size_t workspace_bytes,
+    int32_t *status, void *stream) {
+    PCM_API_GUARD;
+    PCM_REQUIRE(end_token, PCM_EINVAL,
+                "stackgru_generate_joint_beam: null end token");
+    return generate_joint_beam(
+        dims, weights, out_w, out_b, h0, h0_layer_stride, prime, prime_len,
+        generate_len, beam_width, {temperature, -1, end_token}, tokens_out,
+        beam_tokens_out, beam_scores_out, workspace, workspace_bytes, status,
+        stream);
 }
 
 }  // extern "C"

@@ -697,6 +697,7 @@ struct BeamArgs {
     uint8_t *finished_out;
     long long ld;
     int beams, batch, V, width, parts, len, end;
+    const int32_t *end_at;   // the end token on the device, or null: end
     double inv_t;         // 1 / temperature
     double scale, least;  // log2(e) / temperature; the difference 2^-1000 is of
 };
@@ -737,12 +738,15 @@ __device__ __forceinline__ double beam_score(const BeamArgs &a, double score,
     return score + (((double)v - m) * a.inv_t - log_s);
 }
 
+__device__ __forceinline__ int end_token_of(const BeamArgs &a) {
+    return a.end_at ? *a.end_at : a.end;
+}
+
 // The j-th candidate of a beam that has ended: end_token, then the others, which are
 // -inf, in order; of one that holds no score all are, so all are in order.
-__device__ __forceinline__ int ended_token(const BeamArgs &a, int j,
-                                           double score) {
+__device__ __forceinline__ int ended_token(int end, int j, double score) {
     if (!(score > -INFINITY)) return j;
-    return j == 0 ? a.end : j - 1 + (j - 1 >= a.end ? 1 : 0);
+    return j == 0 ? end : j - 1 + (j - 1 >= end ? 1 : 0);
 }
 
 // Per beam row (or part of one): the `width` largest logits -- the row's
@@ -818,7 +822,8 @@ __global__ __launch_bounds__(NT, ONE ? 8 : 4) void beam_rows_kernel(BeamArgs a) 
 // row and mostly read the same entry.  An entry's flat place is 2 (beam V + token),
 // plus 1 if the beam had ended (a load of `finished` here would be 0.3 us more).
 __device__ __forceinline__ void beam_rank(const double *all_c, const int *all_f,
-                                          const BeamArgs &a, int rows, int b0) {
+                                          const BeamArgs &a, int end, int rows,
+                                          int b0) {
     const int W = a.width, n = a.beams * W;
     for (int at = threadIdx.x; at < rows * n; at += blockDim.x) {
         const int r = at / n, i = at - r * n, own = i / W;
@@ -842,7 +847,7 @@ __device__ __forceinline__ void beam_rank(const double *all_c, const int *all_f,
             a.parents[o] = from;
             a.scores_out[o] = mine;
             if (a.finished_out)
-                a.finished_out[o] = (flat & 1) || t == a.end;
+                a.finished_out[o] = (flat & 1) || t == end;
         }
     }
 }
@@ -857,7 +862,7 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
     __shared__ int s_f[PCM_BEAM_MAX * PCM_BEAM_MAX];
     const int lane = threadIdx.x & 63;
     const int k = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int b = blockIdx.x, W = a.width;
+    const int b = blockIdx.x, W = a.width, end = end_token_of(a);
     const long long row = (long long)k * a.batch + b;
     // everything a beam needs is asked for at once (rows that are not looked at
     // hold whatever the workspace held)
@@ -872,7 +877,7 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
     int tok = -1;
     double c = -INFINITY;
     if (done) {
-        tok = ended_token(a, lane, score);
+        tok = ended_token(end, lane, score);
         if (lane == 0 && score > -INFINITY) c = score;
     } else {
         const double m = score > -INFINITY ? wave_max(pm) : -INFINITY;
@@ -912,7 +917,7 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
             tok < a.V ? 2 * (k * a.V + tok) + (done ? 1 : 0) : 0x7fffffff;
     }
     __syncthreads();
-    beam_rank(s_c, s_f, a, 1, b);
+    beam_rank(s_c, s_f, a, end, 1, b);
 }
 
 // Short rows, everything in one launch: a block takes 64 / LPR batch rows, one
@@ -927,7 +932,7 @@ __global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
     int *beam_f = (int *)(beam_c + RB * per); // ... beam * V + token
     const int lane = threadIdx.x & 63, sub = lane % LPR, rb = lane / LPR;
     const int k = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int b = blockIdx.x * RB + rb;
+    const int b = blockIdx.x * RB + rb, end = end_token_of(a);
     if (b < a.batch) {
         const long long row = (long long)k * a.batch + b;
         const double score = a.scores[row];
@@ -968,7 +973,7 @@ __global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
                 int tok = j;   // a row without a distribution: tokens in order
                 double c = -INFINITY;
                 if (done) {
-                    tok = ended_token(a, j, score);
+                    tok = ended_token(end, j, score);
                     if (j == 0 && score > -INFINITY) c = score;
                 } else if (live) {
                     tok = top.l[j] > KEY_NONE ? key_index(top.l[j]) : a.V;
@@ -983,8 +988,8 @@ __global__ __launch_bounds__(1024) void beam_short_kernel(BeamArgs a) {
             }
     }
     __syncthreads();
-    beam_rank(beam_c, beam_f, a, min(RB, a.batch - (int)blockIdx.x * RB),
-              blockIdx.x * RB);
+    beam_rank(beam_c, beam_f, a, end,
+              min(RB, a.batch - (int)blockIdx.x * RB), blockIdx.x * RB);
 }
 
 // How a row of V logits is dealt out: `parts` blocks of `len` elements each.
@@ -1182,9 +1187,18 @@ __global__ __launch_bounds__(256) void reorder_kernel(ReorderArgs a) {
 // ---- joint beam search: first scores, final sequences -----------------------------
 __global__ __launch_bounds__(256) void beam_start_kernel(double *scores,
                                                          uint8_t *finished,
-                                                         int beams, int batch) {
+                                                         int beams, int batch,
+                                                         const int64_t *end_in,
+                                                         int vocab,
+                                                         int32_t *end_at,
+                                                         int32_t *status) {
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i >= beams * batch) return;
+    if (end_in && i == 0) {
+        const int64_t end = *end_in;
+        *end_at = end >= 0 && end < vocab ? (int32_t)end : -1;
+        if (end >= vocab && status) atomicOr(status, PCM_STATUS_BAD_TOKEN);
+    }
     scores[i] = i < batch ? 0. : -INFINITY;   // one beam to begin with
     finished[i] = 0;
 }
@@ -1210,9 +1224,11 @@ __global__ __launch_bounds__(256) void beam_trace_kernel(
 }  // namespace
 
 void pcm_launch_beam_start(double *scores, uint8_t *finished, int beams,
-                           int batch, hipStream_t st) {
+                           int batch, const int64_t *end_in, int vocab,
+                           int32_t *end_at, int32_t *status, hipStream_t st) {
     hipLaunchKernelGGL(beam_start_kernel, dim3((beams * batch + 255) / 256),
-                       dim3(256), 0, st, scores, finished, beams, batch);
+                       dim3(256), 0, st, scores, finished, beams, batch, end_in,
+                       vocab, end_at, status);
 }
 
 void pcm_launch_beam_trace(const int64_t *tokens, const int32_t *parents,
@@ -1304,14 +1320,16 @@ size_t pcm_beam_select_workspace_bytes(int32_t beams, int32_t batch,
     return rows * row_plan(rows, vocab, BEAM_SPLIT).parts * (width + 2) * sizeof(double);
 }
 
-int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
-                    const double *scores, const uint8_t *finished,
-                    int32_t beams, int32_t batch, int32_t vocab, int32_t width,
-                    double temperature, int32_t end_token, int64_t *tokens,
-                    int32_t *parents, double *scores_out,
-                    uint8_t *finished_out, void *workspace,
-                    size_t workspace_bytes, void *stream) {
-    PCM_API_GUARD;
+}  // extern "C"
+
+int pcm_launch_beam_select(const void *logits, int32_t dtype, int64_t ld,
+                           const double *scores, const uint8_t *finished,
+                           int32_t beams, int32_t batch, int32_t vocab,
+                           int32_t width, double temperature, int32_t end_token,
+                           const int32_t *end_at, int64_t *tokens,
+                           int32_t *parents, double *scores_out,
+                           uint8_t *finished_out, void *workspace,
+                           size_t workspace_bytes, hipStream_t st) {
     PCM_REQUIRE(logits && scores && tokens && parents && scores_out, PCM_EINVAL,
                 "beam_select: null pointer");
     PCM_REQUIRE(pcm_dtype_known(dtype), PCM_EINVAL,
@@ -1331,8 +1349,9 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
                 (long long)ld, vocab);
     PCM_REQUIRE(temperature > 1e-30 && temperature < 1e30, PCM_EINVAL,
                 "beam_select: temperature must be positive");
-    PCM_REQUIRE(!finished || (finished_out && end_token >= 0 &&
-                              end_token < vocab), PCM_EINVAL,
+    PCM_REQUIRE(!finished || (finished_out &&
+                              (end_at || (end_token >= 0 && end_token < vocab))),
+                PCM_EINVAL,
                 "beam_select: finished beams need finished_out and an end_token "
                 "in [0, %d), got %d", vocab, end_token);
     const size_t need =
@@ -1341,7 +1360,6 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
                 "beam_select: workspace %zu < %zu bytes", workspace_bytes, need);
     PCM_REQUIRE(((uintptr_t)workspace & 7) == 0, PCM_EINVAL,
                 "beam_select: workspace must be 8-byte aligned");
-    hipStream_t st = (hipStream_t)stream;
     const long long rows = (long long)beams * batch;
     const RowPlan plan = row_plan(rows, vocab, BEAM_SPLIT);
     PCM_REQUIRE(rows_fit(rows, vocab, width, plan), PCM_EINVAL,
@@ -1354,7 +1372,7 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
     a.tokens = tokens; a.parents = parents; a.scores_out = scores_out;
     a.finished_out = finished_out;
     a.ld = ld; a.beams = beams; a.batch = batch; a.V = vocab; a.width = width;
-    a.parts = plan.parts; a.len = plan.len; a.end = end_token;
+    a.parts = plan.parts; a.len = plan.len; a.end = end_token; a.end_at = end_at;
     a.inv_t = 1.0 / temperature;
     a.scale = 1.4426950408889634 / temperature;
     a.least = -1000. / a.scale;
@@ -1377,6 +1395,22 @@ int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
     hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)batch), dim3(64 * beams),
                        0, st, a);
     return pcm_check_launch("beam_select");
+}
+
+extern "C" {
+
+int pcm_beam_select(const void *logits, int32_t dtype, int64_t ld,
+                    const double *scores, const uint8_t *finished,
+                    int32_t beams, int32_t batch, int32_t vocab, int32_t width,
+                    double temperature, int32_t end_token, int64_t *tokens,
+                    int32_t *parents, double *scores_out,
+                    uint8_t *finished_out, void *workspace,
+                    size_t workspace_bytes, void *stream) {
+    PCM_API_GUARD;
+    return pcm_launch_beam_select(
+        logits, dtype, ld, scores, finished, beams, batch, vocab, width,
+        temperature, end_token, nullptr, tokens, parents, scores_out,
+        finished_out, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 int pcm_reorder_states(const int32_t *parents, int32_t beams, int32_t batch,

@@ -652,9 +652,10 @@ def stackgru_generate_joint_beam(
     dims, weights, out_w, out_b, h0, prime, generate_len, beam_width,
     temperature, end_token=None, want_beams=False, status=None
 ):
-    """pcm_stackgru_generate_joint_beam; h0 is [B,H] (broadcast) or [L,B,H].
-    Returns tokens i64[B, G] (the best beam of every row, without the prime),
-    and with ``want_beams`` also (beam tokens i64[B, width, G], scores
+    """pcm_stackgru_generate_joint_beam; h0 is [B,H] (broadcast) or [L,B,H],
+    ``end_token`` None, a number or a tensor of one (on the device it is read
+    there).  Returns tokens i64[B, G] (the best beam of every row, without the
+    prime), and with ``want_beams`` also (beam tokens i64[B, width, G], scores
     f64[B, width]), best first."""
     lib = load()
     require_device(h0, 'generate h0')
@@ -681,15 +682,23 @@ def stackgru_generate_joint_beam(
     work = torch.empty(nbytes // 4, dtype=torch.float32, device=dev)
     out_w = _f32(out_w, 'output_layer.weight').contiguous()
     out_b = _f32(out_b, 'output_layer.bias').contiguous()
+    call = lib.pcm_stackgru_generate_joint_beam
+    if end_token is None:
+        end = -1
+    elif torch.is_tensor(end_token) and end_token.is_cuda:
+        call = lib.pcm_stackgru_generate_joint_beam_until
+        end_token = end_token.reshape(-1)[0].to(device=dev, dtype=torch.int64)
+        end = end_token.data_ptr()
+    else:
+        end = int(torch.as_tensor(end_token).reshape(-1)[0])
     with _on(dev):
         check(
-            lib.pcm_stackgru_generate_joint_beam(
+            call(
                 ctypes.byref(dims), ctypes.byref(wstruct), ptr(out_w),
                 ptr(out_b), ptr(h0), h0_stride, ptr(prime), prime.numel(),
                 int(generate_len), int(beam_width), float(temperature),
-                -1 if end_token is None else int(end_token), ptr(tokens),
-                ptr(beams), ptr(scores), ptr(work), nbytes, ptr(status),
-                stream_ptr(dev)
+                end, ptr(tokens), ptr(beams), ptr(scores), ptr(work), nbytes,
+                ptr(status), stream_ptr(dev)
             ), 'pcm_stackgru_generate_joint_beam'
         )
     if want_beams:

@@ -348,16 +348,14 @@ class StackGRUDecoder(StackGRU):
         ``return_beams`` also every beam i64[B, width, generate_len] and its
         score f64[B, width], best first."""
         batch_size = latent_z.shape[1]
-        end = None
-        if end_token is not None:
-            end = int(torch.as_tensor(end_token).view(-1)[0])
         with torch.no_grad():
             hidden = self._latent_to_hidden(latent_z)
             return stackgru_generate_joint_beam(
                 self._dims(batch_size), self._weights(),
                 self.output_layer.weight, self.output_layer.bias, hidden,
                 prime_input.view(-1), generate_len, search.beam_width,
-                search.temperature, end_token=end, want_beams=return_beams,
+                search.temperature, end_token=end_token,
+                want_beams=return_beams,
                 status=self._status_word(hidden.device)
             )
 

@@ -1,6 +1,7 @@
 """What the entry points of top logits, distillation, beam selection and state
 reordering promise beside their numbers: what they refuse, what autograd is told,
 orders among equals, values bit for bit, the paths of the model around them."""
+import ctypes
 import json
 import math
 
@@ -8,8 +9,9 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from test_top_distill_beam import DTYPES, _check_beam, _dev, _gen, _host
-from test_top_distill_beam import _refused, _rows_of, gpu, ref_beam
+from test_top_distill_beam import DTYPES, PARAMS, _check_beam, _dev, _gen
+from test_top_distill_beam import _host, _refused, _rows_of, _vae, gpu
+from test_top_distill_beam import ref_beam
 
 
 def _bits(t):
@@ -85,8 +87,9 @@ def test_top_logits_refuses_temperatures_beyond_its_range():
 @gpu
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('rows,vocab,k', [
-    (3, 16, 16), (9000, 13, 13), (3, 60, 60), (9000, 60, 4), (9000, 700, 16), (3, 300, 20), (2, 5003, 40),
-    (2, 33001, 64), (1, 262144, 50)])
+    (3, 16, 16), (9000, 13, 13), (3, 60, 60), (9000, 60, 4),
+    (9000, 700, 16), (3, 300, 20), (2, 5003, 40), (2, 33001, 64),
+    (1, 262144, 50)])
 def test_top_logits_values_keep_their_bits(rows, vocab, k, dtype):
     """-0 and NaN come back as they are."""
     import paccmann_chemistry_amd as P
@@ -305,6 +308,65 @@ def test_every_search_comes_from_the_params():
     assert type(search_from_params({})) is P.SamplingSearch
     with pytest.raises(KeyError):
         search_from_params({'decoder_search': 'widest'})
+
+
+def test_generation_until_a_token_on_the_device_refusals():
+    from paccmann_chemistry_amd import _lib
+    lib = _lib.load()
+    dims = _lib.make_dims(4, 20, 20, 32, 2, 7, 5, True)
+    at, _keep = _host()
+    weights = _lib.PcmStackGRUParams()
+
+    def call(end=at, tau=1.0, width=3):
+        return lib.pcm_stackgru_generate_joint_beam_until(
+            ctypes.byref(dims), ctypes.byref(weights), at, at, None, 0, at, 1,
+            4, width, tau, end, at, None, None, at, 0, None, None)
+    _refused(lib, call(end=None), 'end token')
+    _refused(lib, call(tau=0.0), 'temperature')
+    _refused(lib, call(width=17), 'beam_width')
+
+
+@gpu
+def test_joint_beam_search_does_not_wait_for_the_device():
+    """An end token on the device is read there."""
+    import paccmann_chemistry_amd as P
+    vae, _ = _vae(PARAMS, 88)
+    vae.eval()
+    dev = _dev()
+    z = torch.randn(1, 21, 16, generator=_gen(3)).to(dev)
+    prime = torch.tensor([2, 7], device=dev)
+    search = P.JointBeamSearch(beam_width=3)
+
+    def run(end):
+        return vae.decoder.generate_from_latent(z, prime, end, search=search,
+                                                generate_len=12)
+    free = run(None).cpu()
+    first, second = int(free[0, 1]), int(free[5, 3])
+    want = {end: run(end) for end in (None, first, second)}
+    assert not torch.equal(want[first], want[None])
+    ends = {end: torch.tensor([end], device=dev) for end in (first, second)}
+    far = torch.tensor([99], device=dev)
+    vae.check_tokens()
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode('error')
+    try:
+        got = {end: run(t) for end, t in ends.items()}
+        lost = run(far)
+    finally:
+        torch.cuda.set_sync_debug_mode('default')
+    for end in ends:
+        assert torch.equal(got[end], want[end])
+    # a token that the vocabulary does not hold ends nothing, and is reported
+    assert torch.equal(lost, want[None])
+    with pytest.raises(RuntimeError, match='index out of range'):
+        vae.check_tokens()
+    batches = [torch.randn(1, 21, 16, generator=_gen(i)).to(dev)
+               for i in range(4)]
+    one = [vae.decoder.generate_from_latent(b, prime, first, search=search,
+                                            generate_len=7) for b in batches]
+    many = list(P.generate_batches(vae, batches, prime, ends[first],
+                                   generate_len=7, search=search))
+    assert all(torch.equal(a, b) for a, b in zip(one, many))
 
 
 def test_the_example_reads_the_search_from_its_params():
