@@ -3,6 +3,7 @@
 Same function names and arguments; TensorBoard / rdkit image logging (off the
 path, optional in the reference) is not carried over.
 """
+import contextlib
 import json
 import logging
 import os
@@ -135,6 +136,18 @@ def _reconstruction_example(outputs, target_seq, smiles_language):
     return to_text(target), to_text(pred)
 
 
+@contextlib.contextmanager
+def _evaluating(model):
+    """``model`` in eval mode; afterwards every module of it in its own again."""
+    modes = [(module, module.training) for module in model.modules()]
+    model.eval()
+    try:
+        yield
+    finally:
+        for module, mode in modes:
+            module.training = mode
+
+
 def train_vae(
     epoch, model, train_dataloader, val_dataloader, smiles_language,
     model_dir, search=SamplingSearch(), optimizer='adam', lr=1e-3,
@@ -163,7 +176,7 @@ def train_vae(
     vae_model = model.to(device)
     vae_model.train()
     if teacher is not None:
-        teacher = teacher.to(device).eval()
+        teacher = teacher.to(device)
     train_loss = 0
     if persistent_optimizer is not None:
         optimizer = persistent_optimizer
@@ -189,10 +202,11 @@ def train_vae(
                 encoder_seq, decoder_seq, target_seq
             )
         else:
+            with _evaluating(teacher):
+                top = teacher.teach(encoder_seq, decoder_seq, teacher_top,
+                                    teacher_temperature)
             decoder_loss, mu, logvar = vae_model.distill(
-                encoder_seq, decoder_seq, target_seq,
-                teacher.teach(encoder_seq, decoder_seq, teacher_top,
-                              teacher_temperature), hard_weight
+                encoder_seq, decoder_seq, target_seq, top, hard_weight
             )
         loss, kl_div = vae_loss_function(
             decoder_loss, mu, logvar, kl_growth=kl_growth, step=global_step

@@ -369,6 +369,58 @@ def test_joint_beam_search_does_not_wait_for_the_device():
     assert all(torch.equal(a, b) for a, b in zip(one, many))
 
 
+def _train(tmp_path, student, teacher, **more):
+    import logging
+    import os
+    from paccmann_chemistry_amd.training import train_vae
+    from paccmann_chemistry_amd.utils import collate_fn
+
+    class Language:
+        start_index, stop_index = 2, 3
+    g = _gen(21)
+    data = [torch.randint(4, 37, (int(n), ), generator=g)
+            for n in torch.randint(3, 12, (32, ), generator=g)]
+    loader = torch.utils.data.DataLoader(data, batch_size=8,
+                                         collate_fn=collate_fn, drop_last=True)
+    os.makedirs(tmp_path / 'weights', exist_ok=True)
+    train_vae(0, student, loader, loader, Language(), str(tmp_path),
+              log_interval=2, generate_len=6, batch_mode='packed',
+              logger=logging.getLogger('test'), teacher=teacher, teacher_top=4,
+              **more)
+
+
+@gpu
+def test_train_vae_leaves_the_teacher_as_it_was(tmp_path):
+    """It teaches in eval mode, and every module of it has its mode back."""
+    params = dict(PARAMS, batch_size=8, batch_mode='packed')
+    student, _ = _vae(params, 5, scale=0.1)
+    teacher, _ = _vae(params, 6)
+    teacher.train()
+    teacher.encoder.eval()
+    modes = {n: m.training for n, m in teacher.named_modules()}
+    seen = []
+    teach = teacher.teach
+
+    def watched(*args, **kwargs):
+        seen.append([m.training for m in teacher.modules()])
+        return teach(*args, **kwargs)
+    teacher.teach = watched
+    _train(tmp_path, student, teacher)
+    assert len(seen) == 4 and not any(any(s) for s in seen)
+    assert modes == {n: m.training for n, m in teacher.named_modules()}
+    # a student that is its own teacher goes on training
+    _train(tmp_path, student, student)
+    assert all(m.training for m in student.modules())
+    # and if teaching fails
+
+    def broken(*args, **kwargs):
+        raise KeyError('no teacher today')
+    teacher.teach = broken
+    with pytest.raises(KeyError):
+        _train(tmp_path, student, teacher)
+    assert modes == {n: m.training for n, m in teacher.named_modules()}
+
+
 def test_the_example_reads_the_search_from_its_params():
     """Its default params name a search that there is."""
     import os
