@@ -176,6 +176,12 @@ def train_vae(
     vae_model = model.to(device)
     vae_model.train()
     if teacher is not None:
+        if teacher.decoder.vocab_size != vae_model.decoder.vocab_size:
+            # (its token ids would be clamped, or mean other tokens)
+            raise ValueError(
+                f'the teacher has a vocabulary of {teacher.decoder.vocab_size}'
+                f', the model one of {vae_model.decoder.vocab_size}'
+            )
         teacher = teacher.to(device)
     train_loss = 0
     if persistent_optimizer is not None:

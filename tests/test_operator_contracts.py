@@ -421,6 +421,15 @@ def test_train_vae_leaves_the_teacher_as_it_was(tmp_path):
     assert modes == {n: m.training for n, m in teacher.named_modules()}
 
 
+@gpu
+def test_train_vae_refuses_a_teacher_of_another_vocabulary(tmp_path):
+    params = dict(PARAMS, batch_size=8, batch_mode='packed')
+    student, _ = _vae(params, 5, scale=0.1)
+    other, _ = _vae(dict(params, vocab_size=41, embedding_size=41), 6)
+    with pytest.raises(ValueError, match='vocabulary'):
+        _train(tmp_path, student, other)
+
+
 def test_the_example_reads_the_search_from_its_params():
     """Its default params name a search that there is."""
     import os
