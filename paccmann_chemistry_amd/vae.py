@@ -242,7 +242,7 @@ class StackGRUDecoder(StackGRU):
         )
         self.logits = logits.detach()
         # for monitoring, as in _decode
-        argmax = self.logits.argmax(-1).t()
+        argmax = top_logits(self.logits, 1).indices[..., 0].long().t()
         if lengths is not None:
             steps = torch.arange(tokens.shape[0], device=argmax.device)
             running = steps < lengths.to(argmax.device).view(-1, 1)

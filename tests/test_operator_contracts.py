@@ -430,6 +430,34 @@ def test_train_vae_refuses_a_teacher_of_another_vocabulary(tmp_path):
         _train(tmp_path, student, other)
 
 
+@gpu
+@pytest.mark.parametrize('mode', ['padded', 'packed'])
+def test_distill_step_reports_its_most_probable_tokens(mode, monkeypatch):
+    """``outputs`` is what a step on the targets alone leaves there, and comes
+    from this framework's kernels."""
+    params = dict(PARAMS, batch_size=6, batch_mode=mode)
+    student, _ = _vae(params, 5)
+    dev = _dev()
+    g = _gen(9)
+    lens = [9, 9, 7, 5, 2, 1]
+    seqs = [torch.randint(4, 37, (n, ), generator=g) for n in lens]
+    if mode == 'packed':
+        enc = torch.nn.utils.rnn.pack_sequence([s.to(dev) for s in seqs])
+    else:
+        enc = torch.nn.utils.rnn.pad_sequence(seqs).to(dev)
+    eps = torch.randn(6, 16, generator=g).to(dev)
+    student(enc, enc, enc, eps=eps)
+    want = student.decoder.outputs
+    top = student.teach(enc, enc, k=5, eps=eps)
+
+    def refused(*args, **kwargs):
+        raise AssertionError('a library reduction over the logits')
+    monkeypatch.setattr(torch.Tensor, 'argmax', refused)
+    student.distill(enc, enc, enc, top, eps=eps)
+    got = student.decoder.outputs
+    assert got.dtype == want.dtype and torch.equal(got, want)
+
+
 def test_the_example_reads_the_search_from_its_params():
     """Its default params name a search that there is."""
     import os
