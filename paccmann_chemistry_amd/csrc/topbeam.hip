@@ -702,14 +702,15 @@ struct BeamArgs {
     double scale, least;  // log2(e) / temperature; the difference 2^-1000 is of
 };
 
-// exp of logits relative to a maximum m (finite) in 64 bits, to 8e-13 of itself:
+// exp of logits relative to a maximum m (finite) in 64 bits, to a step of theirs:
 // beams compete by the difference of two log-sum-exps, for which 32 bits are too
 // few.  d = v - m first (of a product less a rounded product 3e38 times
 // temperature leaves 1e22, of either sign); what is below 2^-1000 counts as that.
 // d scale, rounded to the nearest integer n (by adding 1.5 * 2^52: n is then the
-// low word too), leaves at most 1/2, where the polynomial of degree 8 with the
-// least largest relative error (found by a Remez exchange) is off by 7.8e-13; n
-// goes into the exponent's bits.  Additions and fused multiplications only.
+// low word too), leaves at most 1/2, where the polynomial of degree 10 with the
+// least largest relative error (found by a Remez exchange) is off by 2.1e-16; n
+// goes into the exponent's bits.  Additions and fused multiplications only.  (Of
+// degree 8 it is off by 7.7e-13 and 1.1 us faster over 8 x 64 x 32000 logits.)
 struct Exp64 {
     double scale, least, m;
     __device__ __forceinline__ Exp64(const BeamArgs &a, float m_)
@@ -718,15 +719,17 @@ struct Exp64 {
         const double big = 6755399441055744.0;
         const double d = fmax((double)v - m, least);
         const double r = fma(d, scale, big), f = fma(d, scale, -(r - big));
-        double p = 1.3175858821424589139e-6;
-        p = fma(p, f, 0.000015309737294734560971);
-        p = fma(p, f, 0.00015403851744514194029);
-        p = fma(p, f, 0.0013333452062791777427);
-        p = fma(p, f, 0.009618128542870409837);
-        p = fma(p, f, 0.05550410939341089077);
-        p = fma(p, f, 0.24022650698880322565);
-        p = fma(p, f, 0.69314718054651433602);
-        p = fma(p, f, 0.9999999999997623493);
+        double p = 7.0372783532743875056e-9;
+        p = fma(p, f, 1.0208537941213722185e-7);
+        p = fma(p, f, 1.3215662838955003129e-6);
+        p = fma(p, f, 0.000015252658116348336923);
+        p = fma(p, f, 0.00015403529961120784315);
+        p = fma(p, f, 0.0013333558228561871466);
+        p = fma(p, f, 0.0096181291080346023214);
+        p = fma(p, f, 0.055504108664458830714);
+        p = fma(p, f, 0.24022650695908767754);
+        p = fma(p, f, 0.69314718055994977511);
+        p = fma(p, f, 1.0);
         return __hiloint2double(__double2hiint(p) + (__double2loint(r) << 20),
                                 __double2loint(p));
     }

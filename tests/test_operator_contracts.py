@@ -167,6 +167,38 @@ def test_beams_of_infinite_score(V, batch):
     assert bool((step.tokens.cpu()[9:] == torch.tensor([[0], [1], [2]])).all())
 
 
+@gpu
+@pytest.mark.parametrize('K,B,V', [(3, 40, 60), (5, 9, 128), (4, 9, 700),
+                                   (3, 4, 5003), (2, 3, 32000), (4, 1, 131071),
+                                   (2, 2, 200001)])
+@pytest.mark.parametrize('scale,tau', [(3.0, 1.0), (0.1, 0.7), (20.0, 2.5)])
+def test_beam_scores_have_the_bits_of_their_type(K, B, V, scale, tau):
+    """Sums of exponentials in 64 bits all the way.  With u half a step of
+    theirs, 2^-53, and D = (maximum - x) / tau: the exponent's factor and the
+    temperature's inverse are rounded (2 u D), the exponential is good to a step
+    and the remainder's rounding (4 u), a sum passes an element through 8 groups
+    of additions at most per 4096 (of a thread; 13 for those of a wave and the
+    waves, 64 parts); the score is a difference and a sum."""
+    import paccmann_chemistry_amd as P
+    g = _gen(K, B, V, scale * 10)
+    logits = torch.randn(K, B, V, generator=g) * scale
+    scores = -20 * torch.rand(K, B, generator=g, dtype=torch.float64)
+    step = P.beam_select(logits.to(_dev()), scores.to(_dev()), temperature=tau)
+    x = logits.double() / tau
+    far = x.amax(-1, keepdim=True) - x
+    lse = torch.logsumexp(x, -1)
+    rows = step.parents.cpu().long(), torch.arange(B).expand(K, B)
+    at = (*rows, step.tokens.cpu())
+    want = scores[rows] + (x[at] - lse[rows])
+    u = 2.0 ** -53
+    mean = ((x - lse[..., None]).exp() * far).sum(-1)[rows]
+    size = x.abs().amax(-1)[rows] + scores[rows].abs() + lse[rows].abs() + 20
+    tol = u * (2 * mean + 4 + 8 * max(4, V // 4096) + 13 + 64
+               + 2 * far[at] + 4 * size)
+    # (the comparison's own rounding is in the last term)
+    assert bool(((step.scores.cpu() - want).abs() <= tol).all())
+
+
 def test_launches_of_too_many_threads_are_refused():
     """A launch has less than 2^32 threads, those of its last block included."""
     from paccmann_chemistry_amd import _lib
