@@ -71,6 +71,29 @@ def test_distill_second_derivative_is_not_left_out(dtype):
     assert torch.equal(grad, want)
 
 
+def test_distill_grad_refusals():
+    """The gradient's own entry refuses what the loss's does."""
+    from paccmann_chemistry_amd import _lib
+    lib = _lib.load()
+    at, _keep = _host()
+
+    def call(logits=at, dtype=2, ld=20, k=3, targets=at, steps=2, vocab=20,
+             tau=1.0, hard=0.5, factor=at, dlogits=at, scratch=at):
+        return lib.pcm_distill_grad(
+            logits, dtype, ld, at, 0, at, None, k, targets, None, None, steps,
+            2, vocab, tau, hard, factor, dlogits, scratch, None)
+    for what in ('logits', 'factor', 'dlogits', 'scratch'):
+        _refused(lib, call(**{what: None}), 'null')
+    _refused(lib, call(dtype=3), 'dtype')
+    _refused(lib, call(steps=0), 'shape')
+    _refused(lib, call(vocab=(1 << 18) + 1, ld=1 << 20), 'shape')
+    _refused(lib, call(ld=19), 'row stride')
+    _refused(lib, call(k=65), 'k=65')
+    _refused(lib, call(tau=1e-4), 'temperature')
+    _refused(lib, call(hard=-0.5), 'hard_weight')
+    _refused(lib, call(targets=None), 'targets')
+
+
 # --------------------------------------------------------------------------
 # top logits
 # --------------------------------------------------------------------------
