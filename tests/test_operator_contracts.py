@@ -524,3 +524,85 @@ def test_the_example_reads_the_search_from_its_params():
     assert search_from_params(params).temperature == params['temperature']
     with open(os.path.join(ROOT, 'examples', 'train_vae_synthetic.py')) as fp:
         assert 'search_from_params(params)' in fp.read()
+
+
+# --------------------------------------------------------------------------
+# streams and graphs
+# --------------------------------------------------------------------------
+@gpu
+def test_split_rows_on_two_streams_and_captured():
+    """Long rows of few, whose parts meet in a workspace: at once on two streams,
+    and replayed from two graphs between eager calls."""
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    V = 150001
+
+    def inputs(i):
+        g = _gen(i, V)
+        return [torch.randn(3, 1, V, generator=g).half().to(dev),
+                (-torch.rand(3, 1, generator=g, dtype=torch.float64)).to(dev)]
+
+    def work(x, s):
+        top = P.top_logits(x, 40, 2.0)
+        step = P.beam_select(x, s, width=5, temperature=0.7)
+        return [top.values, top.indices, top.rest, *step[:3]]
+    want = [[t.clone() for t in work(*inputs(i))] for i in range(3)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    data = [inputs(i) for i in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for i in (0, 1, 2, 1, 0, 2):
+        with torch.cuda.stream(streams[len(got) % 2]):
+            got.append((i, work(*data[i])))
+    torch.cuda.synchronize()
+    for i, outs in got:
+        assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
+    held = [inputs(0), inputs(1)]
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for graph, h in zip(graphs, held):
+        with torch.cuda.graph(graph):
+            outs.append(work(*h))
+    for i in (2, 0, 1, 2):
+        for h, j in zip(held, (i, (i + 1) % 3)):
+            for t, new in zip(h, data[j]):
+                t.copy_(new)
+        graphs[0].replay()
+        eager = work(*data[i])
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for have, j in ((outs[0], i), (outs[1], (i + 1) % 3), (eager, i)):
+            assert all(torch.equal(a, b) for a, b in zip(have, want[j]))
+
+
+@gpu
+def test_joint_generation_captured():
+    """A whole generation in a graph, replayed for other latents and another end
+    token on the device."""
+    import paccmann_chemistry_amd as P
+    vae, _ = _vae(PARAMS, 88)
+    vae.eval()
+    dev = _dev()
+    prime = torch.tensor([2, 7], device=dev)
+    search = P.JointBeamSearch(beam_width=4, temperature=0.9)
+    z = torch.randn(1, 21, 16, generator=_gen(3)).to(dev)
+    end = torch.tensor([3], device=dev)
+    vae.decoder._update_batch_size(21)
+
+    def run(z, end):
+        return vae.decoder._generate_joint_beam(z, prime, end, search, 11,
+                                                return_beams=True)
+    run(z, end)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run(z, end)
+    for i, token in ((4, 3), (5, 9), (4, 9), (6, 3)):
+        new = torch.randn(1, 21, 16, generator=_gen(i)).to(dev)
+        z.copy_(new)
+        end.fill_(token)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, run(new, token)):
+            assert torch.equal(a, b)
+    vae.check_tokens()
