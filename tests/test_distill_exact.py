@@ -392,3 +392,54 @@ def test_distill_of_half_precision_on_a_side_stream_and_captured(V):
         eager = step(new.clone().requires_grad_(True))
         torch.cuda.synchronize()
         assert torch.equal(grad, eager)
+
+
+@gpu
+@pytest.mark.parametrize('V', [60, 900, 70001])
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('said', DTYPES)
+def test_distill_of_a_teacher_of_another_type(V, dtype, said):
+    import paccmann_chemistry_amd as P
+    g = _gen(V, 8)
+    logits, values, indices, rest = _case(2, 3, V, 7, dtype, 'normal', True, g)
+    values = values.to(said)
+    exact = Exact(logits, values, indices, rest, 2.0)
+    x = logits.to(_dev()).requires_grad_(True)
+    loss = P.distill_loss(x, _teacher(values, indices, rest, 2.0))
+    grad, = torch.autograd.grad(loss, x)
+    exact.check(loss.detach(), grad.cpu())
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_distill_offsets_beyond_32_bits(dtype):
+    """2.15e9 logits, of which the rows at the end take part: what they give by
+    themselves, and zeros before them."""
+    import paccmann_chemistry_amd as P
+    dev = _dev()
+    T, B, V, k = 2, 4100, 262144, 5
+    x = torch.empty(T, B, V, dtype=dtype, device=dev)
+    x.fill_(math.nan)
+    g = _gen(V)
+    mine = (torch.randn(T, 1, V, generator=g) * 3).to(dtype).to(dev)
+    x[:, -1:] = mine
+    places = torch.randint(0, V, (T, B, k), generator=g).int().to(dev)
+    values = torch.randn(T, B, k, generator=g).to(dev)
+    rest = torch.ones(T, B, device=dev)
+    targets = torch.randint(0, V, (T, B), generator=g).to(dev)
+    lengths = torch.zeros(B, dtype=torch.int32, device=dev)
+    lengths[-1] = T
+
+    def run(x, s):
+        x.requires_grad_(True)
+        teacher = P.TopLogits(values[:, s].contiguous(),
+                              places[:, s].contiguous(),
+                              rest[:, s].contiguous(), 2.0)
+        loss = P.distill_loss(x, teacher, targets=targets[:, s].contiguous(),
+                              lengths=lengths[s], hard_weight=0.25)
+        return loss.detach(), torch.autograd.grad(loss * 64, x)[0]
+    want, want_grad = run(mine, slice(B - 1, B))
+    loss, grad = run(x, slice(0, B))
+    assert torch.equal(loss, want)
+    assert torch.equal(grad[:, -1:], want_grad)
+    assert not bool(grad[0, :-1].any()) and not bool(grad[1, :-1].any())
