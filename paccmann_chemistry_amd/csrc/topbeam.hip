@@ -253,8 +253,9 @@ __device__ __forceinline__ double top_of_threads(
 // lanes' lists are merged pairwise; every lane ends with the row's list.  A row
 // of 60 costs about 40 instructions of a wave this way (16 rows in it) against
 // 800 for a wave per row.  All elements are ranked, -inf and NaN too.  Top 8 of
-// 61440 x 60 fp32: 11.7 us (70 for a wave per row), 18.9 MB at 1.6 TB/s: bound by
-// the comparators in 64 bits and, at four waves per SIMD, by waiting for the loads.
+// 61440 x 60 fp32: 11.6 us (70 for a wave per row), 18.9 MB at 1.6 TB/s: bound by
+// the comparators in 64 bits and, at four waves per SIMD, by waiting for the loads;
+// bf16 10.0, fp16 10.5.
 template <int KT> struct ShortTop {
     double l[KT];
     static __device__ __forceinline__ void order(double &a, double &b) {
@@ -461,11 +462,13 @@ __global__ __launch_bounds__(256) void top_short_kernel(TopArgs a, long long row
 // maximum; a wave takes the sums of the threads that hold listed elements again,
 // without those.  (The whole row's sum minus the listed ones' would lose what
 // the others are when the list holds nearly all of it.)
-// Top 32 of 1024 x 50021 bf16: 34 us (102.6 MB, 3.0 TB/s): 22 at the rate of a large
-// copy, then the selection, a chain of sorts and reads that all 1024 blocks are in
-// at once, being resident together (a sixth fewer instructions in it changed
-// nothing); k passes took 8.4 ms.  Top 64 of three rows of 131071 fp16: 8.6 us in 31
-// blocks a row, and 5.0 to join them: latency.
+// Top 32 of 1024 x 50021 bf16: 34 us (102.6 MB, 3.0 TB/s; 22 at the rate of a large
+// copy), bound by the issue of vector instructions, which have 0.81 of the slots:
+// 1526 per wave, about 700 of them in the pass (7 per element), the rest in the
+// selection and the second look; k passes took 8.4 ms.  (The holders' sums without
+// wave reductions, 250 instructions fewer, were level; why is not known.)  The same
+// in fp32: 50 us (4.1 TB/s), memory.  Top 64 of three rows of 131071 fp16: 8.4 to 9.6 us in
+// 31 blocks a row, and 4.9 to join them: latency.
 template <int DT, int NT, bool ONE>
 __global__ __launch_bounds__(NT, 8) void top_kernel(TopArgs a) {
     typedef RowType<DT> R;
@@ -754,9 +757,10 @@ __device__ __forceinline__ int ended_token(int end, int j, double score) {
 
 // Per beam row (or part of one): the `width` largest logits -- the row's
 // normaliser does not change their order -- and its maximum and sum, in one
-// pass.  8 x 64 rows of 32000 bf16: 23 us (26 MB; 17 operations in 64 bits per
-// element are 10 us of it, the first loads and the selection most of the rest);
-// four rows of 131071 in 31 blocks each: 7.3 us, latency.
+// pass.  8 x 64 rows of 32000 bf16: 24 us (26 MB; 19 operations in 64 bits per
+// element are 11 us of it, the first loads and the selection most of the rest);
+// four rows of 131071 in 31 blocks each: 7.5 us, latency.  5 x 256 rows of 129: 6.7 us,
+// of 700: 7.9 (latency), of 5003: 22, of 8192 bf16: 24.
 // (Long rows: 4 waves per SIMD, not 8, so that the eight exponentials in flight
 // stay in registers; it is bound by 64-bit arithmetic, not by latency.)
 template <int DT, int NT, bool ONE>
