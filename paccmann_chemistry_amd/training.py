@@ -253,6 +253,8 @@ def train_vae(
             # applied to the in-memory model, but nothing is saved from it.
             train_loss += pending.result()
             pending = None
+        if (saves or evaluates) and teacher is not None:
+            teacher.check_tokens()   # (nor from what a teacher made of such)
         if _iter and _iter % save_interval == 0:
             save_dir = os.path.join(
                 model_dir, f'weights/saved_model_epoch_{epoch}_iter_{_iter}.pt'
@@ -295,6 +297,8 @@ def train_vae(
     if pending is not None:
         # (a bad token in the last step raises here)
         train_loss += pending.result()
+    if teacher is not None:
+        teacher.check_tokens()
     if loss is not None:
         logger.info(
             f'Epoch {epoch} finished, \t Training Loss = {loss.item():.4f},'

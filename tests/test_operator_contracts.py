@@ -486,6 +486,26 @@ def test_train_vae_refuses_a_teacher_of_another_vocabulary(tmp_path):
 
 
 @gpu
+def test_train_vae_reports_what_its_teacher_saw(tmp_path):
+    """Token ids that the teacher's encoder does not hold raise, at a save before
+    anything is written."""
+    import os
+    import paccmann_chemistry_amd as P
+    params = dict(PARAMS, batch_size=8, batch_mode='packed')
+    student, _ = _vae(params, 5, scale=0.1)
+    small, _ = _vae(dict(params, vocab_size=20, embedding_size=20), 6)
+    whole, _ = _vae(params, 6)
+    teacher = P.TeacherVAE(small.encoder, whole.decoder)
+    with pytest.raises(RuntimeError, match='index out of range'):
+        _train(tmp_path, student, teacher)
+    with pytest.raises(RuntimeError, match='index out of range'):
+        _train(tmp_path, student, teacher, save_interval=2)
+    assert os.listdir(tmp_path / 'weights') == []
+    _train(tmp_path, student, whole, save_interval=2)
+    assert len(os.listdir(tmp_path / 'weights')) == 1
+
+
+@gpu
 @pytest.mark.parametrize('mode', ['padded', 'packed'])
 def test_distill_step_reports_its_most_probable_tokens(mode, monkeypatch):
     """``outputs`` is what a step on the targets alone leaves there, and comes
