@@ -3,7 +3,7 @@ kind "port") costs what the reference itself costs: one training step
 (forward + backward + Adam) of the configs[1] model at a bounded batch, timed
 for the imported reference (/root/reference, pytoda / rdkit stubbed as in
 make_golden.py) and for the oracle on the same weights, tokens and threads.
-Prints one line; the result is quoted in DESIGN.md.
+Prints one line.
 
     python oracle/time_vs_reference.py [batch]
 """

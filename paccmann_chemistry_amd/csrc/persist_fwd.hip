@@ -661,7 +661,7 @@ bool pcm_persist_fwd_supported(const SGLayout &lay, const int32_t *lengths) {
                        lay.B <= 8 * PROWS &&
                        LDS_FIXED_FLOATS + 4 * ((lay.DW + 3) & ~3) <= LDS_MAX_FLOATS;
     if (!shape) return false;
-    // Measured on MI355X at batch 512 (DESIGN.md): 48 us per step against 42.7 us
+    // Measured on MI355X at batch 512: 48 us per step against 42.7 us
     // for the launch chain, so the chain stays the default; PCM_PERSIST=1 selects
     // this kernel wherever the shape allows.
     return mode == 1;

@@ -45,7 +45,7 @@ def global_step_weights(lengths, steps, batch, device=None):
     reference's per-step cross-entropy mean (vae.py:343 padded, vae.py:386
     packed: the mean runs over the rows of the whole batch that are still
     active), when the batch is sharded over ranks.  One all-reduce of T counts
-    per step (SURVEY.md section 8e); a single process gets 1 / local counts.
+    per step; a single process gets 1 / local counts.
 
     lengths: per-row lengths of THIS rank's shard (None = padded mode, every
     row runs ``steps`` steps).  Padded mode: every rank must run the same

@@ -1,5 +1,5 @@
-"""Factories: same keys as the reference's ``utils/hyperparams.py``, and the search
-that a params file names."""
+"""Factories: same keys as the reference's ``utils/hyperparams.py``, and the
+search that a params file names."""
 import torch.optim as optim
 
 from .search import (
@@ -25,6 +25,7 @@ def search_from_params(params):
         beam_width=params.get('beam_width', 3),
         top_tokens=params.get('top_tokens', 5)
     )
+
 
 OPTIMIZER_FACTORY = {
     'adadelta': optim.Adadelta,

@@ -8,7 +8,7 @@ independent, and on MI355X a launch chain leaves the chip idle at every kernel
 boundary and in every kernel's prologue / epilogue; with two or three batches
 enqueued on separate streams those gaps are filled by another batch's MFMA
 loops (batch 4096: encoder-only 174 k -> 184 k molecules/s, greedy decode
-201 k -> 211 k over three streams, DESIGN.md section 5).  Results are the ones
+201 k -> 211 k over three streams).  Results are the ones
 the one-stream calls give, bit for bit.
 """
 import collections

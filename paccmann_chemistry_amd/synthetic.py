@@ -1,12 +1,12 @@
 """Deterministic synthetic weights and SMILES-shaped token batches.
 
 Input synthesis for benchmarks, examples and tests (no arithmetic of the hot
-path lives here): the workloads of SURVEY.md section 8d are regenerated from a
+path lives here): the benchmarks' workloads are regenerated from a
 numpy seed wherever they are needed, so that config-shaped fixtures need not
 store 22 MB of weights.
 
 State-dict layout follows the reference (``stack_rnn.py:68-105``,
-``vae.py:54-61,283-286``; key list in SURVEY.md section 8b).
+``vae.py:54-61,283-286``).
 """
 import numpy as np
 import torch
@@ -75,7 +75,7 @@ def make_state_dict(p, seed, scale=None, dtype=torch.float32):
 
 
 def synthetic_tokens(seq_len, batch, vocab, seed, lengths=None):
-    """SMILES-shaped batch (SURVEY.md section 8d): START(2) first, tokens
+    """SMILES-shaped batch: START(2) first, tokens
     uniform in [4, V), STOP(3) at len-1, PAD(0) after.  Returns i64[T,B]."""
     rng = np.random.default_rng(seed)
     toks = rng.integers(4, vocab, size=(seq_len, batch), dtype=np.int64)
