@@ -102,11 +102,13 @@ __device__ __forceinline__ float uniform(float v) {
     return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
 }
 
-// p (log p - log q) + q - p of an outcome, d = log q - log p.  (Below 1e-30 p has
-// lost digits, and what it adds to q is nothing unless q is 0.)
-__device__ __forceinline__ float kl_term(float p, double d, float q) {
-    if (!(p <= 1e-30f)) return (float)((double)p * (expm1(d) - d));
-    return p == 0.f ? q : (float)((double)q - (double)p * (1. + d));
+// c (p (log p - log q) + q - p) of an outcome, d = log q - log p.  (Below 1e-30 p
+// has lost digits, and what it adds to q is nothing unless q is 0.  The row's factor c
+// goes in before 64 bits become 32: masks of the type's lowest value have parts
+// that leave them where the loss does not.)
+__device__ __forceinline__ float kl_term(float p, double d, float q, double c) {
+    if (!(p <= 1e-30f)) return (float)(c * ((double)p * (expm1(d) - d)));
+    return (float)(c * (p == 0.f ? (double)q : (double)q - (double)p * (1. + d)));
 }
 
 // probability of the outcome "any other token".  (Where none is left mo is not a
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
     if (!a.rowloss) return;
     float loss = 0.f;
     if (live && taught) {
-        const double c = (double)uo + logf(us / st.sa);
+        const double c = (double)uo + logf(us / st.sa), soft = (double)a.soft * w;
         // (entry k: any other token)
         for (int j = sub; j <= k; j += LPR) {
             const bool other = j == k;
@@ -359,14 +361,13 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
                                     : (double)u[j] * a.inv_t64);
             const float q = other ? other_q(mo, s, st.ma, st.sa, a.scale)
                                   : exp_below(at, st.ma, a.scale) / st.sa;
-            if (idx != -1 || p != p) loss += kl_term(p, d, q);
-            if (idx < -1) loss -= q;
+            if (idx != -1 || p != p) loss += kl_term(p, d, q, soft);
+            if (idx < -1) loss -= (float)(q * soft);
         }
-        loss *= a.soft;
     }
     if (HARD && live && sub == 0)
-        loss += a.hard * (logf(st.ha) - (xt - st.ma));
-    loss = wave_sum(live ? loss * w : 0.f);
+        loss += a.hard * w * (logf(st.ha) - (xt - st.ma));
+    loss = wave_sum(loss);
     if (lane == 0) a.rowloss[blockIdx.x] = loss;
 }
 
@@ -616,22 +617,22 @@ distill_row_kernel(DistillArgs a) {
         float loss = 0.f;
         if (taught) {
             const float us = s_list[5], uo = s_list[6], rest = s_list[7];
-            const double c = (double)uo + logf(us / st.sa);
+            const double c = (double)uo + logf(us / st.sa), soft = (double)a.soft * w;
             const float p = w_p[lane], at = w_x[lane];
             const float q = exp_below(at, st.ma, a.scale) / st.sa;
             const int li = w_idx[lane];
             if (li != -1 || p != p)
                 loss = kl_term(p, ((double)at - st.ma) * a.inv_t64 + c -
-                                      (double)w_value[lane] * a.inv_t64, q);
-            if (li < -1) loss -= q;
+                                      (double)w_value[lane] * a.inv_t64, q, soft);
+            if (li < -1) loss -= (float)(q * soft);
             if (lane == 0)
                 loss += kl_term(pr, ((double)mo - st.ma) * a.inv_t64 + c -
                                         (rest - log((double)s)),
-                                other_q(mo, s, st.ma, st.sa, a.scale));
-            loss = a.soft * wave_sum(loss);
+                                other_q(mo, s, st.ma, st.sa, a.scale), soft);
+            loss = wave_sum(loss);
         }
-        if (HARD) loss += a.hard * (logf(st.ha) - (s_list[8] - st.ma));
-        if (lane == 0) a.rowloss[row] = loss * w;
+        if (HARD) loss += a.hard * w * (logf(st.ha) - (s_list[8] - st.ma));
+        if (lane == 0) a.rowloss[row] = loss;
     };
     if (!dl) {
         if (tid >= NT - 64) row_loss();
