@@ -2,8 +2,8 @@
 // its gradient with respect to the student's logits.
 //
 // A row is compared over k + 1 outcomes, the listed tokens and "any other".
-// With x = logits / tau, R = lse of the x that are not listed and Z = lse of
-// all:
+// With u = the teacher's values / tau, N = lse of these and the rest, x = logits / tau,
+// R = lse of the x that are not listed and Z = lse of all:
 //   row = sum_j p_j (u_j - N - x_j + Z) + p_rest (rest - N - R + Z)
 //   d row / d x_v = q_v - p_v (listed),  q_v (1 - p_rest / q_rest) (other)
 // R is summed over the other tokens themselves and Z joined from R and the
@@ -38,7 +38,7 @@ struct DistillArgs {
     int B, V, k, values_dtype;
     float weight_all;
     double inv_t64;        // 1 / tau
-    float inv_t, scale;    // the same; log2(e) / tau
+    float scale;           // log2(e) / tau
     float soft, hard;      // (1 - hard) tau^2; hard
     float dsoft;           // (1 - hard) tau
 };
@@ -117,6 +117,35 @@ __device__ __forceinline__ float other_q(float mo, float s, float ma, float sa,
                                          float scale) {
     return s == 0.f ? 0.f : exp_below(mo, ma, scale) * s / sa;
 }
+
+// A teacher's outcomes relative to its largest listed value v0 (0 if it lists none):
+// differences of values before the product with 1 / tau, so that neither a list far
+// from 0 nor one of nothing but the type's lowest value loses digits or range.
+// The rest, which is at the temperature already, is relative to it in 64 bits; h,
+// not below 0 if anything is listed, is the largest of both.
+struct Teacher {
+    float v0, hl;     // hl: h log2(e)
+    double rb, h;     // the rest, relative
+    __device__ __forceinline__ Teacher(const DistillArgs &a, float vmax, float rest) {
+        v0 = finite_or_0(vmax);
+        rb = rest - (double)v0 * a.inv_t64;
+        h = fmax(rb, vmax > -INFINITY ? 0. : rb);
+        if (h == -INFINITY) h = 0.;
+        hl = (float)(h * 1.4426950408889634);
+    }
+    __device__ __forceinline__ float listed(const DistillArgs &a, float v) const {
+        return __builtin_amdgcn_exp2f(fmaf(v - v0, a.scale, -hl));
+    }
+    __device__ __forceinline__ float other() const {
+        return __builtin_amdgcn_exp2f((float)((rb - h) * 1.4426950408889634));
+    }
+    // log of the same
+    __device__ __forceinline__ double log_listed(const DistillArgs &a,
+                                                 float v) const {
+        return ((double)v - v0) * a.inv_t64 - h;
+    }
+    __device__ __forceinline__ double log_other() const { return rb - h; }
+};
 
 // What a row's factors are made of: the others' maximum m and sum(s), the listed
 // tokens' xm and sums, the teacher's; w: the weight of its gradient.  (Sums relative
@@ -204,13 +233,13 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
             }
     }
     __syncthreads();
-    float xt = 0.f, um = rest;
+    float xt = 0.f, um = -INFINITY;
     int flags = rest != rest ? 1 : 0;   // 1: a NaN; 2: an index twice
     if (live) {
         if (HARD) xt = tile[tg];
         for (int j = sub; j < k; j += LPR) {
             const int idx = li[j];
-            um = fmaxf(um, u[j] * a.inv_t);
+            um = fmaxf(um, u[j]);
             if (u[j] != u[j]) flags |= 1;
             lx[j] = idx < 0 ? -INFINITY : tile[idx];
             if (idx >= 0) {
@@ -237,17 +266,18 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
                 }
     __syncthreads();
     // teacher, and the listed tokens' part of the student
-    const bool taught = a.soft > 0.f && (um > -INFINITY || (flags & 1));
-    const float uo = finite_or_0(um);
+    const bool taught =
+        a.soft > 0.f && (um > -INFINITY || rest > -INFINITY || (flags & 1));
+    const Teacher said(a, um, rest);
     float us = 0.f, xm = -INFINITY;
     if (live)
         for (int j = sub; j < k; j += LPR) {
-            us += __builtin_amdgcn_exp2f((u[j] * a.inv_t - uo) * LOG2E);
+            us += said.listed(a, u[j]);
             if (li[j] >= 0) xm = fmaxf(xm, lx[j]);
         }
     us = row_sum<LPR>(us);
     xm = row_max<LPR>(xm);
-    const float ro = __builtin_amdgcn_exp2f((rest - uo) * LOG2E);
+    const float ro = said.other();
     us += ro;
     const float ius = 1.f / us, pr = taught ? ro * ius : 0.f;
     const float xo = finite_or_0(xm);
@@ -290,9 +320,7 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
     s = row_sum<LPR>(s);
     if (HARD) h = row_sum<LPR>(h);
     const RowStats st = row_stats(a, wg, m, s, h, xm, xs, xh, taught, pr);
-    auto teacher_p = [&](int j) {
-        return __builtin_amdgcn_exp2f((u[j] * a.inv_t - uo) * LOG2E) * ius;
-    };
+    auto teacher_p = [&](int j) { return said.listed(a, u[j]) * ius; };
     // gradients: the others', the listed ones', the target's
     if (a.dlogits) {
         if (live) {
@@ -350,15 +378,15 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
     if (!a.rowloss) return;
     float loss = 0.f;
     if (live && taught) {
-        const double c = (double)uo + logf(us / st.sa), soft = (double)a.soft * w;
+        const double c = logf(us / st.sa), soft = (double)a.soft * w;
         // (entry k: any other token)
         for (int j = sub; j <= k; j += LPR) {
             const bool other = j == k;
             const int idx = other ? 0 : li[j];
             const float p = other ? pr : teacher_p(j), at = other ? mo : lx[j];
             const double d = ((double)at - st.ma) * a.inv_t64 + c -
-                             (other ? rest - log((double)s)
-                                    : (double)u[j] * a.inv_t64);
+                             (other ? said.log_other() - log((double)s)
+                                    : said.log_listed(a, u[j]));
             const float q = other ? other_q(mo, s, st.ma, st.sa, a.scale)
                                   : exp_below(at, st.ma, a.scale) / st.sa;
             if (idx != -1 || p != p) loss += kl_term(p, d, q, soft);
@@ -391,7 +419,9 @@ distill_row_kernel(DistillArgs a) {
     typedef typename R::T T;
     extern __shared__ __align__(16) unsigned marks[];   // a bit per element
     __shared__ float red[NT / 64], red2[NT / 64];
-    __shared__ float s_list[9];
+    __shared__ float s_list[8];
+    __shared__ double s_other;   // log of the other's p, not normalised; h
+    __shared__ double s_high;
     // what wave 0 needs of its list after the passes (registers are the row's)
     __shared__ int w_idx[64];
     __shared__ float w_x[64], w_p[64], w_value[64], w_mass[64];
@@ -527,12 +557,12 @@ distill_row_kernel(DistillArgs a) {
             }
             first = idx >= 0 && !again;
         }
-        const float u = value * a.inv_t, um = wave_max(fmaxf(u, rest));
-        const bool bad = __any(u != u || rest != rest);
-        const bool taught = a.soft > 0.f && (um > -INFINITY || bad);
-        const float uo = finite_or_0(um);
-        const float e = __builtin_amdgcn_exp2f((u - uo) * LOG2E);
-        const float ro = __builtin_amdgcn_exp2f((rest - uo) * LOG2E);
+        const float um = wave_max(value);
+        const bool bad = __any(value != value || rest != rest);
+        const bool taught =
+            a.soft > 0.f && (um > -INFINITY || rest > -INFINITY || bad);
+        const Teacher said(a, um, rest);
+        const float e = said.listed(a, value), ro = said.other();
         const float us = wave_sum(e) + ro;
         if (taught) p = e / us;
         mass = p;
@@ -557,9 +587,10 @@ distill_row_kernel(DistillArgs a) {
         w_mass[lane] = mass;
         if (lane == 0) {
             s_list[5] = us;
-            s_list[6] = uo;
-            s_list[7] = rest;
-            s_list[8] = xt;
+            s_list[6] = said.v0;
+            s_list[7] = xt;
+            s_other = said.log_other();
+            s_high = said.h;
             s_list[0] = xm;
             s_list[1] = xs;
             s_list[2] = xh;
@@ -616,22 +647,22 @@ distill_row_kernel(DistillArgs a) {
         if (!a.rowloss) return;
         float loss = 0.f;
         if (taught) {
-            const float us = s_list[5], uo = s_list[6], rest = s_list[7];
-            const double c = (double)uo + logf(us / st.sa), soft = (double)a.soft * w;
+            const double c = logf(s_list[5] / st.sa), soft = (double)a.soft * w;
             const float p = w_p[lane], at = w_x[lane];
             const float q = exp_below(at, st.ma, a.scale) / st.sa;
             const int li = w_idx[lane];
             if (li != -1 || p != p)
                 loss = kl_term(p, ((double)at - st.ma) * a.inv_t64 + c -
-                                      (double)w_value[lane] * a.inv_t64, q, soft);
+                                      (((double)w_value[lane] - s_list[6]) *
+                                           a.inv_t64 - s_high), q, soft);
             if (li < -1) loss -= (float)(q * soft);
             if (lane == 0)
                 loss += kl_term(pr, ((double)mo - st.ma) * a.inv_t64 + c -
-                                        (rest - log((double)s)),
+                                        (s_other - log((double)s)),
                                 other_q(mo, s, st.ma, st.sa, a.scale), soft);
             loss = wave_sum(loss);
         }
-        if (HARD) loss += a.hard * w * (logf(st.ha) - (s_list[8] - st.ma));
+        if (HARD) loss += a.hard * w * (logf(st.ha) - (s_list[7] - st.ma));
         if (lane == 0) a.rowloss[row] = loss;
     };
     if (!dl) {
@@ -851,7 +882,6 @@ static int distill(const void *logits, int32_t dtype, int64_t ld,
     a.weight = step_weight;
     a.weight_all = 1.0f / (float)batch;
     a.inv_t64 = 1.0 / temperature;
-    a.inv_t = (float)a.inv_t64;
     a.scale = (float)(1.4426950408889634 / temperature);
     a.soft = (float)((1.0 - hard_weight) * temperature * temperature);
     a.dsoft = (float)((1.0 - hard_weight) * temperature);

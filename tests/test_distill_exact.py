@@ -78,11 +78,14 @@ class Exact:
         adds = _additions(vocab)
         sums = EPS * (adds + 4 + 4 * (q * far).sum(-1, keepdim=True) +
                       4 * (others * far).sum(-1, keepdim=True))
-        live = torch.where(torch.isfinite(u), u, 0.0).abs().amax(-1)
-        said = EPS * (2 * (live + last.nan_to_num(0, 0, 0).abs()) + 4 * live +
-                      64 + 16)[..., None]
+        # (the teacher's exponents: of differences too, those that count)
+        wide = (p * torch.where(p > 0, top_u + n - u, 0.0)).sum(-1)
+        said = EPS * (8 * wide + 64 + 16)[..., None]
         own = EPS * (4 * far + 8)
-        self.grad_tol = soft * ((own + sums) * q +
+        each = torch.zeros_like(x).scatter_add_(-1, at, torch.where(
+            there, 4 * EPS * (p * torch.where(p > 0, top_u + n - u, 0.0))
+            [..., :-1], 0.0))
+        self.grad_tol = soft * ((own + sums) * q + each +
                                 (own + sums + said) * teacher)
         # What moves every d = log q - log p by the same is met by sum (q - p) = 0
         # but for the roundings; the rest is relative to the terms, which are not
@@ -477,3 +480,47 @@ def test_distill_of_a_loss_in_range_whose_parts_are_not(V, dtype):
     assert abs(float(loss.detach()) - float(exact.loss)) <= \
         1e-5 * float(exact.loss)
     assert bool(exact.fine(grad.cpu()).all())
+
+
+@gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('tau', [0.02, 0.7, 1.0, 3.0, 900.0])
+@pytest.mark.parametrize('V', [20, 400, 900, 5000, 70001])
+def test_distill_of_teachers_that_are_far_away(V, tau, dtype):
+    """Lists of nothing but the type's lowest value (uniform), with the others at
+    -inf, absent or finite; lists near the largest one, and far below their
+    rest; what counts is differences."""
+    import paccmann_chemistry_amd as P
+    g = _gen(V, 78)
+    T, B, k = 2, 5, 7
+    logits = torch.randn(T, B, V, generator=g).to(dtype)
+    indices = torch.rand(T, B, V, generator=g).topk(k, -1).indices.int()
+    values = torch.randn(T, B, k, generator=g) * min(tau, 30.0)
+    low = torch.finfo(dtype).min
+    rest = torch.full((T, B), -math.inf)
+    values[0, 0] = low
+    values[0, 1] = low
+    rest[0, 1] = -2.0
+    values[0, 2, 1:] = low
+    values[0, 3] = low
+    indices[0, 3, 3:] = -1
+    values[0, 4] = -low          # all of them at the largest value
+    values[1, 0, 3] = -low       # one
+    values[1, 1] += 1e4          # (in 32 bits to 1e-3)
+    rest[1, 1] = 1e4 / tau
+    values[1, 2] -= 1e4
+    rest[1, 3] = 88.0
+    values[1, 4] = -math.inf
+    rest[1, 4] = -1e30
+    values = values.to(dtype)
+    targets = torch.randint(0, V, (T, B), generator=g)
+    exact = Exact(logits, values, indices, rest, tau, targets, None, 0.25)
+    assert math.isfinite(float(exact.loss))
+    x = logits.to(_dev()).requires_grad_(True)
+    for r in (rest, None):
+        if r is None:
+            exact = Exact(logits, values, indices, r, tau, targets, None, 0.25)
+        loss = P.distill_loss(x, _teacher(values, indices, r, tau),
+                              targets=targets.to(_dev()), hard_weight=0.25)
+        grad, = torch.autograd.grad(loss, x)
+        exact.check(loss.detach(), grad.cpu())
