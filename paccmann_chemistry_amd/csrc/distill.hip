@@ -188,9 +188,9 @@ __device__ __forceinline__ RowStats row_stats(const DistillArgs &a, float w,
 // with a wave per row.  The row is in registers; a copy in LDS is where the
 // listed tokens are looked up, and where the gradients meet: of the others from the
 // registers, of the listed ones and the target from their entries.
-// 61440 ragged x 60 fp32, k = 8, with targets: 18.7 us for 24.6 MB (1.3 TB/s), bound
+// 61440 ragged x 60 fp32, k = 8, with targets: 18.9 us for 24.6 MB (1.3 TB/s), bound
 // by the instructions and LDS accesses of the lists (2.5 us of it are the loss's 64
-// bits); a wave per row took 201 us.  fp16, the loss alone 13 us, the gradient 14.5.
+// bits); a wave per row took 201 us.  fp16, the loss alone 13.5 us, the gradient 15.
 template <int DT, int LPR, int G, bool HARD>
 __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
     typedef RowType<DT> R;
@@ -405,9 +405,9 @@ __global__ __launch_bounds__(64) void distill_short_kernel(DistillArgs a) {
 // listed tokens are marked in a bitmap in LDS -- a group of eight elements is one
 // byte of it -- and become -inf in the registers, so the passes see the others
 // only.  What bounds it is memory, as long as two blocks fit a CU and one loads
-// while the other computes: 2048 x 32000 bf16 in 59 us (4.5 TB/s; a large copy
-// reaches 4.7), fp16 in 47 (the loss alone, vector units 0.87) and 55 (the gradient);
-// 1024 ragged x 50021 fp32 with targets in 86 us (3.6 TB/s: at most four rows per CU,
+// while the other computes: 2048 x 32000 bf16 in 60 us (4.4 TB/s; a large copy
+// reaches 4.7), fp16 in 47 (the loss alone, vector units 0.87) and 54 (the gradient);
+// 1024 ragged x 50021 fp32 with targets in 85 us (3.6 TB/s: at most four rows per CU,
 // so two turns of loads with little to hide behind); 7 x 601 fp16 in 5.2 us (latency).
 // LG: up to so many more groups of a thread are kept in LDS, in the threads' order
 // (each thread reads what it wrote: no barrier).
